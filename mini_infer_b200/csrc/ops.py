@@ -436,7 +436,25 @@ def _sig_attention_stage(lib: ctypes.CDLL) -> None:
                                     c_float, c_int, c_void_p]
 
 
+def _sig_adapters(lib: ctypes.CDLL) -> None:
+    ll = ctypes.c_longlong
+    lib.mi_adapter_add.argtypes = [c_void_p, ll, c_void_p, ll, c_void_p, c_void_p, c_void_p, ll, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                   c_int, c_void_p]
+
+
+def _sig_logits(lib: ctypes.CDLL) -> None:
+    ll = ctypes.c_longlong
+    lib.mi_adjust_logits.argtypes = [c_void_p, ll, c_void_p, ll, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                     c_void_p]
+    lib.mi_record_tokens.argtypes = [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                     c_int, c_void_p]
+
+
 _SIGNATURES = {
+    "adapters": _sig_adapters,
+    "logits": _sig_logits,
     "attention_stage": _sig_attention_stage,
     "attention_rows": _sig_attention_rows,
     "depth": _sig_depth,
@@ -2937,3 +2955,245 @@ def branch_norm_then_norm(stream: torch.Tensor, branch: torch.Tensor, gain_y: to
                                       _code(dtype), _stream())
     _finish(lib, rc, "norms")
     return out
+
+
+# --------------------------------------------------------------------------------------- what a request brings of its own
+
+
+def _same_device(what: str, *tensors: torch.Tensor | None) -> None:
+    """Every tensor on the current CUDA device: the kernels are launched on its current stream."""
+    here = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError(f"{what}: kernels run on CUDA tensors only (got a tensor on {t.device})")
+        if here is None:
+            here = torch._C._cuda_getDevice()
+        if t.get_device() != here:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The bytes from a matrix's first to its last element."""
+    first = t.data_ptr()
+    if t.numel() == 0:
+        return first, first
+    return first, first + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size()
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0
+
+
+def _vector(what: str, name: str, t: torch.Tensor | None, dtype: torch.dtype, n: int) -> None:
+    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous()):
+        raise KernelError(f"{what}: {name} must be a contiguous {dtype} vector of {n}")
+
+
+ADAPTER_MAX_PARTS = 4
+
+
+class AdapterPlan:
+    """Which of ``adapters`` low-rank adapters each row of a step uses (``ids``), prepared for ``adapter_add``: made once a
+    step by ``adapter_plan`` and handed to every projection."""
+
+    __slots__ = ("ids", "rows", "adapters")
+
+    def __init__(self, ids: torch.Tensor, adapters: int) -> None:
+        self.ids, self.rows, self.adapters = ids, ids.shape[0], adapters
+
+
+def adapter_plan(ids: torch.Tensor, adapters: int) -> AdapterPlan:
+    """``ids`` int32 ``[M]``: the adapter of each row, in any order; a number outside ``[0, adapters)`` is none."""
+    if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous():
+        raise KernelError("adapter_plan: ids must be a contiguous int32 vector")
+    if adapters < 0:
+        raise KernelError(f"adapter_plan: {adapters} adapters")
+    _same_device("adapter_plan", ids)
+    return AdapterPlan(ids, int(adapters))
+
+
+def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: AdapterPlan, *,
+                scale: torch.Tensor | None = None, ranks: torch.Tensor | None = None, parts: tuple[int, ...] | None = None,
+                pairs: bool = False, out: torch.Tensor | None = None, w_constant: bool = False) -> torch.Tensor:
+    """``out[t] = y[t] + scale[i] * b[i] (a[i] x[t])`` with ``i = plan.ids[t]``, and ``y[t]`` for rows without an adapter:
+    what the low-rank adapters of a step's requests add to the output ``y [M, N]`` of the projection of ``x [M, K]`` that
+    they share.  ``out`` is a new tensor, ``y`` itself, or one that overlaps neither operand.
+
+    ``a [adapters, P, R, K]``, ``b [adapters, N, R]``, contiguous and in the dtype of ``x`` and ``y`` (float32 or bfloat16; sums
+    are fp32 and rounded once).  ``P`` projections may be merged along their columns: ``parts`` are their widths, side by
+    side, at most four (default: one), or with ``pairs`` two of equal width that alternate column by column (gate 0, up 0,
+    gate 1, ...).  A column of part ``p`` takes ``a[:, p]``.  ``ranks`` (int32): adapters whose rank is below ``R``; what lies
+    behind it is not read.  ``w_constant``: no kernel in flight writes ``a`` and ``b``."""
+    what = "adapter_add"
+    if x.dim() != 2 or y.dim() != 2 or a.dim() != 4 or b.dim() != 3:
+        raise KernelError(f"{what}: y [M, N], x [M, K], a [adapters, parts, R, K] and b [adapters, N, R]")
+    M, K = x.shape
+    N = y.shape[1]
+    n, P, R = a.shape[0], a.shape[1], a.shape[2]
+    if y.shape[0] != M or a.shape[3] != K or tuple(b.shape) != (n, N, R):
+        raise KernelError(f"{what}: shapes y {tuple(y.shape)}, x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)} do not match")
+    dtype = x.dtype
+    code = _code(dtype)
+    if y.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
+        raise KernelError(f"{what}: operands of {x.dtype}, {y.dtype}, {a.dtype} and {b.dtype}")
+    if not (a.is_contiguous() and b.is_contiguous()) or (K and x.stride(1) != 1) or (N and y.stride(1) != 1):
+        raise KernelError(f"{what}: the adapters must be contiguous, x and y have unit inner stride")
+    if plan.rows != M or plan.adapters != n:
+        raise KernelError(f"{what}: a plan of {plan.rows} rows and {plan.adapters} adapters for {M} rows and {n} adapters")
+    if pairs:
+        if P != 2 or N % 2 or (parts is not None and tuple(parts) != (N // 2, N // 2)):
+            raise KernelError(f"{what}: pairs are two parts of equal width, got {P} parts {parts} of {N} columns")
+        ends = (N, N, N, N)
+    else:
+        widths = (N,) if parts is None else tuple(parts)
+        if len(widths) != P or P > ADAPTER_MAX_PARTS or sum(widths) != N or min(widths) < 0:
+            raise KernelError(f"{what}: parts {widths} for {P} stacked parts of {N} columns (at most {ADAPTER_MAX_PARTS})")
+        e0 = widths[0]
+        e1 = e0 + (widths[1] if P > 1 else 0)
+        e2 = e1 + (widths[2] if P > 2 else 0)
+        ends = (e0, e1, e2, N)
+    if scale is not None:
+        _vector(what, "scale", scale, torch.float32, n)
+    if ranks is not None:
+        _vector(what, "ranks", ranks, torch.int32, n)
+    if out is None:
+        _same_device(what, x, y, a, b, plan.ids, scale, ranks)
+        out = torch.empty((M, N), dtype=dtype, device=x.device)
+    else:
+        if out.shape != y.shape or out.dtype != dtype or (N and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise KernelError(f"{what}: out must be [M, N] in the operands' dtype, rows apart, with unit inner stride")
+        same = out.data_ptr() == y.data_ptr() and (M <= 1 or out.stride(0) == y.stride(0))
+        if not (same or _apart(out, y)) or not _apart(out, x):
+            raise KernelError(f"{what}: out overlaps x, or y without being y")
+        _same_device(what, x, y, a, b, plan.ids, scale, ranks, out)
+    if M == 0 or N == 0:
+        return out
+    h = torch.empty((M, P * R), dtype=torch.float32, device=x.device)
+    lib = _lib("adapters")
+    rc = lib.mi_adapter_add(_ptr(y), y.stride(0), _ptr(x), x.stride(0), _ptr(a), _ptr(b), _ptr(out), out.stride(0),
+                            _ptr(plan.ids), _ptr(scale), _ptr(ranks), _ptr(h), M, N, K, n, P, R, *ends, 1 if pairs else 0, code,
+                            _stream())
+    _finish(lib, rc, what)
+    return out
+
+
+def _history(what: str, counts: torch.Tensor | None, seen: torch.Tensor, V: int) -> int:
+    n = seen.shape[0]
+    if seen.dtype != torch.int32 or seen.dim() != 2 or seen.shape[1] != -(-V // 32) or not seen.is_contiguous():
+        raise KernelError(f"{what}: seen must be contiguous int32 [slots, {-(-V // 32)}]")
+    if counts is not None and (counts.dtype != torch.int32 or tuple(counts.shape) != (n, V) or not counts.is_contiguous()):
+        raise KernelError(f"{what}: counts must be contiguous int32 [{n}, {V}]")
+    return n
+
+
+def adjust_logits(logits: torch.Tensor, out: torch.Tensor | None = None, *, slots: torch.Tensor | None = None,
+                  seen: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                  repetition: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                  frequency: torch.Tensor | None = None,
+                  bias: "tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None" = None,
+                  masks: torch.Tensor | None = None, mask_rows: torch.Tensor | None = None) -> torch.Tensor:
+    """fp32 ``logits [B, V]`` after what each row's request asks for, in this order; ``out`` is a new tensor, ``logits`` itself
+    (only what changes is then read and written), or one that does not overlap them.
+
+    *Penalties* from token histories as ``record_tokens`` keeps them, ``seen [slots, ceil(V / 32)]`` and ``counts [slots, V]``,
+    row ``slots[b]`` for row ``b`` (default ``b``; a row outside the histories has none): a logit whose token has been seen is
+    divided by ``repetition[b]`` where it is positive and multiplied by it where not, and one whose token was generated ``c > 0``
+    times loses ``frequency[b] * c + presence[b]``.  ``counts`` are looked at where ``seen`` has its bit.
+
+    *Biases* ``(starts [B + 1], ids, values)`` int32, int32 and fp32: row ``b`` adds ``values[j]`` to token ``ids[j]`` for ``starts[b] <= j <
+    starts[b + 1]``; a token named twice gets both, an id outside the vocabulary is left out.
+
+    *Masks* ``[n, ceil(V / 32)]`` int32, one bit a token (bit ``v % 32`` of word ``v / 32``): row ``b`` keeps the tokens of
+    mask ``mask_rows[b]`` (default ``b``; a number outside the masks: all tokens), the others become minus infinity whatever they were."""
+    what = "adjust_logits"
+    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] and logits.stride(1) != 1):
+        raise KernelError(f"{what}: logits must be fp32 [B, V] with unit inner stride")
+    B, V = logits.shape
+    n_slots = n_masks = n_bias = 0
+    if seen is not None:
+        n_slots = _history(what, counts, seen, V)
+    elif counts is not None or slots is not None or repetition is not None or presence is not None or frequency is not None:
+        raise KernelError(f"{what}: penalties need the histories' seen bits")
+    if counts is None and (presence is not None or frequency is not None):
+        raise KernelError(f"{what}: presence and frequency penalties need the histories' counts")
+    if slots is not None:
+        _vector(what, "slots", slots, torch.int32, B)
+    elif seen is not None and n_slots < B:
+        raise KernelError(f"{what}: {n_slots} histories for {B} rows without slots")
+    _vector(what, "repetition", repetition, torch.float32, B)
+    _vector(what, "presence", presence, torch.float32, B)
+    _vector(what, "frequency", frequency, torch.float32, B)
+    starts = ids = values = None
+    if bias is not None:
+        starts, ids, values = bias
+        n_bias = ids.shape[0] if ids.dim() == 1 else -1
+        _vector(what, "the biases' starts", starts, torch.int32, B + 1)
+        _vector(what, "the biases' ids", ids, torch.int32, n_bias)
+        _vector(what, "the biases' values", values, torch.float32, n_bias)
+    if masks is not None:
+        if masks.dtype != torch.int32 or masks.dim() != 2 or masks.shape[1] != -(-V // 32) or not masks.is_contiguous():
+            raise KernelError(f"{what}: masks must be contiguous int32 [n, {-(-V // 32)}]")
+        n_masks = masks.shape[0]
+        _vector(what, "mask_rows", mask_rows, torch.int32, B)
+        if mask_rows is None and n_masks < B:
+            raise KernelError(f"{what}: {n_masks} masks for {B} rows without mask_rows")
+    elif mask_rows is not None:
+        raise KernelError(f"{what}: mask_rows without masks")
+    if B > 1 and logits.stride(0) < V:
+        raise KernelError(f"{what}: the rows of the logits overlap")
+    _same_device(what, logits, out, slots, seen, counts, repetition, presence, frequency, starts, ids, values, masks, mask_rows)
+    if out is None:
+        out = torch.empty((B, V), dtype=torch.float32, device=logits.device)
+    else:
+        if out.dtype != torch.float32 or out.shape != logits.shape or (V and out.stride(1) != 1) or (B > 1 and out.stride(0) < V):
+            raise KernelError(f"{what}: out must be fp32 [B, V], rows apart, with unit inner stride")
+        same = out.data_ptr() == logits.data_ptr() and (B <= 1 or out.stride(0) == logits.stride(0))
+        if not (same or _apart(out, logits)):
+            raise KernelError(f"{what}: out overlaps the logits without being them")
+    if B == 0 or V == 0:
+        return out
+    lib = _lib("logits")
+    rc = lib.mi_adjust_logits(_ptr(logits), logits.stride(0), _ptr(out), out.stride(0), B, V, _ptr(slots), _ptr(seen),
+                              _ptr(counts), n_slots, _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(starts), _ptr(ids),
+                              _ptr(values), n_bias, _ptr(masks), _ptr(mask_rows), n_masks, _stream())
+    _finish(lib, rc, what)
+    return out
+
+
+def record_tokens(counts: torch.Tensor, seen: torch.Tensor, slots: torch.Tensor | None, starts: torch.Tensor | None,
+                  tokens: torch.Tensor, *, n_prompt: torch.Tensor | None = None, fresh: bool = False) -> None:
+    """Tokens into the histories that ``adjust_logits`` reads: ``counts [slots, V]`` int32, the times a token was generated,
+    and ``seen [slots, ceil(V / 32)]`` int32, one bit for a token of the prompt or generated.
+
+    Request ``i`` has the tokens ``tokens[starts[i]:starts[i + 1]]`` (int32; without ``starts`` the one token ``tokens[i]``) and
+    the history ``slots[i]`` (default ``i``).  The first ``n_prompt[i]`` of them are its prompt's (default: none, all are
+    generated).  ``fresh``: the history is written anew, and the slots of a call are different ones; otherwise the tokens
+    are added to it.  A token outside the vocabulary and a slot outside the histories are left out."""
+    what = "record_tokens"
+    if counts.dim() != 2:
+        raise KernelError(f"{what}: counts must be contiguous int32 [slots, V]")
+    V = counts.shape[1]
+    n_slots = _history(what, counts, seen, V)
+    if tokens.dtype != torch.int32 or tokens.dim() != 1 or not tokens.is_contiguous():
+        raise KernelError(f"{what}: tokens must be a contiguous int32 vector")
+    if starts is not None:
+        if starts.dim() != 1 or starts.shape[0] < 1:
+            raise KernelError(f"{what}: starts must be a contiguous int32 vector, one more than requests")
+        B = starts.shape[0] - 1
+        _vector(what, "starts", starts, torch.int32, B + 1)
+    else:
+        B = tokens.shape[0]
+    _vector(what, "slots", slots, torch.int32, B)
+    if slots is None and B > n_slots:
+        raise KernelError(f"{what}: {n_slots} histories for {B} requests without slots")
+    _vector(what, "n_prompt", n_prompt, torch.int32, B)
+    _same_device(what, counts, seen, slots, starts, tokens, n_prompt)
+    if B == 0 or V == 0:
+        return
+    lib = _lib("logits")
+    rc = lib.mi_record_tokens(_ptr(counts), _ptr(seen), n_slots, V, _ptr(slots), _ptr(starts), _ptr(tokens), tokens.shape[0],
+                              _ptr(n_prompt), B, 1 if fresh else 0, _stream())
+    _finish(lib, rc, what)
