@@ -13,8 +13,8 @@
 MI_DEFINE_ERROR_API()
 
 #define ADJUST_THREADS 256
-#define ADJUST_GROUPS 4       // groups of 4 columns that a thread has under way at once
-#define ADJUST_COLS (ADJUST_THREADS * ADJUST_GROUPS * 4)
+#define ADJUST_GROUPS 8                         // groups of 4 columns of a lane: a word of bits per lane, in other order
+#define ADJUST_WARP_COLS (32 * ADJUST_GROUPS * 4)
 
 struct AdjustArgs {
   const float* logits;
@@ -34,143 +34,164 @@ struct AdjustArgs {
   int n_masks;
 };
 
-// The bits of columns c .. c + 3 of a row of bits.
-__device__ __forceinline__ uint32_t four_bits(const uint32_t* row, int c, int words) {
-  const int w = c >> 5;
-  return __funnelshift_r(row[w], row[min(w + 1, words - 1)], c & 31) & 15u;
-}
-
-// A block takes ADJUST_COLS columns of one row, a thread four groups of four columns: all its loads are under way before the
-// first is looked at, and a row that starts off a 16-byte boundary is taken from its first boundary on (the up to three columns
-// in front are a group of their own).  In place, a group of which nothing changes is neither read nor written.
+// A warp takes 1024 columns of a row.  All of them pass through in groups of four a lane, eight loads under way at once, with minus
+// infinity put in by the mask's bits; what else changes are single columns, and they are done on their own behind that: each lane
+// goes through the seen bits of one word (32 columns; where one has many, they are shared out among the lanes), four at a time, and the warp through the row's biases.  So the way of
+// the many columns that stay as they are is a load, a few bits and a store.  A row that starts off a 16-byte boundary is taken
+// from its first boundary on; the up to three columns in front are the first warp's.  In place, columns that do not change are
+// neither read nor written.
 template <bool IN_PLACE>
 __global__ void __launch_bounds__(ADJUST_THREADS) adjust_logits_kernel(const AdjustArgs a) {
   mi_pdl_enter();   // the logits and the histories come from the kernels before this one
-  __shared__ float bias_at[ADJUST_COLS + 4];
-  __shared__ uint32_t biased[ADJUST_COLS / 32 + 1];
-  const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  __shared__ unsigned short lists[ADJUST_THREADS / 32][ADJUST_WARP_COLS];
+  const int row = blockIdx.y, lane = threadIdx.x & 31;
+  const int part = blockIdx.x * (ADJUST_THREADS / 32) + (threadIdx.x >> 5);
   const float* in = a.logits + (size_t)row * a.ld_in;
   float* out = a.out + (size_t)row * a.ld_out;
-  // columns before the first 16-byte boundary, and this block's columns: [begin, end), the first block's from 0 on
+  const bool biases = a.bias_starts != nullptr;
+  const int slot = a.seen ? (a.slots ? a.slots[row] : row) : -1;
+  const int mrow = a.masks ? (a.mask_rows ? a.mask_rows[row] : row) : -1;
+  const int first = biases ? max(0, a.bias_starts[row]) : 0, last = biases ? min(a.n_bias, a.bias_starts[row + 1]) : 0;
+  // the columns before the first 16-byte boundary; this warp's: [start, end)
   const int head = (int)((16 - (reinterpret_cast<uintptr_t>(in) & 15)) & 15) / 4;
-  const int start = blockIdx.x * ADJUST_COLS + head;
-  const int begin = blockIdx.x ? start : 0, end = min(a.V, start + ADJUST_COLS);
-  const bool vec_out = (reinterpret_cast<uintptr_t>(out + head) & 15) == 0;
+  const int start = part * ADJUST_WARP_COLS + head, end = min(a.V, start + ADJUST_WARP_COLS);
+  const int lead = part ? 0 : min(head, a.V);
+  if (start >= end && !lead) return;
 
   float4 z[ADJUST_GROUPS];
   if (!IN_PLACE) {
 #pragma unroll
     for (int j = 0; j < ADJUST_GROUPS; ++j) {
-      const int c = start + (j * ADJUST_THREADS + tid) * 4;
+      const int c = start + j * 128 + lane * 4;
       if (c + 4 <= end) z[j] = *reinterpret_cast<const float4*>(in + c);
     }
   }
-  const int slot = a.seen ? (a.slots ? a.slots[row] : row) : -1;
-  const int mrow = a.masks ? (a.mask_rows ? a.mask_rows[row] : row) : -1;
   const bool known = slot >= 0 && slot < a.n_slots, masked = mrow >= 0 && mrow < a.n_masks;
   const uint32_t* seen = a.seen + (size_t)(known ? slot : 0) * a.words;
   const uint32_t* mask = a.masks + (size_t)(masked ? mrow : 0) * a.words;
-  uint32_t told[ADJUST_GROUPS], shut[ADJUST_GROUPS];
-#pragma unroll
-  for (int j = 0; j < ADJUST_GROUPS; ++j) {
-    const int c = start + (j * ADJUST_THREADS + tid) * 4;
-    told[j] = known && c < end ? four_bits(seen, c, a.words) : 0u;
-    shut[j] = masked && c < end ? ~four_bits(mask, c, a.words) & 15u : 0u;
-  }
+  const int* counts = known && a.counts ? a.counts + (size_t)slot * a.V : nullptr;
   const float rep = known && a.repetition ? a.repetition[row] : 1.f;
   const float pres = known && a.presence ? a.presence[row] : 0.f;
   const float freq = known && a.frequency ? a.frequency[row] : 0.f;
-  const int* counts = known && a.counts ? a.counts + (size_t)slot * a.V : nullptr;
-
-  // The biases of this block's columns into shared memory, a bit for each column that has one.  One warp adds them in the
-  // order of the list: of equal ids within 32 entries the first one's lane adds all, so that every sum has one order.
-  const bool biases = a.bias_starts != nullptr;
-  if (biases) {
-    for (int i = tid; i < ADJUST_COLS / 32 + 1; i += ADJUST_THREADS) biased[i] = 0u;
-    __syncthreads();
-    if (tid < 32) {
-      const int first = max(0, a.bias_starts[row]), last = min(a.n_bias, a.bias_starts[row + 1]);
-      for (int j0 = first; j0 < last; j0 += 128) {
-        int ids[4];
-        float values[4];
+  int ids[4];
+  float values[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int j = j0 + 32 * u + lane;
-          ids[u] = j < last ? a.bias_ids[j] : -1;
-          values[u] = j < last ? a.bias_values[j] : 0.f;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const bool mine = ids[u] >= begin && ids[u] < end;
-          unsigned any = __ballot_sync(0xffffffffu, mine);
-          if (!any) continue;
-          const unsigned same = __match_any_sync(0xffffffffu, mine ? ids[u] : -1 - lane);
-          const bool leads = mine && lane == __ffs(same) - 1;
-          const int at = ids[u] - begin;
-          bool there = leads && ((biased[at >> 5] >> (at & 31)) & 1u);
-          float sum = there ? bias_at[at] : 0.f;
-          while (any) {
-            const int from = __ffs(any) - 1;
-            any &= any - 1;
-            const float add = __shfl_sync(0xffffffffu, values[u], from);
-            if (leads && ((same >> from) & 1u)) {
-              sum = there ? __fadd_rn(sum, add) : add;
-              there = true;
-            }
-          }
-          __syncwarp();
-          if (leads) {
-            bias_at[at] = sum;
-            atomicOr(&biased[at >> 5], 1u << (at & 31));
-          }
-          __syncwarp();
-        }
-      }
-    }
-    __syncthreads();
+  for (int u = 0; u < 4; ++u) {
+    const int j = first + 32 * u + lane;
+    ids[u] = j < last ? a.bias_ids[j] : -1;
+    values[u] = j < last ? a.bias_values[j] : 0.f;
   }
 
-  const auto one = [&](float v, int c, bool here, bool closed, bool more) {
-    if (here) {
-      v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-      const int n = counts ? counts[c] : 0;
-      if (n > 0) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)n)), pres);
-    }
-    if (more) v = __fadd_rn(v, bias_at[c - begin]);
-    return closed ? -INFINITY : v;
-  };
+  // the lane's word: columns mine .. mine + 31
+  const int mine = start + lane * 32, w = mine >> 5;
+  uint32_t told = 0u, shut = 0u;
+  if (mine < end) {
+    const uint32_t valid = end - mine >= 32 ? ~0u : (1u << (end - mine)) - 1u;
+    const int w1 = head ? min(w + 1, a.words - 1) : w;
+    if (known) told = __funnelshift_r(seen[w], seen[w1], head) & valid;
+    if (masked) shut = ~__funnelshift_r(mask[w], mask[w1], head) & valid;
+  }
+  const bool any_shut = __any_sync(0xffffffffu, shut != 0u);
+  if (!IN_PLACE || any_shut) {
+    const bool vec_out = (reinterpret_cast<uintptr_t>(out + start) & 15) == 0;
 #pragma unroll
-  for (int j = 0; j < ADJUST_GROUPS; ++j) {
-    const int c = start + (j * ADJUST_THREADS + tid) * 4;
-    if (c >= end) break;
-    uint32_t more = 0u;
-    if (biases) {
-      const int w = (c - begin) >> 5;
-      more = __funnelshift_r(biased[w], biased[min(w + 1, ADJUST_COLS / 32)], (c - begin) & 31) & 15u;
-    }
-    const uint32_t changed = told[j] | shut[j] | more;
-    if (IN_PLACE && !changed) continue;
-    if (c + 4 <= end) {
-      if (IN_PLACE) z[j] = *reinterpret_cast<const float4*>(in + c);
-      if (changed) {
-        z[j].x = one(z[j].x, c, told[j] & 1u, shut[j] & 1u, more & 1u);
-        z[j].y = one(z[j].y, c + 1, told[j] & 2u, shut[j] & 2u, more & 2u);
-        z[j].z = one(z[j].z, c + 2, told[j] & 4u, shut[j] & 4u, more & 4u);
-        z[j].w = one(z[j].w, c + 3, told[j] & 8u, shut[j] & 8u, more & 8u);
-      }
-      if (vec_out) {
-        *reinterpret_cast<float4*>(out + c) = z[j];
+    for (int j = 0; j < ADJUST_GROUPS; ++j) {
+      const int c = start + j * 128 + lane * 4;
+      const uint32_t four = any_shut ? (__shfl_sync(0xffffffffu, shut, j * 4 + (lane >> 3)) >> ((lane & 7) * 4)) & 15u : 0u;
+      if (IN_PLACE ? four == 15u && vec_out : c + 4 <= end && vec_out) {
+        float4 v = IN_PLACE ? make_float4(0.f, 0.f, 0.f, 0.f) : z[j];
+        if (four & 1u) v.x = -INFINITY;
+        if (four & 2u) v.y = -INFINITY;
+        if (four & 4u) v.z = -INFINITY;
+        if (four & 8u) v.w = -INFINITY;
+        *reinterpret_cast<float4*>(out + c) = v;
       } else {
-        out[c] = z[j].x; out[c + 1] = z[j].y; out[c + 2] = z[j].z; out[c + 3] = z[j].w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (IN_PLACE ? (four >> i) & 1u : c + i < end) out[c + i] = (four >> i) & 1u ? -INFINITY : in[c + i];
       }
-    } else {
-      for (int i = 0; c + i < end; ++i) out[c + i] = one(in[c + i], c + i, (told[j] >> i) & 1u, (shut[j] >> i) & 1u, (more >> i) & 1u);
     }
   }
-  if (blockIdx.x == 0 && tid < min(head, a.V)) {          // the columns before the boundary
-    const uint32_t here = known ? (seen[0] >> tid) & 1u : 0u, closed = masked ? ~(mask[0] >> tid) & 1u : 0u;
-    const uint32_t more = biases ? (biased[0] >> tid) & 1u : 0u;
-    if (!IN_PLACE || (here | closed | more)) out[tid] = one(in[tid], tid, here, closed, more);
+  const auto penalised = [&](float v, int n) {
+    v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+    if (n > 0) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)n)), pres);
+    return v;
+  };
+  if (lane < lead) {
+    const bool closed = masked && !((mask[0] >> lane) & 1u), here = known && ((seen[0] >> lane) & 1u);
+    if (closed) out[lane] = -INFINITY;
+    else if (here) out[lane] = penalised(in[lane], counts ? counts[lane] : 0);
+    else if (!IN_PLACE) out[lane] = in[lane];
+  }
+  __syncwarp();
+  // Where a word has many, the columns of all lanes are listed in shared memory first and shared out evenly.
+  uint32_t left = told & ~shut;
+  int todo = __popc(left), listed = 0;
+  if (__any_sync(0xffffffffu, todo > 4)) {
+    unsigned short* list = lists[threadIdx.x >> 5];
+    int at = todo;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += n;
+    }
+    listed = __shfl_sync(0xffffffffu, at, 31);
+    for (at -= todo; left; left &= left - 1u) list[at++] = (unsigned short)(lane * 32 + __ffs(left) - 1);
+    __syncwarp();
+    for (int j = lane; j < listed; j += 128) {
+      int c[4], n[4];
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = j + 32 * i < listed ? start + list[j + 32 * i] : -1;
+        v[i] = c[i] >= 0 ? in[c[i]] : 0.f;
+        n[i] = c[i] >= 0 && counts ? counts[c[i]] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c[i] >= 0) out[c[i]] = penalised(v[i], n[i]);
+    }
+  } else if (left) {
+    int c[4], n[4];
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = left ? mine + __ffs(left) - 1 : -1;
+      left &= left - 1u;
+      v[i] = c[i] >= 0 ? in[c[i]] : 0.f;
+      n[i] = c[i] >= 0 && counts ? counts[c[i]] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c[i] >= 0) out[c[i]] = penalised(v[i], n[i]);
+  }
+  // The biases in the order of the list: of equal ids within 32 entries the first one's lane adds all, so that every sum has
+  // one order.
+  const int from = part ? start : 0;
+  for (int j0 = first; j0 < last; j0 += 128) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int v = ids[u];
+      const bool ours = v >= from && v < end && (!masked || ((mask[v >> 5] >> (v & 31)) & 1u));
+      unsigned any = __ballot_sync(0xffffffffu, ours);
+      if (any) {
+        __syncwarp();                             // what other lanes have written of these columns
+        const unsigned same = __match_any_sync(0xffffffffu, ours ? v : -1 - lane);
+        const bool leads = ours && lane == __ffs(same) - 1;
+        float sum = leads ? out[v] : 0.f;
+        while (any) {
+          const int l = __ffs(any) - 1;
+          any &= any - 1;
+          const float add = __shfl_sync(0xffffffffu, values[u], l);
+          if (leads && ((same >> l) & 1u)) sum = __fadd_rn(sum, add);
+        }
+        if (leads) out[v] = sum;
+        __syncwarp();
+      }
+      const int j = j0 + 128 + 32 * u + lane;
+      ids[u] = j < last ? a.bias_ids[j] : -1;
+      values[u] = j < last ? a.bias_values[j] : 0.f;
+    }
   }
 }
 
@@ -180,13 +201,15 @@ extern "C" int mi_adjust_logits(const float* logits, long long ld_in, float* out
                                 const int* bias_starts, const int* bias_ids, const float* bias_values, int n_bias,
                                 const uint32_t* masks, const int* mask_rows, int n_masks, cudaStream_t stream) {
   if (B <= 0 || V <= 0) return 0;
+  if (n_bias > 0x7fffffff - 65536) MI_REFUSE("adjust_logits: %d biases", n_bias);
   if (B > 65535) MI_REFUSE("adjust_logits: %d rows, at most 65535", B);
-  if (V > 0x7fffffff - ADJUST_COLS) MI_REFUSE("adjust_logits: vocabulary %d", V);
+  if (V > 0x7fffffff - 65536) MI_REFUSE("adjust_logits: vocabulary %d", V);
   const bool in_place = out == logits;
   AdjustArgs a = {logits, out, ld_in, ld_out, V, (int)(((long long)V + 31) / 32), slots, seen, counts, n_slots, repetition,
                   presence, frequency, bias_starts, bias_ids, bias_values, n_bias, masks, mask_rows, n_masks};
   // (a row whose first columns lie before a boundary may need no more blocks for it: the first block's stretch is the longer)
-  const dim3 grid((V + ADJUST_COLS - 1) / ADJUST_COLS, B);
+  const int cols = ADJUST_WARP_COLS * (ADJUST_THREADS / 32);
+  const dim3 grid((V + cols - 1) / cols, B);
   if (in_place)
     MI_LAUNCH((adjust_logits_kernel<true>), grid, ADJUST_THREADS, 0, stream, a);
   else
@@ -196,7 +219,8 @@ extern "C" int mi_adjust_logits(const float* logits, long long ld_in, float* out
 
 // ---------------------------------------------------------------------------------------------- histories
 
-#define RECORD_THREADS 512
+#define RECORD_THREADS 256      // of a block that adds tokens
+#define RECORD_AHEAD 4
 
 // Tokens [first, last) are the request's (without `starts`: one token each), those from `made` on are generated ones.
 __device__ __forceinline__ void tokens_of(int req, const int* starts, int n_tokens, const int* n_prompt, int& first, int& last,
@@ -207,10 +231,34 @@ __device__ __forceinline__ void tokens_of(int req, const int* starts, int n_toke
   made = n_prompt ? (long long)from + n_prompt[req] : from;
 }
 
+// op(token) for the tokens [lo, hi), four to a load where they lie on a 16-byte boundary, several loads under way at once.
+template <int THREADS, typename F>
+__device__ __forceinline__ void scan_tokens(const int* tokens, int lo, int hi, int tid, F op) {
+  if (lo >= hi) return;
+  const int to_boundary = (int)((16 - (reinterpret_cast<uintptr_t>(tokens + lo) & 15)) & 15) / 4;
+  const int a = min(hi, lo + to_boundary), n4 = (hi - a) >> 2;
+  if (tid < a - lo) op(tokens[lo + tid]);
+  const int4* p = reinterpret_cast<const int4*>(tokens + a);
+  for (int j0 = tid; j0 < n4; j0 += RECORD_AHEAD * THREADS) {
+    int4 v[RECORD_AHEAD];
+#pragma unroll
+    for (int u = 0; u < RECORD_AHEAD; ++u) v[u] = j0 + u * THREADS < n4 ? p[j0 + u * THREADS] : make_int4(-1, -1, -1, -1);
+#pragma unroll
+    for (int u = 0; u < RECORD_AHEAD; ++u) {
+      op(v[u].x);
+      op(v[u].y);
+      op(v[u].z);
+      op(v[u].w);
+    }
+  }
+  if (tid < hi - a - 4 * n4) op(tokens[a + 4 * n4 + tid]);
+}
+
 // A history written anew: the block counts the request's tokens within its stretch of the vocabulary in shared memory
 // (whole numbers: their order does not matter) and writes the stretch once.  A prompt's token sets a byte (all that do write the
 // same), a generated one adds to its count.
-__global__ void __launch_bounds__(RECORD_THREADS)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS)
 record_fresh_kernel(int* counts, uint32_t* seen, int n_slots, int V, int words, const int* slots, const int* starts,
                     const int* tokens, int n_tokens, const int* n_prompt, int cols) {
   mi_pdl_launch_dependents();
@@ -219,30 +267,28 @@ record_fresh_kernel(int* counts, uint32_t* seen, int n_slots, int V, int words, 
   unsigned char* told = (unsigned char*)(tally + cols);  // [cols]
   const int req = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
   const int begin = blockIdx.x * cols, n = min(V - begin, cols);
-  for (int i = tid; i < cols * 5 / 16; i += RECORD_THREADS) record_smem[i] = make_int4(0, 0, 0, 0);
+  for (int i = tid; i < cols * 5 / 16; i += THREADS) record_smem[i] = make_int4(0, 0, 0, 0);
   mi_pdl_wait();
   const int slot = slots ? slots[req] : req;
   if (slot < 0 || slot >= n_slots) return;
   int first, last;
   long long made;
   tokens_of(req, starts, n_tokens, n_prompt, first, last, made);
+  const int turn = (int)max((long long)first, min(made, (long long)last));
   __syncthreads();
-  for (int i0 = first + tid; i0 < last; i0 += 8 * RECORD_THREADS) {
-    int v[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = i0 + u * RECORD_THREADS < last ? tokens[i0 + u * RECORD_THREADS] : -1;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const unsigned at = (unsigned)v[u] - (unsigned)begin;      // (a token below `begin` wraps to a large number)
-      if (v[u] < 0 || at >= (unsigned)n) continue;
-      if (i0 + u * RECORD_THREADS < made) told[at] = 1;
-      else atomicAdd(&tally[at], 1);
-    }
-  }
+  // (a token below `begin` wraps to a large number, and so does a negative one, but for a block that begins above 2^31)
+  scan_tokens<THREADS>(tokens, first, turn, tid, [&](int v) {
+    const unsigned at = (unsigned)v - (unsigned)begin;
+    if (at < (unsigned)n) told[at] = 1;
+  });
+  scan_tokens<THREADS>(tokens, turn, last, tid, [&](int v) {
+    const unsigned at = (unsigned)v - (unsigned)begin;
+    if (at < (unsigned)n) atomicAdd(&tally[at], 1);
+  });
   __syncthreads();
   int* c = counts + (size_t)slot * V + begin;
   uint32_t* s = seen + (size_t)slot * words + begin / 32;
-  for (int i = tid; i < ((n + 31) & ~31); i += RECORD_THREADS) {
+  for (int i = tid; i < ((n + 31) & ~31); i += THREADS) {
     const int k = tally[i];
     const unsigned bits = __ballot_sync(0xffffffffu, k > 0 || told[i]);
     if (i < n) c[i] = k;
@@ -250,22 +296,39 @@ record_fresh_kernel(int* counts, uint32_t* seen, int n_slots, int V, int words, 
   }
 }
 
-// Tokens added to what a history holds.
+// Tokens added to what a history holds, RECORD_EACH a thread.  A frequent token's bit is mostly there already: it is looked at
+// (in L2, where the others set it) before it is set.
+#define RECORD_EACH 4
 __global__ void __launch_bounds__(RECORD_THREADS)
 record_more_kernel(int* counts, uint32_t* seen, int n_slots, int V, int words, const int* slots, const int* starts,
-                   const int* tokens, int n_tokens, const int* n_prompt) {
+                   const int* tokens, int n_tokens, const int* n_prompt, int B) {
   mi_pdl_enter();
-  const int req = blockIdx.x;
-  const int slot = slots ? slots[req] : req;
-  if (slot < 0 || slot >= n_slots) return;
-  int first, last;
-  long long made;
-  tokens_of(req, starts, n_tokens, n_prompt, first, last, made);
-  for (int i = first + threadIdx.x; i < last; i += RECORD_THREADS) {
-    const int v = tokens[i];
-    if (v < 0 || v >= V) continue;
-    atomicOr(&seen[(size_t)slot * words + (v >> 5)], 1u << (v & 31));
-    if (i >= made) atomicAdd(&counts[(size_t)slot * V + v], 1);
+  const int i0 = blockIdx.x * (RECORD_THREADS * RECORD_EACH) + threadIdx.x;
+  int v[RECORD_EACH];
+#pragma unroll
+  for (int u = 0; u < RECORD_EACH; ++u) v[u] = i0 + u * RECORD_THREADS < n_tokens ? tokens[i0 + u * RECORD_THREADS] : -1;
+  const int begins = starts ? starts[0] : 0;
+#pragma unroll
+  for (int u = 0; u < RECORD_EACH; ++u) {
+    const int i = i0 + u * RECORD_THREADS;
+    if (v[u] < 0 || v[u] >= V || i < begins) continue;
+    int req = i;                                         // the last request that begins at or before token i
+    if (starts) {
+      int hi = B;
+      for (req = 0; hi - req > 1;) {
+        const int mid = (req + hi) >> 1;
+        if (starts[mid] <= i) req = mid;
+        else hi = mid;
+      }
+      if (i >= starts[req + 1]) continue;
+    }
+    if (req >= B) continue;
+    const int slot = slots ? slots[req] : req;
+    if (slot < 0 || slot >= n_slots) continue;
+    uint32_t* word = seen + (size_t)slot * words + (v[u] >> 5);
+    const uint32_t bit = 1u << (v[u] & 31);
+    if (!(__ldcg(word) & bit)) atomicOr(word, bit);
+    if (!n_prompt || i >= (long long)(starts ? starts[req] : i) + n_prompt[req]) atomicAdd(&counts[(size_t)slot * V + v[u]], 1);
   }
 }
 
@@ -276,27 +339,43 @@ extern "C" int mi_record_tokens(int* counts, uint32_t* seen, int n_slots, int V,
   if (B > 65535) MI_REFUSE("record_tokens: %d requests, at most 65535", B);
   if (V > 0x7fffffff - 65536 || n_tokens > 0x7fffffff - 65536) MI_REFUSE("record_tokens: vocabulary %d, %d tokens", V, n_tokens);
   const int words = (int)(((long long)V + 31) / 32);
-  if (fresh) {
-    // Every block of a request reads all its tokens: long stretches read them less often, short ones are more blocks.
-    int cols = 16384;
-    while (cols > 2048 && (long long)B * ((V + cols - 1) / cols) < 296) cols /= 2;
-    static size_t allowed[64];
-    const size_t smem = (size_t)cols * 5;
+  if (!fresh) {
+    const int blocks = (n_tokens + RECORD_THREADS * RECORD_EACH - 1) / (RECORD_THREADS * RECORD_EACH);
+    if (!blocks) return 0;
+    MI_LAUNCH((record_more_kernel), blocks, RECORD_THREADS, 0, stream, counts, seen, n_slots, V, words, slots, starts, tokens,
+              n_tokens, n_prompt, B);
+    MI_RETURN_LAUNCH_STATUS();
+  }
+  // Every block of a request reads all its tokens: long stretches read them less often, short ones are more blocks.  64 requests
+  // of 128256 tokens each, us with stretches of 16384 (1024 threads), 8192 (512) and 4096 (512): up to 32768 tokens 17.6, 19.2
+  // and 26.8; 100 tokens 12.6, 11.4 and 14.8; 16 requests of up to 2048 tokens 5.6, 4.9 and 4.6; one of 17 and a vocabulary of 32000
+  // 3.6, 2.9 and 2.4, and 2.2 with 2048 (256).
+  const bool many = n_tokens / B > 8192;
+  int cols = many ? 16384 : 8192;
+  while (cols > 2048 && (long long)B * ((V + cols - 1) / cols) < 2 * 148) cols /= 2;
+  const int threads = many ? 1024 : cols >= 4096 ? 512 : 256;
+  const size_t smem = (size_t)cols * 5;
+  const dim3 grid((V + cols - 1) / cols, B);
+  if (threads == 1024) {
+    static bool allowed[64];                  // more than 48 KB, once per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && smem > 48 * 1024 && dev >= 0 && dev < 64 && smem > allowed[dev]) {
-      e = cudaFuncSetAttribute(record_fresh_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e == cudaSuccess) allowed[dev] = smem;
+    if (e == cudaSuccess && !(dev < 64 && allowed[dev])) {
+      e = cudaFuncSetAttribute(record_fresh_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, 16384 * 5);
+      if (e == cudaSuccess && dev < 64) allowed[dev] = true;
     }
     if (e != cudaSuccess) {
       (void)cudaGetLastError();
       MI_REFUSE("record_tokens: CUDA: %s", cudaGetErrorString(e));
     }
-    MI_LAUNCH((record_fresh_kernel), dim3((V + cols - 1) / cols, B), RECORD_THREADS, smem, stream, counts, seen, n_slots, V,
-              words, slots, starts, tokens, n_tokens, n_prompt, cols);
+    MI_LAUNCH((record_fresh_kernel<1024>), grid, threads, smem, stream, counts, seen, n_slots, V, words, slots, starts, tokens,
+              n_tokens, n_prompt, cols);
+  } else if (threads == 512) {
+    MI_LAUNCH((record_fresh_kernel<512>), grid, threads, smem, stream, counts, seen, n_slots, V, words, slots, starts, tokens,
+              n_tokens, n_prompt, cols);
   } else {
-    MI_LAUNCH((record_more_kernel), B, RECORD_THREADS, 0, stream, counts, seen, n_slots, V, words, slots, starts, tokens,
-              n_tokens, n_prompt);
+    MI_LAUNCH((record_fresh_kernel<256>), grid, threads, smem, stream, counts, seen, n_slots, V, words, slots, starts, tokens,
+              n_tokens, n_prompt, cols);
   }
   MI_RETURN_LAUNCH_STATUS();
 }
