@@ -29,8 +29,11 @@ struct AdapterArgs {
   int M, N, K, n, P, R;
   int ends[ADAPTER_MAX_PARTS];    // where each part's columns end (side by side)
   int pairs;
-  int chunks;                     // of columns (find_chunk)
   int vec;                        // 4 columns of y and out are one access
+  int span;                       // columns of a block
+  int ks;                         // parts of the sum over K
+  const int* order;
+  const int4* items;
 };
 
 // One warp per (row, part and rank).
@@ -118,22 +121,6 @@ __device__ __forceinline__ void split_bf16(float v, bf16& hi, bf16& lo) {
   lo = __float2bfloat16_rn(isinf(v) || isinf(__bfloat162float(hi)) ? 0.f : rest);
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// a float of the same place in the shared memory of another block of the cluster
-__device__ __forceinline__ float load_remote(const float* p, uint32_t rank) {
-  uint32_t addr = (uint32_t)__cvta_generic_to_shared(p), there;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-  return v;
-}
-
 // The stride, in elements, of a token's row of h in shared memory: whole groups of 32 k, and 64 bytes off a multiple of 128,
 // so that the 8 lanes of a quarter warp (2 tokens x 4 pieces of 16 bytes) touch all banks once.
 __host__ __device__ inline int h_stride(int R) {
@@ -172,186 +159,365 @@ inline int count_chunks(const AdapterArgs& g, int size) {
   return n;
 }
 
-// ---- few rows: both products in one kernel, a cluster of blocks per adapter in use
+// ---- items: up to 8 NT rows that share an adapter (or have none)
 //
-// Every cluster takes up to 8 rows that share an adapter (or have none).  Its blocks cut K between them, exchange their shares of
-// the first sums through distributed shared memory, and cut the columns of the result.  Nothing goes through global memory
-// between the products and there is no second launch.
+// For up to FEW_MAX rows every block finds its item in the ids; for more, adapter_plan has put the rows in order.
 
-#define FEW_CLUSTER 8
-#define FEW_THREADS 256
-#define FEW_ROWS 8            // rows of a cluster
-#define FEW_MAX 256           // rows of a call: one per thread in the search for a cluster's rows
-#define FEW_GROUP 64          // sums of the first product that a pass makes
-#define FEW_MAX_SUMS 1024     // parts * R
+#define TILE_THREADS 256
+#define TILE_WARPS (TILE_THREADS / 32)
+#define FEW_MAX 128           // rows of a call whose items the blocks find by themselves
+#define SUM_GROUP 64          // sums of the first product that a block makes
+#define MAX_ROWS 64           // of an item
 
-__global__ void __launch_bounds__(FEW_THREADS) adapter_few_kernel(const AdapterArgs g) {
-  mi_pdl_enter();
-  extern __shared__ __align__(16) unsigned char few_smem[];
-  __shared__ uint32_t votes[FEW_THREADS / 32];
-  __shared__ int rows[FEW_ROWS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t = lane & 3;
-  const int cand = blockIdx.x / FEW_CLUSTER, rank_in = (int)cluster_rank();
-  const int PR = g.P * g.R, stride = h_stride(g.R);
+struct Item {
+  int id, count;              // adapter (-1: none), rows
+};
 
-  // The cluster stands for row `cand` and those behind it with the same adapter, if `cand` is the first, ninth, ... of them.
-  int mine = tid < g.M ? g.ids[tid] : -1, id = g.ids[cand];
-  if (mine < 0 || mine >= g.n) mine = -1;
-  if (id < 0 || id >= g.n) id = -1;
-  const bool match = tid < g.M && mine == id;
-  const uint32_t vote = __ballot_sync(0xffffffffu, match);
-  if (lane == 0) votes[warp] = vote;
-  __syncthreads();
-  int before = __popc(vote & ((1u << lane) - 1u)), at = 0;
-  for (int w = 0; w < FEW_THREADS / 32; ++w) {
-    if (w < warp) before += __popc(votes[w]);
-    if (w < cand / 32) at += __popc(votes[w]);
-    else if (w == cand / 32) at += __popc(votes[w] & ((1u << (cand & 31)) - 1u));
+// Item `index` of a call of few rows, 8 rows each: rows with one adapter are put together in their order, and items are in the order of
+// their first rows.  `rows` and `ids` are shared memory; count 0: there is no such item.
+__device__ __forceinline__ Item few_item(const AdapterArgs& g, int index, int* rows, int* ids, int* found) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int id = -1;
+  if (tid < FEW_MAX) {
+    id = tid < g.M ? __ldcg(g.ids + tid) : -2;
+    if (id >= g.n || id < -1) id = tid < g.M ? -1 : -2;
+    ids[tid] = id;
   }
-  if (at % FEW_ROWS) return;                       // (all blocks of the cluster alike)
-  int total = 0;
-  for (int w = 0; w < FEW_THREADS / 32; ++w) total += __popc(votes[w]);
-  const int count = min(FEW_ROWS, total - at);
-  if (match && before >= at && before < at + FEW_ROWS) rows[before - at] = tid;
+  if (tid < 2) found[tid] = 0;
   __syncthreads();
+  int before = 0;                                   // earlier rows with this adapter
+  if (tid < g.M) {
+    const int4* p = reinterpret_cast<const int4*>(ids);
+    for (int j = 0; j < tid / 4; ++j) {
+      const int4 v = p[j];
+      before += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
+    }
+    for (int j = tid & ~3; j < tid; ++j) before += ids[j] == id;
+  }
+  const bool leads = tid < g.M && before % 8 == 0;
+  const unsigned vote = __ballot_sync(0xffffffffu, leads);
+  int* votes = ids + FEW_MAX;                       // [warps]
+  if (lane == 0) votes[warp] = __popc(vote);
+  __syncthreads();
+  int at = __popc(vote & ((1u << lane) - 1u));
+  for (int w = 0; w < warp; ++w) at += votes[w];
+  if (leads && at == index) {
+    found[0] = id + 2;
+    found[1] = before;
+  }
+  __syncthreads();
+  Item item = {found[0] - 2, 0};
+  const int base = found[1];
+  const bool mine = tid < g.M && found[0] && id == item.id && before >= base && before < base + 8;
+  if (mine) rows[before - base] = tid;
+  item.count = __syncthreads_count(mine);
+  return item;
+}
 
-  const bf16 *x = (const bf16*)g.x, *y = (const bf16*)g.y;
+template <int NT>
+__device__ __forceinline__ Item get_item(const AdapterArgs& g, int index, int* rows, int* ids, int* found) {
+  if (NT == 1) return few_item(g, index, rows, ids, found);
+  const int4 v = __ldcg(g.items + index);
+  if (threadIdx.x < (unsigned)v.z) rows[threadIdx.x] = __ldcg(g.order + v.y + threadIdx.x);
+  __syncthreads();
+  return Item{v.x, v.z};
+}
+
+__device__ __forceinline__ int rank_of(const AdapterArgs& g, int id) {
+  return id < 0 ? 0 : g.ranks ? max(0, min(__ldcg(g.ranks + id), g.R)) : g.R;
+}
+
+// ---- the first product: a block makes SUM_GROUP sums of an item over a share of K.  NT: 8-token columns of tiles of an item.
+//
+// Warps cut the share of K between them (with 64 tokens, four ways, and the tokens two ways), their sums meet in shared memory
+// and go to h as one part of the sum over K.
+
+template <int NT>
+__global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 2 : 1) adapter_sums_kernel(const AdapterArgs g) {
+  constexpr int TW = NT == 1 ? 1 : 2, KW = TILE_WARPS / TW, NW = NT / TW, TOK = 8 * NT, MT = SUM_GROUP / 16, PAD = SUM_GROUP + 4;
+  // The kernel behind this one starts once the ids and operands of both are there; it waits for these sums alone.
+  mi_pdl_wait();
+  mi_pdl_launch_dependents();
+  extern __shared__ __align__(16) float sums_smem[];          // [KW][TOK][PAD]
+  __shared__ int rows[MAX_ROWS];
+  __shared__ __align__(16) int ids[FEW_MAX + TILE_WARPS];
+  __shared__ int found[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t = lane & 3;
+  const int kw = warp % KW, tw = warp / KW;
+  const Item item = get_item<NT>(g, blockIdx.y, rows, ids, found);
+  const int rank = rank_of(g, item.id);
+  if (item.count == 0 || rank == 0) return;
+  const int PR = g.P * g.R, m0 = blockIdx.z * SUM_GROUP;
+  const int units = (g.K + 31) / 32;                          // 32 values of k: 64 bytes of a row
+  const int u0 = (int)((long long)units * blockIdx.x / g.ks), u1 = (int)((long long)units * (blockIdx.x + 1) / g.ks);
+
+  const bf16* xr[NW];
+  bool live[NW];
+#pragma unroll
+  for (int j = 0; j < NW; ++j) {
+    const int tok = (tw * NW + j) * 8 + gq;
+    live[j] = tok < item.count;
+    xr[j] = (const bf16*)g.x + (long long)rows[live[j] ? tok : 0] * g.ldx + t * 8;
+  }
+  const bf16* ar = (const bf16*)g.a + ((size_t)item.id * PR + m0 + gq) * g.K + t * 8;
+  bool have[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = m0 + m * 16 + hf * 8 + gq;
+      have[m][hf] = r < PR && r % g.R < rank;
+    }
+  float acc[MT][NW][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+#pragma unroll 2
+  for (int u = u0 + kw; u < u1; u += KW) {
+    const bool in = u * 32 + t * 8 < g.K;
+    uint4 xv[NW], av[MT][2];
+#pragma unroll
+    for (int j = 0; j < NW; ++j) xv[j] = in && live[j] ? load16(xr[j] + u * 32) : zero4();
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        av[m][hf] = in && have[m][hf] ? load16(ar + (size_t)(m * 16 + hf * 8) * g.K + u * 32) : zero4();
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < NW; ++j) mma_k32(acc[m][j], av[m][0], av[m][1], xv[j]);
+  }
+  float* mine = sums_smem + (kw * TOK + tw * NW * 8) * PAD;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine[(j * 8 + 2 * t + (i & 1)) * PAD + m * 16 + (i >> 1) * 8 + gq] = acc[m][j][i];
+  __syncthreads();
+  float* h = g.h + (size_t)blockIdx.x * g.M * PR + m0;
+  for (int i = tid; i < item.count * (SUM_GROUP / 4); i += TILE_THREADS) {
+    const int tok = i / (SUM_GROUP / 4), r = i % (SUM_GROUP / 4) * 4;
+    if (m0 + r >= PR) continue;                               // (PR is a multiple of 8)
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(sums_smem + (w * TOK + tok) * PAD + r);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    *reinterpret_cast<float4*>(h + (size_t)rows[tok] * PR + r) = s;
+  }
+}
+
+// ---- the second product and the sum with y: a warp takes 32 columns of 8 or 32 rows at a time; lane (g, t) ends with columns
+// 4 g .. 4 g + 3 of tokens 2 t and 2 t + 1 of every 8.
+//
+// KG: groups of 32 k (0: as many as there are).  FOLD (up to 16 k): the rests of the sums stand where the second 16 k of a group would, so
+// that one pass does for both.
+
+template <int NT, int KG, bool FOLD>
+__global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_kernel(const AdapterArgs g) {
+  constexpr int TW = NT == 1 ? 1 : 2, CW = TILE_WARPS / TW, NW = NT / TW, TOK = 8 * NT;
+  extern __shared__ __align__(16) unsigned char add_smem[];
+  bf16* h = (bf16*)add_smem;                                  // [parts of the block][hi, lo][TOK][stride]
+  __shared__ int rows[MAX_ROWS];
+  __shared__ __align__(16) int ids[FEW_MAX + TILE_WARPS];
+  __shared__ int found[2];
+  mi_pdl_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t = lane & 3;
+  const int cw = warp % CW, tw = warp / CW;
+  // (the kernel in front was started behind everything that wrote the ids and the operands, and started this one behind that)
+  const Item item = get_item<NT>(g, blockIdx.y, rows, ids, found);
+  const int rank = rank_of(g, item.id);
+  const bf16* y = (const bf16*)g.y;
   bf16* out = (bf16*)g.out;
-  int rank = id < 0 ? 0 : g.ranks ? max(0, min(g.ranks[id], g.R)) : g.R;
-  if (rank == 0 && out == y) return;
-
-  float* partial = (float*)few_smem;                                   // [warps][FEW_GROUP][FEW_ROWS]
-  float* sums = partial + (FEW_THREADS / 32) * FEW_GROUP * FEW_ROWS;   // [PR][FEW_ROWS], this block's share of K
-  bf16* h = (bf16*)(sums + PR * FEW_ROWS);                             // [P][hi, lo][FEW_ROWS][stride]
+  int part, c_first, c_end;
+  const bool there = find_chunk(g, blockIdx.x, g.span, part, c_first, c_end) && item.count > 0 && (rank > 0 || out != y);
+  mi_pdl_wait();
+  if (!there) return;
+  c_end = min(c_end, c_first + g.span);
+  const int PR = g.P * g.R, stride = h_stride(g.R), np = g.pairs ? 2 : 1, r32 = FOLD ? 32 : (g.R + 31) / 32 * 32;
 
   if (rank > 0) {
-    const int units = (g.K + 31) / 32;                                 // 32 values of k: 64 bytes of a row
-    const int u0 = (int)((long long)units * rank_in / FEW_CLUSTER), u1 = (int)((long long)units * (rank_in + 1) / FEW_CLUSTER);
-    const bf16* xr = x + (long long)rows[min(gq, count - 1)] * g.ldx + t * 8;
-    const bf16* ad = (const bf16*)g.a + (size_t)id * PR * g.K + t * 8;
-    for (int m0 = 0; m0 < PR; m0 += FEW_GROUP) {
-      float acc[FEW_GROUP / 16][4];
-#pragma unroll
-      for (int m = 0; m < FEW_GROUP / 16; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
-      bool have[FEW_GROUP / 16][2];
-#pragma unroll
-      for (int m = 0; m < FEW_GROUP / 16; ++m)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int r = m0 + m * 16 + hf * 8 + gq;
-          have[m][hf] = r < PR && r % g.R < rank;
-        }
-#pragma unroll 2
-      for (int u = u0 + warp; u < u1; u += FEW_THREADS / 32) {
-        const int k = u * 32 + t * 8;
-        const bool in = k < g.K;
-        const uint4 xv = in && gq < count ? load16(xr + u * 32) : zero4();
-        uint4 av[FEW_GROUP / 16][2];
-#pragma unroll
-        for (int m = 0; m < FEW_GROUP / 16; ++m)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-            av[m][hf] = in && have[m][hf] ? load16(ad + (size_t)(m0 + m * 16 + hf * 8 + gq) * g.K + u * 32) : zero4();
-#pragma unroll
-        for (int m = 0; m < FEW_GROUP / 16; ++m) mma_k32(acc[m], av[m][0], av[m][1], xv);
-      }
-      if (m0) __syncthreads();                     // the last pass's shares have been read
-      float* mineP = partial + warp * FEW_GROUP * FEW_ROWS;
-#pragma unroll
-      for (int m = 0; m < FEW_GROUP / 16; ++m) {
-        *reinterpret_cast<float2*>(mineP + (m * 16 + gq) * FEW_ROWS + 2 * t) = make_float2(acc[m][0], acc[m][1]);
-        *reinterpret_cast<float2*>(mineP + (m * 16 + 8 + gq) * FEW_ROWS + 2 * t) = make_float2(acc[m][2], acc[m][3]);
-      }
-      __syncthreads();
-      for (int i = tid; i < FEW_GROUP * FEW_ROWS && m0 * FEW_ROWS + i < PR * FEW_ROWS; i += FEW_THREADS) {
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < FEW_THREADS / 32; ++w) s += partial[w * FEW_GROUP * FEW_ROWS + i];
-        sums[m0 * FEW_ROWS + i] = s;
-      }
-    }
-    cluster_arrive();
-    cluster_wait();
-    const float scale = g.scale ? g.scale[id] : 1.f;
-    for (int i = tid; i < g.P * FEW_ROWS * stride; i += FEW_THREADS) {
-      const int p = i / (FEW_ROWS * stride), tok = i / stride % FEW_ROWS, r = i % stride;
+    const float scale = g.scale ? g.scale[item.id] : 1.f;
+    const int width = FOLD ? 16 : r32;
+    for (int i = tid; i < np * TOK * width; i += TILE_THREADS) {
+      const int p = i / (TOK * width), tok = i / width % TOK, r = i % width;
       float s = 0.f;
-      if (r < rank) {
-#pragma unroll
-        for (int c = 0; c < FEW_CLUSTER; ++c) s += load_remote(sums + (p * g.R + r) * FEW_ROWS + tok, c);
+      if (r < rank && tok < item.count) {
+        const float* from = g.h + (size_t)rows[tok] * PR + (part + p) * g.R + r;
+#pragma unroll 4
+        for (int k = 0; k < g.ks; ++k) s += __ldcg(from + (size_t)k * g.M * PR);
         s *= scale;
       }
       bf16 hi, lo;
       split_bf16(s, hi, lo);
-      h[((p * 2 + 0) * FEW_ROWS + tok) * stride + r] = hi;
-      h[((p * 2 + 1) * FEW_ROWS + tok) * stride + r] = lo;
+      bf16* to = h + ((p * 2 + 0) * TOK + tok) * stride + r;
+      to[0] = hi;
+      to[FOLD ? 16 : TOK * stride] = lo;
     }
-    cluster_arrive();                              // this block reads nobody's sums any more
     __syncthreads();
   }
 
-  // 32 columns of up to 8 rows a warp and pass; lane (g, t) ends with columns 4 g .. 4 g + 3 of tokens 2 t and 2 t + 1.
-  const int chunks = g.chunks;
-  for (int chunk = rank_in * (FEW_THREADS / 32) + warp; chunk < chunks; chunk += FEW_CLUSTER * (FEW_THREADS / 32)) {
-    int part, c0, cend;
-    if (!find_chunk(g, chunk, 32, part, c0, cend)) break;
+  for (int c0 = c_first + cw * 32; c0 < c_end; c0 += CW * 32) {
     const int c = c0 + 4 * gq;
-    float acc[2][4];
+    float acc[2][NW][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
-    const bf16* b = (const bf16*)g.b + ((size_t)max(id, 0) * g.N + c) * g.R + t * 8;
-    for (int k0 = 0; k0 < rank; k0 += 32) {
-      const int n = rank - k0 - t * 8;             // values of this lane's piece that there are
+      for (int j = 0; j < NW; ++j)
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        uint4 w[2];
+        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+    const bf16* b = (const bf16*)g.b + ((size_t)max(item.id, 0) * g.N + c) * g.R;
+    const auto group = [&](int k0) {
+      const int k = k0 + (FOLD ? t & 1 : t) * 8, n = rank - k;         // this lane's piece, and values of it that there are
+      uint4 w[2][2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          const int j = 2 * hf + m;                // column 4 g + j
-          w[hf] = n > 0 && c + j < cend ? first_of(load16(b + (size_t)j * g.R + k0), n) : zero4();
+          const int j = 2 * hf + m;                                    // column 4 g + j
+          w[m][hf] = n > 0 && c + j < c_end ? first_of(load16(b + (size_t)j * g.R + k), n) : zero4();
         }
-        const bf16* hp = h + ((g.pairs ? m : part) * 2 * FEW_ROWS + gq) * stride + k0 + t * 8;
-        mma_k32(acc[m], w[0], w[1], load16(hp));
-        mma_k32(acc[m], w[0], w[1], load16(hp + FEW_ROWS * stride));
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const bf16* hp = h + (((g.pairs ? m : 0) * 2) * TOK + tw * NW * 8 + gq) * stride + k0 + t * 8;
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+          mma_k32(acc[m][j], w[m][0], w[m][1], load16(hp + j * 8 * stride));
+          if (!FOLD) mma_k32(acc[m][j], w[m][0], w[m][1], load16(hp + (TOK + j * 8) * stride));
+        }
       }
+    };
+    if (KG) {
+#pragma unroll
+      for (int k = 0; k < KG; ++k)
+        if (k * 32 < rank) group(k * 32);
+    } else {
+      for (int k0 = 0; k0 < rank; k0 += 32) group(k0);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int tok = 2 * t + i;
-      if (tok >= count) continue;
-      const long long row = rows[tok];
-      const bf16* yp = y + row * g.ldy + c;
-      bf16* op = out + row * g.ldo + c;
-      const float d[4] = {acc[0][i], acc[1][i], acc[0][2 + i], acc[1][2 + i]};
-      if (g.vec && c + 4 <= cend) {
-        Vec4<bf16> v;
-        float f[4];
-        v.load(yp);
-        if (rank > 0) {
-          v.get(f);
+    for (int j = 0; j < NW; ++j)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) f[j] += d[j];
-          v.set(f);
+      for (int i = 0; i < 2; ++i) {
+        const int tok = (tw * NW + j) * 8 + 2 * t + i;
+        if (tok >= item.count) continue;
+        const long long row = rows[tok];
+        const bf16* yp = y + row * g.ldy + c;
+        bf16* op = out + row * g.ldo + c;
+        const float d[4] = {acc[0][j][i], acc[1][j][i], acc[0][j][2 + i], acc[1][j][2 + i]};
+        if (g.vec && c + 4 <= c_end) {
+          Vec4<bf16> v;
+          float f[4];
+          v.load(yp);
+          if (rank > 0) {
+            v.get(f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f[q] += d[q];
+            v.set(f);
+          }
+          v.store(op);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (c + q < c_end) op[q] = rank > 0 ? __float2bfloat16_rn(__bfloat162float(yp[q]) + d[q]) : yp[q];
         }
-        v.store(op);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < cend) op[j] = rank > 0 ? __float2bfloat16_rn(__bfloat162float(yp[j]) + d[j]) : yp[j];
       }
-    }
   }
-  __syncwarp();
-  if (rank > 0) cluster_wait();                    // the block's shared memory stays until all have read it
 }
 
-static size_t few_smem_bytes(int P, int R) {
-  return (size_t)(FEW_THREADS / 32) * FEW_GROUP * FEW_ROWS * 4 + (size_t)P * R * FEW_ROWS * 4 +
-         (size_t)P * 2 * FEW_ROWS * h_stride(R) * 2;
+// ---- the plan: rows in the order of their adapters, and items of up to 64 of them
+
+#define PLAN_THREADS 1024
+#define PLAN_MAX_ADAPTERS 4096
+
+__global__ void __launch_bounds__(PLAN_THREADS)
+adapter_plan_kernel(const int* ids, int M, int n, int* order, int4* items, int max_items) {
+  mi_pdl_enter();
+  extern __shared__ int plan_smem[];
+  int* count = plan_smem;                  // [n + 1] rows of each adapter, the last: rows without one
+  int* next = count + n + 1;               // [n + 1] where the next row of each goes
+  __shared__ int warp_rows[32], warp_items[32], carry[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i <= n; i += PLAN_THREADS) count[i] = 0;
+  if (tid < 2) carry[tid] = 0;
+  __syncthreads();
+  const auto bucket = [&](int i) {
+    const int id = ids[i];
+    return id >= 0 && id < n ? id : n;
+  };
+  for (int i0 = 0; i0 < M; i0 += PLAN_THREADS) {
+    const int i = i0 + tid, b = i < M ? bucket(i) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, b);
+    if (b >= 0 && lane == __ffs(same) - 1) atomicAdd(&count[b], __popc(same));
+  }
+  __syncthreads();
+  // first rows and first items, from running sums over the adapters
+  for (int i0 = 0; i0 <= n; i0 += PLAN_THREADS) {
+    const int i = i0 + tid, rows = i <= n ? count[i] : 0, mine = (rows + MAX_ROWS - 1) / MAX_ROWS;
+    int r = rows, m = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, r, o), b = __shfl_up_sync(0xffffffffu, m, o);
+      if (lane >= o) {
+        r += a;
+        m += b;
+      }
+    }
+    if (lane == 31) {
+      warp_rows[warp] = r;
+      warp_items[warp] = m;
+    }
+    __syncthreads();
+    int before_r = carry[0], before_m = carry[1];
+    for (int w = 0; w < warp; ++w) {
+      before_r += warp_rows[w];
+      before_m += warp_items[w];
+    }
+    const int first = before_r + r - rows, item = before_m + m - mine;
+    if (i <= n) next[i] = first;
+    for (int k = 0; k < mine; ++k)
+      if (item + k < max_items)
+        items[item + k] = make_int4(i < n ? i : -1, first + k * MAX_ROWS, min(MAX_ROWS, rows - k * MAX_ROWS), 0);
+    __syncthreads();
+    if (tid == PLAN_THREADS - 1) {
+      carry[0] = before_r + r;
+      carry[1] = before_m + m;
+    }
+    __syncthreads();
+  }
+  for (int i = carry[1] + tid; i < max_items; i += PLAN_THREADS) items[i] = make_int4(-1, 0, 0, 0);
+  // rows into their order (which one of an adapter's rows comes first changes nothing that is computed)
+  for (int i0 = 0; i0 < M; i0 += PLAN_THREADS) {
+    const int i = i0 + tid, b = i < M ? bucket(i) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, b);
+    int at = 0;
+    if (b >= 0 && lane == __ffs(same) - 1) at = atomicAdd(&next[b], __popc(same));
+    at = __shfl_sync(0xffffffffu, at, __ffs(same) - 1) + __popc(same & ((1u << lane) - 1u));
+    if (b >= 0) order[at] = i;
+  }
+}
+
+static int plan_items(int M, int n) { return M / MAX_ROWS + (M < n + 1 ? M : n + 1); }
+extern "C" int mi_adapter_plan_sizes(int M, int n, int* max_items) {
+  if (M <= FEW_MAX) {
+    *max_items = 0;
+    return 0;
+  }
+  if (n > PLAN_MAX_ADAPTERS) MI_REFUSE("adapter_plan: %d adapters, at most %d with more than %d rows", n, PLAN_MAX_ADAPTERS, FEW_MAX);
+  *max_items = plan_items(M, n);
+  return 0;
+}
+extern "C" int mi_adapter_plan(const int* ids, int M, int n, int* order, void* items, cudaStream_t stream) {
+  if (M <= FEW_MAX) return 0;
+  if (n > PLAN_MAX_ADAPTERS) MI_REFUSE("adapter_plan: %d adapters, at most %d with more than %d rows", n, PLAN_MAX_ADAPTERS, FEW_MAX);
+  MI_LAUNCH((adapter_plan_kernel), 1, PLAN_THREADS, (size_t)(n + 1) * 2 * sizeof(int), stream, ids, M, n, order, (int4*)items,
+            plan_items(M, n));
+  MI_RETURN_LAUNCH_STATUS();
 }
 
 static int refused_by_cuda(cudaError_t e) {
@@ -360,60 +526,87 @@ static int refused_by_cuda(cudaError_t e) {
   return (int)e;
 }
 
-template <typename K>
-static cudaError_t launch_cluster(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
-                                  const AdapterArgs& g) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = mi_pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, g);
-}
-// Dynamic shared memory over 48 KB is allowed once per kernel and device.
+// Dynamic shared memory that takes a block over 48 KB (with what the kernel has besides) is allowed once per kernel and device.
 template <typename K>
 static cudaError_t allow_smem(K kernel, size_t bytes, size_t* allowed) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64 || bytes <= 48 * 1024 || bytes <= allowed[dev]) return cudaSuccess;
+  if (dev < 0 || dev >= 64 || bytes <= 40 * 1024 || bytes <= allowed[dev]) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e == cudaSuccess) allowed[dev] = bytes;
   return e;
 }
 
+template <int NT>
+static cudaError_t launch_tiles(const AdapterArgs& g0, int max_items, cudaStream_t stream) {
+  AdapterArgs g = g0;
+  constexpr int KW = NT == 1 ? TILE_WARPS : TILE_WARPS / 2, TOK = 8 * NT;
+  static size_t allowed[4][64];
+  const size_t sums_bytes = (size_t)KW * TOK * (SUM_GROUP + 4) * 4;
+  cudaError_t e = allow_smem(adapter_sums_kernel<NT>, sums_bytes, allowed[0]);
+  if (e != cudaSuccess) return e;
+  const int groups = (g.P * g.R + SUM_GROUP - 1) / SUM_GROUP;
+  e = MI_LAUNCH((adapter_sums_kernel<NT>), dim3(g.ks, max_items, groups), TILE_THREADS, sums_bytes, stream, g);
+  if (e != cudaSuccess) return e;
+  const size_t h_bytes = (size_t)(g.pairs ? 2 : 1) * 2 * TOK * h_stride(g.R) * 2;
+  const dim3 grid(count_chunks(g, g.span), max_items);
+  if (g.R <= 16) return MI_LAUNCH((adapter_add_kernel<NT, 1, true>), grid, TILE_THREADS, h_bytes, stream, g);
+  if (g.R <= 32) return MI_LAUNCH((adapter_add_kernel<NT, 1, false>), grid, TILE_THREADS, h_bytes, stream, g);
+  if (g.R <= 64) {
+    e = allow_smem(adapter_add_kernel<NT, 2, false>, h_bytes, allowed[1]);
+    if (e != cudaSuccess) return e;
+    return MI_LAUNCH((adapter_add_kernel<NT, 2, false>), grid, TILE_THREADS, h_bytes, stream, g);
+  }
+  e = allow_smem(adapter_add_kernel<NT, 0, false>, h_bytes, allowed[2]);
+  if (e != cudaSuccess) return e;
+  return MI_LAUNCH((adapter_add_kernel<NT, 0, false>), grid, TILE_THREADS, h_bytes, stream, g);
+}
+
+// Parts of the sum over K: enough blocks for the chip, at least one unit of 32 k for every warp.
+static int sum_parts(int M, int n, int K, int P, int R) {
+  const int units = (K + 31) / 32, groups = (P * R + SUM_GROUP - 1) / SUM_GROUP;
+  const int items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : (M + MAX_ROWS - 1) / MAX_ROWS;
+  int ks = 2 * 148 / (items * groups);
+  const int most = M <= FEW_MAX ? units / TILE_WARPS : units / (TILE_WARPS / 2) / 2;
+  ks = ks < most ? ks : most;
+  return ks < 1 ? 1 : ks > 16 ? 16 : ks;
+}
+
+// Whether the tensor-core kernels take a call: rows of x, A and B in pieces of 16 bytes, a plan where there are many rows.
+static bool in_pieces(const void* x, long long ldx, const void* a, const void* b, int M, int K, int n, int P, int R, int dtype) {
+  return dtype == MI_DTYPE_BF16 && n > 0 && R > 0 && R <= 256 && K > 0 && R % 8 == 0 && K % 8 == 0 && mi_aligned(a, 16) &&
+         mi_aligned(b, 16) && mi_aligned(x, 16) && (M == 1 || ldx % 8 == 0) && P * R <= 65535 * SUM_GROUP;
+}
+
+// Floats of scratch memory (h) that a call needs.
+extern "C" long long mi_adapter_scratch(const void* x, long long ldx, const void* a, const void* b, int M, int K, int n, int P,
+                                        int R, int dtype) {
+  const long long one = (long long)M * P * R;
+  return in_pieces(x, ldx, a, b, M, K, n, P, R, dtype) ? one * sum_parts(M, n, K, P, R) : one;
+}
+
 extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b,
-                              void* out, long long ldo, const int* ids, const float* scale, const int* ranks, float* h, int M,
-                              int N, int K, int n, int P, int R, int end0, int end1, int end2, int end3, int pairs, int dtype,
-                              cudaStream_t stream) {
+                              void* out, long long ldo, const int* ids, const int* order, const void* items, const float* scale,
+                              const int* ranks, float* h, int M, int N, int K, int n, int P, int R, int end0, int end1, int end2,
+                              int end3, int pairs, int dtype, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  if (M > 65535) MI_REFUSE("adapter_add: %d rows, at most 65535", M);
   if (P < 1 || P > ADAPTER_MAX_PARTS) MI_REFUSE("adapter_add: %d parts, at most %d", P, ADAPTER_MAX_PARTS);
-  AdapterArgs g = {x, ldx, y, ldy, out, ldo, a, b, ids, ranks, scale, h, M, N, K, n, P, R, {end0, end1, end2, end3}, pairs, 0, 0};
-  // The tensor-core kernels take rows of x, A and B in pieces of 16 bytes.
-  const bool pieces = dtype == MI_DTYPE_BF16 && n > 0 && R > 0 && K > 0 && R % 8 == 0 && K % 8 == 0 && mi_aligned(a, 16) &&
-                      mi_aligned(b, 16) && mi_aligned(x, 16) && (M == 1 || ldx % 8 == 0);
-  bool starts4 = true;
-  for (int p = 0; p + 1 < P && !pairs; ++p) starts4 = starts4 && g.ends[p] % 4 == 0;
-  g.vec = starts4 && mi_aligned(y, 8) && mi_aligned(out, 8) && (M == 1 || (ldy % 4 == 0 && ldo % 4 == 0));
-  if (pieces && M <= FEW_MAX && P * R <= FEW_MAX_SUMS) {
-    static size_t allowed[64];
-    const size_t smem = few_smem_bytes(P, R);
-    g.chunks = count_chunks(g, 32);
-    cudaError_t e = allow_smem(adapter_few_kernel, smem, allowed);
-    if (e == cudaSuccess) e = launch_cluster(adapter_few_kernel, dim3(M * FEW_CLUSTER), FEW_THREADS, smem, FEW_CLUSTER, stream, g);
+  AdapterArgs g = {x, ldx, y, ldy, out, ldo, a, b, ids, ranks, scale, h, M, N, K, n, P, R, {end0, end1, end2, end3}, pairs, 0, 0, 1,
+                   order, (const int4*)items};
+  if (in_pieces(x, ldx, a, b, M, K, n, P, R, dtype) && (M <= FEW_MAX || (order && items))) {
+    const int max_items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : plan_items(M, n);
+    if (max_items > 65535) MI_REFUSE("adapter_add: %d rows with %d adapters", M, n);
+    bool starts4 = true;
+    for (int p = 0; p + 1 < P && !pairs; ++p) starts4 = starts4 && g.ends[p] % 4 == 0;
+    g.vec = starts4 && mi_aligned(y, 8) && mi_aligned(out, 8) && (M == 1 || (ldy % 4 == 0 && ldo % 4 == 0));
+    g.ks = sum_parts(M, n, K, P, R);
+    g.span = M <= FEW_MAX ? 256 : 512;
+    const cudaError_t e = M <= FEW_MAX ? launch_tiles<1>(g, max_items, stream) : launch_tiles<8>(g, max_items, stream);
     if (e != cudaSuccess) return refused_by_cuda(e);
     MI_RETURN_LAUNCH_STATUS();
   }
+  if (M > 65535) MI_REFUSE("adapter_add: %d rows, at most 65535 of operands that are not in pieces of 16 bytes", M);
   const long long units = (long long)M * P * R, per = ADAPTER_THREADS / 32;
   if ((units + per - 1) / per > 0x7fffffffLL) MI_REFUSE("adapter_add: %lld sums of the first product", units);
   const unsigned blocks = n > 0 ? (unsigned)((units + per - 1) / per) : 0u;

@@ -439,8 +439,12 @@ def _sig_attention_stage(lib: ctypes.CDLL) -> None:
 def _sig_adapters(lib: ctypes.CDLL) -> None:
     ll = ctypes.c_longlong
     lib.mi_adapter_add.argtypes = [c_void_p, ll, c_void_p, ll, c_void_p, c_void_p, c_void_p, ll, c_void_p, c_void_p, c_void_p,
-                                   c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                   c_int, c_void_p]
+                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                   c_int, c_int, c_int, c_void_p]
+    lib.mi_adapter_scratch.argtypes = [c_void_p, ll, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int]
+    lib.mi_adapter_scratch.restype = ll
+    lib.mi_adapter_plan_sizes.argtypes = [c_int, c_int, ctypes.POINTER(c_int)]
+    lib.mi_adapter_plan.argtypes = [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]
 
 
 def _sig_logits(lib: ctypes.CDLL) -> None:
@@ -2997,12 +3001,17 @@ ADAPTER_MAX_PARTS = 4
 
 class AdapterPlan:
     """Which of ``adapters`` low-rank adapters each row of a step uses (``ids``), prepared for ``adapter_add``: made once a
-    step by ``adapter_plan`` and handed to every projection."""
+    step by ``adapter_plan`` and handed to every projection.  Of more rows than a block looks through by itself, ``order`` puts those
+    of one adapter together and ``items`` are stretches of it."""
 
-    __slots__ = ("ids", "rows", "adapters")
+    __slots__ = ("ids", "rows", "adapters", "order", "items")
 
     def __init__(self, ids: torch.Tensor, adapters: int) -> None:
         self.ids, self.rows, self.adapters = ids, ids.shape[0], adapters
+        self.order = self.items = None
+
+
+ADAPTER_FEW_ROWS = 128       # rows whose adapters the kernels look through by themselves
 
 
 def adapter_plan(ids: torch.Tensor, adapters: int) -> AdapterPlan:
@@ -3012,7 +3021,17 @@ def adapter_plan(ids: torch.Tensor, adapters: int) -> AdapterPlan:
     if adapters < 0:
         raise KernelError(f"adapter_plan: {adapters} adapters")
     _same_device("adapter_plan", ids)
-    return AdapterPlan(ids, int(adapters))
+    plan = AdapterPlan(ids, int(adapters))
+    if plan.rows > ADAPTER_FEW_ROWS:
+        lib = _lib("adapters")
+        n = c_int(0)
+        rc = lib.mi_adapter_plan_sizes(plan.rows, plan.adapters, ctypes.byref(n))
+        if rc == 0:
+            plan.order = torch.empty(plan.rows, dtype=torch.int32, device=ids.device)
+            plan.items = torch.empty((n.value, 4), dtype=torch.int32, device=ids.device)
+            rc = lib.mi_adapter_plan(_ptr(ids), plan.rows, plan.adapters, _ptr(plan.order), _ptr(plan.items), _stream())
+        _finish(lib, rc, "adapter_plan")
+    return plan
 
 
 def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: AdapterPlan, *,
@@ -3071,11 +3090,12 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
         _same_device(what, x, y, a, b, plan.ids, scale, ranks, out)
     if M == 0 or N == 0:
         return out
-    h = torch.empty((M, P * R), dtype=torch.float32, device=x.device)
     lib = _lib("adapters")
+    h = torch.empty(lib.mi_adapter_scratch(_ptr(x), x.stride(0), _ptr(a), _ptr(b), M, K, n, P, R, code), dtype=torch.float32,
+                    device=x.device)
     rc = lib.mi_adapter_add(_ptr(y), y.stride(0), _ptr(x), x.stride(0), _ptr(a), _ptr(b), _ptr(out), out.stride(0),
-                            _ptr(plan.ids), _ptr(scale), _ptr(ranks), _ptr(h), M, N, K, n, P, R, *ends, 1 if pairs else 0, code,
-                            _stream())
+                            _ptr(plan.ids), _ptr(plan.order), _ptr(plan.items), _ptr(scale), _ptr(ranks), _ptr(h), M, N, K, n, P, R,
+                            *ends, 1 if pairs else 0, code, _stream())
     _finish(lib, rc, what)
     return out
 
