@@ -34,6 +34,7 @@ struct AdapterArgs {
   int ks;                         // parts of the sum over K
   const int* order;
   const int4* items;
+  int constant;                   // no kernel in flight writes A and B
 };
 
 // One warp per (row, part and rank).
@@ -275,21 +276,33 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 2 : 1) adapter_sums_ke
     for (int j = 0; j < NW; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-#pragma unroll 2
-  for (int u = u0 + kw; u < u1; u += KW) {
-    const bool in = u * 32 + t * 8 < g.K;
-    uint4 xv[NW], av[MT][2];
+  // The operands of the next 32 k are loaded before the products of the last ones.
+  uint4 xv[NW], av[MT][2];
+  const auto load = [&](int u, uint4 (&xn)[NW], uint4 (&an)[MT][2]) {
+    const bool in = u < u1 && u * 32 + t * 8 < g.K;
 #pragma unroll
-    for (int j = 0; j < NW; ++j) xv[j] = in && live[j] ? load16(xr[j] + u * 32) : zero4();
+    for (int j = 0; j < NW; ++j) xn[j] = in && live[j] ? load16(xr[j] + u * 32) : zero4();
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf)
-        av[m][hf] = in && have[m][hf] ? load16(ar + (size_t)(m * 16 + hf * 8) * g.K + u * 32) : zero4();
+        an[m][hf] = in && have[m][hf] ? load16(ar + (size_t)(m * 16 + hf * 8) * g.K + u * 32) : zero4();
+  };
+  load(u0 + kw, xv, av);
+  for (int u = u0 + kw; u < u1; u += KW) {
+    uint4 xn[NW], an[MT][2];
+    load(u + KW, xn, an);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int j = 0; j < NW; ++j) mma_k32(acc[m][j], av[m][0], av[m][1], xv[j]);
+#pragma unroll
+    for (int j = 0; j < NW; ++j) xv[j] = xn[j];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      av[m][0] = an[m][0];
+      av[m][1] = an[m][1];
+    }
   }
   float* mine = sums_smem + (kw * TOK + tw * NW * 8) * PAD;
 #pragma unroll
@@ -314,7 +327,8 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 2 : 1) adapter_sums_ke
 }
 
 // ---- the second product and the sum with y: a warp takes 32 columns of 8 or 32 rows at a time; lane (g, t) ends with columns
-// 4 g .. 4 g + 3 of tokens 2 t and 2 t + 1 of every 8.
+// 4 g .. 4 g + 3 of tokens 2 t and 2 t + 1 of every 8.  B and y of the next columns are loaded between the products and the
+// stores of the last ones.
 //
 // KG: groups of 32 k (0: as many as there are).  FOLD (up to 16 k): the rests of the sums stand where the second 16 k of a group would, so
 // that one pass does for both.
@@ -325,45 +339,104 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_ker
   extern __shared__ __align__(16) unsigned char add_smem[];
   bf16* h = (bf16*)add_smem;                                  // [parts of the block][hi, lo][TOK][stride]
   __shared__ int rows[MAX_ROWS];
+  __shared__ long long y_at[TOK], out_at[TOK];                // where the rows begin
   __shared__ __align__(16) int ids[FEW_MAX + TILE_WARPS];
   __shared__ int found[2];
   mi_pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t = lane & 3;
-  const int cw = warp % CW, tw = warp / CW;
+  const int cw = warp % CW, tok0 = warp / CW * NW * 8;
   // (the kernel in front was started behind everything that wrote the ids and the operands, and started this one behind that)
   const Item item = get_item<NT>(g, blockIdx.y, rows, ids, found);
-  const int rank = rank_of(g, item.id);
+  const int rank = rank_of(g, item.id), R = g.R;
   const bf16* y = (const bf16*)g.y;
   bf16* out = (bf16*)g.out;
   int part, c_first, c_end;
   const bool there = find_chunk(g, blockIdx.x, g.span, part, c_first, c_end) && item.count > 0 && (rank > 0 || out != y);
+  c_end = min(c_end, c_first + g.span);
+  const int PR = g.P * R, stride = h_stride(R), np = g.pairs ? 2 : 1;
+
+  uint2 yv[NW][2];
+  uint4 w[KG ? KG : 1][2][2];
+  const int t8 = (FOLD ? t & 1 : t) * 8;
+  const bf16* b0 = (const bf16*)g.b + (size_t)max(item.id, 0) * g.N * R + t8;
+  const auto load_b = [&](int c, int k0, uint4 (&v)[2][2]) {
+    const bf16* b = b0 + (size_t)c * R + k0;
+    const bool in = rank > k0 + t8;                           // something of this lane's piece is there
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int j = 2 * hf + m;                             // column 4 g + j
+        v[m][hf] = in && c + j < c_end ? load16(b + j * R) : zero4();
+      }
+  };
+  const auto load_all_b = [&](int c) {
+    if (KG) {
+#pragma unroll
+      for (int k = 0; k < KG; ++k) load_b(c, k * 32, w[k]);
+    }
+  };
+  const auto load_y = [&](int c) {
+    if (!g.vec || c + 4 > c_end) return;
+#pragma unroll
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int tok = tok0 + j * 8 + 2 * t + i;
+        if (tok < item.count) yv[j][i] = *reinterpret_cast<const uint2*>(y + y_at[tok] + c);
+      }
+  };
+  int c0 = c_first + cw * 32;
+  if (g.constant && there) load_all_b(c0 + 4 * gq);
   mi_pdl_wait();
   if (!there) return;
-  c_end = min(c_end, c_first + g.span);
-  const int PR = g.P * g.R, stride = h_stride(g.R), np = g.pairs ? 2 : 1, r32 = FOLD ? 32 : (g.R + 31) / 32 * 32;
-
-  if (rank > 0) {
-    const float scale = g.scale ? g.scale[item.id] : 1.f;
-    const int width = FOLD ? 16 : r32;
-    for (int i = tid; i < np * TOK * width; i += TILE_THREADS) {
-      const int p = i / (TOK * width), tok = i / width % TOK, r = i % width;
-      float s = 0.f;
-      if (r < rank && tok < item.count) {
-        const float* from = g.h + (size_t)rows[tok] * PR + (part + p) * g.R + r;
-#pragma unroll 4
-        for (int k = 0; k < g.ks; ++k) s += __ldcg(from + (size_t)k * g.M * PR);
-        s *= scale;
-      }
-      bf16 hi, lo;
-      split_bf16(s, hi, lo);
-      bf16* to = h + ((p * 2 + 0) * TOK + tok) * stride + r;
-      to[0] = hi;
-      to[FOLD ? 16 : TOK * stride] = lo;
-    }
-    __syncthreads();
+  if (!g.constant) load_all_b(c0 + 4 * gq);
+  for (int i = tid; i < item.count; i += TILE_THREADS) {
+    y_at[i] = rows[i] * g.ldy;
+    out_at[i] = rows[i] * g.ldo;
   }
 
-  for (int c0 = c_first + cw * 32; c0 < c_end; c0 += CW * 32) {
+  if (rank > 0) {
+    // The sums over all of K, scaled, as two bfloat16 numbers each; whole groups of 32 k (what no sum stands for is zero).
+    const float scale = g.scale ? g.scale[item.id] : 1.f;
+    const int r4 = (FOLD ? 16 : (R + 31) / 32 * 32) / 4;
+    for (int l = lane; l < np * r4; l += 32) {
+      const int p = l >= r4, r = (l - p * r4) * 4;
+      const float* from = g.h + (part + p) * R + r;
+      float4 s[NT];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) s[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll NT == 1 ? 8 : 1
+      for (int k = 0; k < g.ks; ++k)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const int tok = warp + u * TILE_WARPS;
+          if (tok < item.count && r < rank) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(from + ((size_t)k * g.M + rows[tok]) * PR));
+            s[u].x += v.x;
+            s[u].y += v.y;
+            s[u].z += v.z;
+            s[u].w += v.w;
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const float f[4] = {s[u].x, s[u].y, s[u].z, s[u].w};
+        bf16 hi[4], lo[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) split_bf16(r + q < rank ? f[q] * scale : 0.f, hi[q], lo[q]);
+        bf16* to = h + (p * 2 * TOK + warp + u * TILE_WARPS) * stride + r;
+        *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
+        *reinterpret_cast<uint2*>(to + (FOLD ? 16 : TOK * stride)) = *reinterpret_cast<uint2*>(lo);
+      }
+    }
+  }
+  __syncthreads();
+  load_y(c0 + 4 * gq);
+
+  const bf16* h0 = h + (tok0 + gq) * stride + t * 8;
+  const int second = g.pairs ? 2 * TOK * stride : 0;          // the columns 2 i + 1 of pairs have sums of their own
+  for (; c0 < c_end; c0 += CW * 32) {
     const int c = c0 + 4 * gq;
     float acc[2][NW][4];
 #pragma unroll
@@ -372,49 +445,57 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_ker
       for (int j = 0; j < NW; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-    const bf16* b = (const bf16*)g.b + ((size_t)max(item.id, 0) * g.N + c) * g.R;
-    const auto group = [&](int k0) {
-      const int k = k0 + (FOLD ? t & 1 : t) * 8, n = rank - k;         // this lane's piece, and values of it that there are
-      uint4 w[2][2];
+    const auto group = [&](int k0, uint4 (&v)[2][2]) {
+      const int n = rank - k0 - t8;
+      if (n < 8 && n > 0) {                                   // what lies behind the rank
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int j = 2 * hf + m;                                    // column 4 g + j
-          w[m][hf] = n > 0 && c + j < c_end ? first_of(load16(b + (size_t)j * g.R + k), n) : zero4();
-        }
+          for (int hf = 0; hf < 2; ++hf) v[m][hf] = first_of(v[m][hf], n);
+      }
+      __syncwarp();
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const bf16* hp = h + (((g.pairs ? m : 0) * 2) * TOK + tw * NW * 8 + gq) * stride + k0 + t * 8;
+        const bf16* hp = h0 + k0 + (m ? second : 0);
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
-          mma_k32(acc[m][j], w[m][0], w[m][1], load16(hp + j * 8 * stride));
-          if (!FOLD) mma_k32(acc[m][j], w[m][0], w[m][1], load16(hp + (TOK + j * 8) * stride));
+          mma_k32(acc[m][j], v[m][0], v[m][1], load16(hp + j * 8 * stride));
+          if (!FOLD) mma_k32(acc[m][j], v[m][0], v[m][1], load16(hp + (TOK + j * 8) * stride));
         }
       }
     };
     if (KG) {
 #pragma unroll
       for (int k = 0; k < KG; ++k)
-        if (k * 32 < rank) group(k * 32);
+        if (k * 32 < rank) group(k * 32, w[k]);
     } else {
-      for (int k0 = 0; k0 < rank; k0 += 32) group(k0);
+      for (int k0 = 0; k0 < rank; k0 += 32) {
+        load_b(c, k0, w[0]);
+        group(k0, w[0]);
+      }
+    }
+    uint2 yc[NW][2];
+#pragma unroll
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) yc[j][i] = yv[j][i];
+    if (c0 + CW * 32 < c_end) {
+      load_all_b(c + CW * 32);
+      load_y(c + CW * 32);
     }
 #pragma unroll
     for (int j = 0; j < NW; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int tok = (tw * NW + j) * 8 + 2 * t + i;
+        const int tok = tok0 + j * 8 + 2 * t + i;
         if (tok >= item.count) continue;
-        const long long row = rows[tok];
-        const bf16* yp = y + row * g.ldy + c;
-        bf16* op = out + row * g.ldo + c;
+        bf16* op = out + out_at[tok] + c;
         const float d[4] = {acc[0][j][i], acc[1][j][i], acc[0][j][2 + i], acc[1][j][2 + i]};
         if (g.vec && c + 4 <= c_end) {
           Vec4<bf16> v;
-          float f[4];
-          v.load(yp);
+          v.v = yc[j][i];
           if (rank > 0) {
+            float f[4];
             v.get(f);
 #pragma unroll
             for (int q = 0; q < 4; ++q) f[q] += d[q];
@@ -422,6 +503,7 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_ker
           }
           v.store(op);
         } else {
+          const bf16* yp = y + y_at[tok] + c;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (c + q < c_end) op[q] = rank > 0 ? __float2bfloat16_rn(__bfloat162float(yp[q]) + d[q]) : yp[q];
@@ -589,11 +671,11 @@ extern "C" long long mi_adapter_scratch(const void* x, long long ldx, const void
 extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b,
                               void* out, long long ldo, const int* ids, const int* order, const void* items, const float* scale,
                               const int* ranks, float* h, int M, int N, int K, int n, int P, int R, int end0, int end1, int end2,
-                              int end3, int pairs, int dtype, cudaStream_t stream) {
+                              int end3, int pairs, int constant, int dtype, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   if (P < 1 || P > ADAPTER_MAX_PARTS) MI_REFUSE("adapter_add: %d parts, at most %d", P, ADAPTER_MAX_PARTS);
   AdapterArgs g = {x, ldx, y, ldy, out, ldo, a, b, ids, ranks, scale, h, M, N, K, n, P, R, {end0, end1, end2, end3}, pairs, 0, 0, 1,
-                   order, (const int4*)items};
+                   order, (const int4*)items, constant};
   if (in_pieces(x, ldx, a, b, M, K, n, P, R, dtype) && (M <= FEW_MAX || (order && items))) {
     const int max_items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : plan_items(M, n);
     if (max_items > 65535) MI_REFUSE("adapter_add: %d rows with %d adapters", M, n);
@@ -601,7 +683,9 @@ extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long 
     for (int p = 0; p + 1 < P && !pairs; ++p) starts4 = starts4 && g.ends[p] % 4 == 0;
     g.vec = starts4 && mi_aligned(y, 8) && mi_aligned(out, 8) && (M == 1 || (ldy % 4 == 0 && ldo % 4 == 0));
     g.ks = sum_parts(M, n, K, P, R);
-    g.span = M <= FEW_MAX ? 256 : 512;
+    // Blocks with many columns look for their rows and sums once for all of them; a few waves of blocks fill the chip.
+    g.span = 2048;
+    while (g.span > 256 && (long long)max_items * count_chunks(g, g.span) < (M <= FEW_MAX ? 3 : 4) * 148) g.span /= 2;
     const cudaError_t e = M <= FEW_MAX ? launch_tiles<1>(g, max_items, stream) : launch_tiles<8>(g, max_items, stream);
     if (e != cudaSuccess) return refused_by_cuda(e);
     MI_RETURN_LAUNCH_STATUS();

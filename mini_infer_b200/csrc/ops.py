@@ -440,7 +440,7 @@ def _sig_adapters(lib: ctypes.CDLL) -> None:
     ll = ctypes.c_longlong
     lib.mi_adapter_add.argtypes = [c_void_p, ll, c_void_p, ll, c_void_p, c_void_p, c_void_p, ll, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                   c_int, c_int, c_int, c_void_p]
+                                   c_int, c_int, c_int, c_int, c_void_p]
     lib.mi_adapter_scratch.argtypes = [c_void_p, ll, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int]
     lib.mi_adapter_scratch.restype = ll
     lib.mi_adapter_plan_sizes.argtypes = [c_int, c_int, ctypes.POINTER(c_int)]
@@ -3095,7 +3095,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
                     device=x.device)
     rc = lib.mi_adapter_add(_ptr(y), y.stride(0), _ptr(x), x.stride(0), _ptr(a), _ptr(b), _ptr(out), out.stride(0),
                             _ptr(plan.ids), _ptr(plan.order), _ptr(plan.items), _ptr(scale), _ptr(ranks), _ptr(h), M, N, K, n, P, R,
-                            *ends, 1 if pairs else 0, code, _stream())
+                            *ends, 1 if pairs else 0, 1 if w_constant else 0, code, _stream())
     _finish(lib, rc, what)
     return out
 
