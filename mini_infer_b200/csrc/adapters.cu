@@ -6,9 +6,10 @@
 // A projection may be several merged along its columns; column c belongs to part p(c), and every part has an A of its own:
 // A is [adapters, parts, R, K], B [adapters, N, R].  Parts lie side by side, or (pairs) two of them alternate column by column.
 // An adapter's own rank may be below R; what lies behind it is not read.  Sums are fp32.
-#include "common.cuh"
+#include "bulk_copy.cuh"
 
 MI_DEFINE_ERROR_API()
+MI_DEFINE_STATUS_API(mi_adapters_status)
 
 #define ADAPTER_MAX_PARTS 4
 #define ADAPTER_THREADS 256
@@ -25,7 +26,8 @@ struct AdapterArgs {
   const int* ids;
   const int* ranks;
   const float* scale;
-  float* h;                       // [M, P R]
+  float* h;                       // [parts of the sum over K][M][P R] the sums of the first product
+  bf16* pairs_of_h;               // [M][P][2][R up to 16s] the same over all of K, as pairs of bfloat16 numbers (many rows)
   int M, N, K, n, P, R;
   int ends[ADAPTER_MAX_PARTS];    // where each part's columns end (side by side)
   int pairs;
@@ -160,15 +162,19 @@ inline int count_chunks(const AdapterArgs& g, int size) {
   return n;
 }
 
-// ---- items: up to 8 NT rows that share an adapter (or have none)
+// ---- few rows: items of up to 8 rows that share an adapter (or have none)
 //
-// For up to FEW_MAX rows every block finds its item in the ids; for more, adapter_plan has put the rows in order.
+// For up to FEW_MAX rows every block finds its item in the ids; for more, adapter_plan has put the rows in order.  The products run on
+// mma.sync, which costs 32 cycles for 16 x 8 x 16 on this chip: enough for rows by the dozen, whose time the adapters' bytes
+// make.
 
 #define TILE_THREADS 256
 #define TILE_WARPS (TILE_THREADS / 32)
 #define FEW_MAX 128           // rows of a call whose items the blocks find by themselves
+#define FEW_ROWS 8            // rows of an item
 #define SUM_GROUP 64          // sums of the first product that a block makes
-#define MAX_ROWS 64           // of an item
+#define MAX_ROWS 128          // rows of an item of a plan
+#define SUB_ITEMS (MAX_ROWS / FEW_ROWS)
 
 struct Item {
   int id, count;              // adapter (-1: none), rows
@@ -215,102 +221,83 @@ __device__ __forceinline__ Item few_item(const AdapterArgs& g, int index, int* r
   return item;
 }
 
-template <int NT>
 __device__ __forceinline__ Item get_item(const AdapterArgs& g, int index, int* rows, int* ids, int* found) {
-  if (NT == 1) return few_item(g, index, rows, ids, found);
-  const int4 v = __ldcg(g.items + index);
-  if (threadIdx.x < (unsigned)v.z) rows[threadIdx.x] = __ldcg(g.order + v.y + threadIdx.x);
+  if (!g.items) return few_item(g, index, rows, ids, found);
+  const int4 v = __ldcg(g.items + index / SUB_ITEMS);
+  const int first = index % SUB_ITEMS * FEW_ROWS, count = max(0, min(FEW_ROWS, v.z - first));
+  if (threadIdx.x < (unsigned)count) rows[threadIdx.x] = __ldcg(g.order + v.y + first + threadIdx.x);
   __syncthreads();
-  return Item{v.x, v.z};
+  return Item{v.x, count};
 }
 
 __device__ __forceinline__ int rank_of(const AdapterArgs& g, int id) {
   return id < 0 ? 0 : g.ranks ? max(0, min(__ldcg(g.ranks + id), g.R)) : g.R;
 }
 
-// ---- the first product: a block makes SUM_GROUP sums of an item over a share of K.  NT: 8-token columns of tiles of an item.
-//
-// Warps cut the share of K between them (with 64 tokens, four ways, and the tokens two ways), their sums meet in shared memory
-// and go to h as one part of the sum over K.
-
-template <int NT>
-__global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 2 : 1) adapter_sums_kernel(const AdapterArgs g) {
-  constexpr int TW = NT == 1 ? 1 : 2, KW = TILE_WARPS / TW, NW = NT / TW, TOK = 8 * NT, MT = SUM_GROUP / 16, PAD = SUM_GROUP + 4;
+// The first product: a block makes SUM_GROUP sums of an item over a share of K.  Its warps cut the share between them, their sums meet in
+// shared memory and go to h as one part of the sum over K.
+__global__ void __launch_bounds__(TILE_THREADS, 2) adapter_sums_kernel(const AdapterArgs g) {
+  constexpr int MT = SUM_GROUP / 16, PAD = SUM_GROUP + 4;
   // The kernel behind this one starts once the ids and operands of both are there; it waits for these sums alone.
   mi_pdl_wait();
   mi_pdl_launch_dependents();
-  extern __shared__ __align__(16) float sums_smem[];          // [KW][TOK][PAD]
-  __shared__ int rows[MAX_ROWS];
+  __shared__ __align__(16) float shares[TILE_WARPS][FEW_ROWS][PAD];
+  __shared__ int rows[FEW_ROWS];
   __shared__ __align__(16) int ids[FEW_MAX + TILE_WARPS];
   __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t = lane & 3;
-  const int kw = warp % KW, tw = warp / KW;
-  const Item item = get_item<NT>(g, blockIdx.y, rows, ids, found);
+  const Item item = get_item(g, blockIdx.y, rows, ids, found);
   const int rank = rank_of(g, item.id);
   if (item.count == 0 || rank == 0) return;
   const int PR = g.P * g.R, m0 = blockIdx.z * SUM_GROUP;
   const int units = (g.K + 31) / 32;                          // 32 values of k: 64 bytes of a row
   const int u0 = (int)((long long)units * blockIdx.x / g.ks), u1 = (int)((long long)units * (blockIdx.x + 1) / g.ks);
 
-  const bf16* xr[NW];
-  bool live[NW];
-#pragma unroll
-  for (int j = 0; j < NW; ++j) {
-    const int tok = (tw * NW + j) * 8 + gq;
-    live[j] = tok < item.count;
-    xr[j] = (const bf16*)g.x + (long long)rows[live[j] ? tok : 0] * g.ldx + t * 8;
-  }
+  const bool live = gq < item.count;
+  const bf16* xr = (const bf16*)g.x + (long long)rows[live ? gq : 0] * g.ldx + t * 8;
   const bf16* ar = (const bf16*)g.a + ((size_t)item.id * PR + m0 + gq) * g.K + t * 8;
-  bool have[MT][2];
+  bool have[MT][2], any[MT];                                  // sums below the adapter's rank; tiles that have one
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int r = m0 + m * 16 + hf * 8 + gq;
       have[m][hf] = r < PR && r % g.R < rank;
     }
-  float acc[MT][NW][4];
+    any[m] = __any_sync(0xffffffffu, have[m][0] || have[m][1]);
+  }
+  float acc[MT][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int j = 0; j < NW; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+    for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
   // The operands of the next 32 k are loaded before the products of the last ones.
-  uint4 xv[NW], av[MT][2];
-  const auto load = [&](int u, uint4 (&xn)[NW], uint4 (&an)[MT][2]) {
+  uint4 xv, av[MT][2];
+  const auto load = [&](int u, uint4& xn, uint4 (&an)[MT][2]) {
     const bool in = u < u1 && u * 32 + t * 8 < g.K;
-#pragma unroll
-    for (int j = 0; j < NW; ++j) xn[j] = in && live[j] ? load16(xr[j] + u * 32) : zero4();
+    xn = in && live ? load16(xr + u * 32) : zero4();
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf)
         an[m][hf] = in && have[m][hf] ? load16(ar + (size_t)(m * 16 + hf * 8) * g.K + u * 32) : zero4();
   };
-  load(u0 + kw, xv, av);
-  for (int u = u0 + kw; u < u1; u += KW) {
-    uint4 xn[NW], an[MT][2];
-    load(u + KW, xn, an);
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int j = 0; j < NW; ++j) mma_k32(acc[m][j], av[m][0], av[m][1], xv[j]);
-#pragma unroll
-    for (int j = 0; j < NW; ++j) xv[j] = xn[j];
+  load(u0 + warp, xv, av);
+  for (int u = u0 + warp; u < u1; u += TILE_WARPS) {
+    uint4 xn, an[MT][2];
+    load(u + TILE_WARPS, xn, an);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
+      if (any[m]) mma_k32(acc[m], av[m][0], av[m][1], xv);
       av[m][0] = an[m][0];
       av[m][1] = an[m][1];
     }
+    xv = xn;
   }
-  float* mine = sums_smem + (kw * TOK + tw * NW * 8) * PAD;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int j = 0; j < NW; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mine[(j * 8 + 2 * t + (i & 1)) * PAD + m * 16 + (i >> 1) * 8 + gq] = acc[m][j][i];
+    for (int i = 0; i < 4; ++i) shares[warp][2 * t + (i & 1)][m * 16 + (i >> 1) * 8 + gq] = acc[m][i];
   __syncthreads();
   float* h = g.h + (size_t)blockIdx.x * g.M * PR + m0;
   for (int i = tid; i < item.count * (SUM_GROUP / 4); i += TILE_THREADS) {
@@ -318,35 +305,31 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 2 : 1) adapter_sums_ke
     if (m0 + r >= PR) continue;                               // (PR is a multiple of 8)
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < KW; ++w) {
-      const float4 v = *reinterpret_cast<const float4*>(sums_smem + (w * TOK + tok) * PAD + r);
+    for (int w = 0; w < TILE_WARPS; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(&shares[w][tok][r]);
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
     *reinterpret_cast<float4*>(h + (size_t)rows[tok] * PR + r) = s;
   }
 }
 
-// ---- the second product and the sum with y: a warp takes 32 columns of 8 or 32 rows at a time; lane (g, t) ends with columns
-// 4 g .. 4 g + 3 of tokens 2 t and 2 t + 1 of every 8.  B and y of the next columns are loaded between the products and the
-// stores of the last ones.
+// The second product and the sum with y: a warp takes 32 columns of the item at a time; lane (g, t) ends with columns
+// 4 g .. 4 g + 3 of tokens 2 t and 2 t + 1.  B and y of the next columns are loaded between the products and the stores of the last
+// ones.
 //
-// KG: groups of 32 k (0: as many as there are).  FOLD (up to 16 k): the rests of the sums stand where the second 16 k of a group would, so
-// that one pass does for both.
-
-template <int NT, int KG, bool FOLD>
-__global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_kernel(const AdapterArgs g) {
-  constexpr int TW = NT == 1 ? 1 : 2, CW = TILE_WARPS / TW, NW = NT / TW, TOK = 8 * NT;
+// KG: groups of 32 k (0: as many as there are).  Sums and their rests take two passes, but for items of up to four rows, where the rests
+// stand in the place of four more tokens, and (FOLD) for up to 16 k, where they stand in the place of 16 more.
+template <int KG, bool FOLD>
+__global__ void __launch_bounds__(TILE_THREADS, 3) adapter_add_kernel(const AdapterArgs g) {
   extern __shared__ __align__(16) unsigned char add_smem[];
-  bf16* h = (bf16*)add_smem;                                  // [parts of the block][hi, lo][TOK][stride]
-  __shared__ int rows[MAX_ROWS];
-  __shared__ long long y_at[TOK], out_at[TOK];                // where the rows begin
+  bf16* h = (bf16*)add_smem;                                  // [parts of the block][hi, lo][FEW_ROWS][stride]
+  __shared__ int rows[FEW_ROWS];
   __shared__ __align__(16) int ids[FEW_MAX + TILE_WARPS];
   __shared__ int found[2];
   mi_pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t = lane & 3;
-  const int cw = warp % CW, tok0 = warp / CW * NW * 8;
   // (the kernel in front was started behind everything that wrote the ids and the operands, and started this one behind that)
-  const Item item = get_item<NT>(g, blockIdx.y, rows, ids, found);
+  const Item item = get_item(g, blockIdx.y, rows, ids, found);
   const int rank = rank_of(g, item.id), R = g.R;
   const bf16* y = (const bf16*)g.y;
   bf16* out = (bf16*)g.out;
@@ -355,7 +338,7 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_ker
   c_end = min(c_end, c_first + g.span);
   const int PR = g.P * R, stride = h_stride(R), np = g.pairs ? 2 : 1;
 
-  uint2 yv[NW][2];
+  uint2 yv[2];
   uint4 w[KG ? KG : 1][2][2];
   const int t8 = (FOLD ? t & 1 : t) * 8;
   const bf16* b0 = (const bf16*)g.b + (size_t)max(item.id, 0) * g.N * R + t8;
@@ -376,25 +359,19 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_ker
       for (int k = 0; k < KG; ++k) load_b(c, k * 32, w[k]);
     }
   };
-  const auto load_y = [&](int c) {
-    if (!g.vec || c + 4 > c_end) return;
-#pragma unroll
-    for (int j = 0; j < NW; ++j)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int tok = tok0 + j * 8 + 2 * t + i;
-        if (tok < item.count) yv[j][i] = *reinterpret_cast<const uint2*>(y + y_at[tok] + c);
-      }
-  };
-  int c0 = c_first + cw * 32;
+  int c0 = c_first + warp * 32;
   if (g.constant && there) load_all_b(c0 + 4 * gq);
   mi_pdl_wait();
   if (!there) return;
   if (!g.constant) load_all_b(c0 + 4 * gq);
-  for (int i = tid; i < item.count; i += TILE_THREADS) {
-    y_at[i] = rows[i] * g.ldy;
-    out_at[i] = rows[i] * g.ldo;
-  }
+  const int mine[2] = {2 * t < item.count ? rows[2 * t] : -1, 2 * t + 1 < item.count ? rows[2 * t + 1] : -1};
+  const auto load_y = [&](int c) {
+    if (!g.vec || c + 4 > c_end) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (mine[i] >= 0) yv[i] = *reinterpret_cast<const uint2*>(y + mine[i] * g.ldy + c);
+  };
+  load_y(c0 + 4 * gq);
 
   if (rank > 0) {
     // The sums over all of K, scaled, as two bfloat16 numbers each; whole groups of 32 k (what no sum stands for is zero).
@@ -402,49 +379,39 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_ker
     const int r4 = (FOLD ? 16 : (R + 31) / 32 * 32) / 4;
     for (int l = lane; l < np * r4; l += 32) {
       const int p = l >= r4, r = (l - p * r4) * 4;
-      const float* from = g.h + (part + p) * R + r;
-      float4 s[NT];
-#pragma unroll
-      for (int u = 0; u < NT; ++u) s[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll NT == 1 ? 8 : 1
-      for (int k = 0; k < g.ks; ++k)
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          const int tok = warp + u * TILE_WARPS;
-          if (tok < item.count && r < rank) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(from + ((size_t)k * g.M + rows[tok]) * PR));
-            s[u].x += v.x;
-            s[u].y += v.y;
-            s[u].z += v.z;
-            s[u].w += v.w;
-          }
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (warp < item.count && r < rank) {
+        const float* from = g.h + (size_t)rows[warp] * PR + (part + p) * R + r;
+#pragma unroll 8
+        for (int k = 0; k < g.ks; ++k) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(from + (size_t)k * g.M * PR));
+          s.x += v.x;
+          s.y += v.y;
+          s.z += v.z;
+          s.w += v.w;
         }
-#pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        const float f[4] = {s[u].x, s[u].y, s[u].z, s[u].w};
-        bf16 hi[4], lo[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) split_bf16(r + q < rank ? f[q] * scale : 0.f, hi[q], lo[q]);
-        bf16* to = h + (p * 2 * TOK + warp + u * TILE_WARPS) * stride + r;
-        *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
-        *reinterpret_cast<uint2*>(to + (FOLD ? 16 : TOK * stride)) = *reinterpret_cast<uint2*>(lo);
       }
+      const float f[4] = {s.x, s.y, s.z, s.w};
+      bf16 hi[4], lo[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) split_bf16(r + q < rank ? f[q] * scale : 0.f, hi[q], lo[q]);
+      bf16* to = h + (p * 2 * FEW_ROWS + warp) * stride + r;
+      *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
+      *reinterpret_cast<uint2*>(to + (FOLD ? 16 : FEW_ROWS * stride)) = *reinterpret_cast<uint2*>(lo);
     }
   }
   __syncthreads();
-  load_y(c0 + 4 * gq);
 
-  const bf16* h0 = h + (tok0 + gq) * stride + t * 8;
-  const int second = g.pairs ? 2 * TOK * stride : 0;          // the columns 2 i + 1 of pairs have sums of their own
-  for (; c0 < c_end; c0 += CW * 32) {
+  const bool half = !FOLD && item.count <= 4;                 // tokens 4 .. 7 are the rests of tokens 0 .. 3
+  const bf16* h0 = h + (half ? (gq & 3) + (gq >> 2) * FEW_ROWS : gq) * stride + t * 8;
+  const int second = g.pairs ? 2 * FEW_ROWS * stride : 0;     // the columns 2 i + 1 of pairs have sums of their own
+  for (; c0 < c_end; c0 += TILE_WARPS * 32) {
     const int c = c0 + 4 * gq;
-    float acc[2][NW][4];
+    float acc[2][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int j = 0; j < NW; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+      for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
     const auto group = [&](int k0, uint4 (&v)[2][2]) {
       const int n = rank - k0 - t8;
       if (n < 8 && n > 0) {                                   // what lies behind the rank
@@ -457,11 +424,8 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_ker
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const bf16* hp = h0 + k0 + (m ? second : 0);
-#pragma unroll
-        for (int j = 0; j < NW; ++j) {
-          mma_k32(acc[m][j], v[m][0], v[m][1], load16(hp + j * 8 * stride));
-          if (!FOLD) mma_k32(acc[m][j], v[m][0], v[m][1], load16(hp + (TOK + j * 8) * stride));
-        }
+        mma_k32(acc[m], v[m][0], v[m][1], load16(hp));
+        if (!FOLD && !half) mma_k32(acc[m], v[m][0], v[m][1], load16(hp + FEW_ROWS * stride));
       }
     };
     if (KG) {
@@ -474,42 +438,405 @@ __global__ void __launch_bounds__(TILE_THREADS, NT == 1 ? 3 : 2) adapter_add_ker
         group(k0, w[0]);
       }
     }
-    uint2 yc[NW][2];
+    const uint2 yc[2] = {yv[0], yv[1]};
+    if (c0 + TILE_WARPS * 32 < c_end) {
+      load_all_b(c + TILE_WARPS * 32);
+      load_y(c + TILE_WARPS * 32);
+    }
+    if (half) {
 #pragma unroll
-    for (int j = 0; j < NW; ++j)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) yc[j][i] = yv[j][i];
-    if (c0 + CW * 32 < c_end) {
-      load_all_b(c + CW * 32);
-      load_y(c + CW * 32);
+        for (int i = 0; i < 4; ++i) acc[m][i] += __shfl_xor_sync(0xffffffffu, acc[m][i], 2);
     }
 #pragma unroll
-    for (int j = 0; j < NW; ++j)
+    for (int i = 0; i < 2; ++i) {
+      if (mine[i] < 0) continue;
+      bf16* op = out + mine[i] * g.ldo + c;
+      const float d[4] = {acc[0][i], acc[1][i], acc[0][2 + i], acc[1][2 + i]};
+      if (g.vec && c + 4 <= c_end) {
+        Vec4<bf16> v;
+        v.v = yc[i];
+        if (rank > 0) {
+          float f[4];
+          v.get(f);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int tok = tok0 + j * 8 + 2 * t + i;
-        if (tok >= item.count) continue;
-        bf16* op = out + out_at[tok] + c;
-        const float d[4] = {acc[0][j][i], acc[1][j][i], acc[0][j][2 + i], acc[1][j][2 + i]};
-        if (g.vec && c + 4 <= c_end) {
-          Vec4<bf16> v;
-          v.v = yc[j][i];
-          if (rank > 0) {
-            float f[4];
-            v.get(f);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) f[q] += d[q];
-            v.set(f);
-          }
-          v.store(op);
-        } else {
-          const bf16* yp = y + y_at[tok] + c;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (c + q < c_end) op[q] = rank > 0 ? __float2bfloat16_rn(__bfloat162float(yp[q]) + d[q]) : yp[q];
+          for (int q = 0; q < 4; ++q) f[q] += d[q];
+          v.set(f);
         }
+        v.store(op);
+      } else {
+        const bf16* yp = y + mine[i] * g.ldy + c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (c + q < c_end) op[q] = rank > 0 ? __float2bfloat16_rn(__bfloat162float(yp[q]) + d[q]) : yp[q];
       }
+    }
   }
+}
+
+// ---- many rows: both products on tcgen05, items of up to 128 rows
+//
+// Operands lie in shared memory as the tensor cores want them: rows of 64 k (128 bytes), 16-byte pieces permuted within a row by the
+// row's number modulo 8.  They are brought there piece by piece with cp.async, which gathers the rows of an item from wherever they
+// are and leaves zeros for what is not there (rows behind the last, k behind the end or the rank).
+
+#define TC_THREADS 256
+#define TC_ROWS 128
+#define TC_ATOM (TC_ROWS * 128)      // bytes of 128 rows of 64 k
+#define SUMS_STAGES 3
+#define SUMS_STAGE_BYTES (2 * TC_ATOM)
+#define ADD_COLS 128                 // columns of a tile of the result
+#define ADD_MAX_STAGES 3
+
+__device__ __forceinline__ void copy_piece(uint32_t to, const void* from, int bytes) {      // the rest of 16 bytes: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// An operand of rows of 64 k, 128-byte swizzle, groups of 8 rows 1024 bytes apart
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// bfloat16 x bfloat16 -> fp32, 128 rows by n columns
+__device__ __forceinline__ uint32_t product_desc(int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+               "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void smem_for_tensor_cores() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_load32(uint32_t from, uint32_t (&r)[32]) {      // 32 columns of this thread's row
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(from)
+      : "memory");
+}
+__device__ __forceinline__ void tc_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+
+// Tensor memory for a block, by its first warp; the address is in `holder` behind a barrier of the block.  Only then may the next kernel's
+// blocks come: one that took the memory while it waits for this kernel would never get an answer.
+__device__ __forceinline__ void tc_alloc(uint32_t* holder, int columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(holder)), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tc_free(uint32_t at, int columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(at), "r"(columns) : "memory");
+}
+
+struct TcBlock {
+  uint64_t bars[SUMS_STAGES > ADD_MAX_STAGES ? SUMS_STAGES : ADD_MAX_STAGES];      // the products that read a stage have ended
+  uint32_t tmem;
+  int give_up;
+  int rows[TC_ROWS];
+};
+
+// The item, its rows, barriers and tensor memory; false (for the whole block): nothing to do.
+__device__ __forceinline__ bool tc_begin(const AdapterArgs& g, TcBlock& s, int4& item, int& rank) {
+  item = __ldcg(g.items + blockIdx.y);
+  rank = rank_of(g, item.x);
+  if (threadIdx.x < TC_ROWS) s.rows[threadIdx.x] = (int)threadIdx.x < item.z ? __ldcg(g.order + item.y + threadIdx.x) : 0;
+  if (threadIdx.x < sizeof(s.bars) / sizeof(s.bars[0])) mbar_init(&s.bars[threadIdx.x], 1);
+  if (threadIdx.x == 0) s.give_up = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  return item.z > 0;
+}
+__device__ __forceinline__ void tc_ready(TcBlock& s, int columns) {
+  if (threadIdx.x < 32) tc_alloc(&s.tmem, columns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  mi_pdl_launch_dependents();
+}
+// A bounded wait of all threads for the products of a stage; false for all of them when it ran out.
+__device__ __forceinline__ bool tc_wait(TcBlock& s, int stage, uint32_t parity) {
+  mbar_wait(&s.bars[stage], parity, &s.give_up);
+  return __syncthreads_and(!*(volatile int*)&s.give_up);
+}
+
+// The first product: up to 128 sums of an item over a share of K, through a ring of stages of 64 k.
+__global__ void __launch_bounds__(TC_THREADS) adapter_sums_tc_kernel(const AdapterArgs g) {
+  mi_pdl_wait();
+  extern __shared__ unsigned char tc_smem[];
+  __shared__ TcBlock s;
+  const uint32_t base = (smem_u32(tc_smem) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int4 item;
+  int rank;
+  if (!tc_begin(g, s, item, rank) || rank == 0) return;
+  tc_ready(s, 128);
+  const int PR = g.P * g.R, m0 = blockIdx.z * 128, sums = min(128, PR - m0), n = (sums + 15) & ~15;
+  const int blocks = (g.K + 63) / 64;
+  const int u0 = (int)((long long)blocks * blockIdx.x / g.ks), u1 = (int)((long long)blocks * (blockIdx.x + 1) / g.ks);
+
+  // piece `tid % 8` of four rows of x and of A, 32 rows apart
+  const int piece = tid & 7, r0 = tid >> 3;
+  const uint32_t place = r0 * 128 + ((piece ^ (r0 & 7)) << 4);
+  const bf16 *xr[4], *ar[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = r0 + 32 * j, pr = m0 + row;
+    xr[j] = row < item.z ? (const bf16*)g.x + (long long)s.rows[row] * g.ldx + piece * 8 : nullptr;
+    ar[j] = row < sums && pr % g.R < rank ? (const bf16*)g.a + ((size_t)item.x * PR + pr) * g.K + piece * 8 : nullptr;
+  }
+  const auto load = [&](int u) {
+    if (u < u1) {
+      const uint32_t to = base + (u - u0) % SUMS_STAGES * SUMS_STAGE_BYTES + place;
+      const bool in = u * 64 + piece * 8 < g.K;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool x_in = in && xr[j], a_in = in && ar[j];
+        copy_piece(to + j * 4096, x_in ? xr[j] + u * 64 : (const bf16*)g.x, x_in ? 16 : 0);
+        if (r0 + 32 * j < n) copy_piece(to + TC_ATOM + j * 4096, a_in ? ar[j] + u * 64 : (const bf16*)g.a, a_in ? 16 : 0);
+      }
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < SUMS_STAGES - 1; ++i) load(u0 + i);
+  const uint32_t desc = product_desc(n);
+  bool ok = true;
+  for (int u = u0; u < u1; ++u) {
+    copies_wait<SUMS_STAGES - 2>();
+    smem_for_tensor_cores();
+    __syncthreads();
+    const int i = u - u0, stage = i % SUMS_STAGES;
+    if (tid == 0) {
+      tc_fence_after();
+      const uint32_t at = base + stage * SUMS_STAGE_BYTES;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tc_mma(s.tmem, operand_desc(at + k * 32), operand_desc(at + TC_ATOM + k * 32), desc, i > 0 || k > 0);
+      tc_commit(&s.bars[stage]);
+    }
+    // the stage of the products before these is free once they have ended
+    if (i > 0 && !tc_wait(s, (i - 1) % SUMS_STAGES, ((i - 1) / SUMS_STAGES) & 1)) {
+      ok = false;
+      break;
+    }
+    load(u + SUMS_STAGES - 1);
+  }
+  copies_wait<0>();
+  const int last = u1 - u0 - 1;
+  if (ok) ok = tc_wait(s, last % SUMS_STAGES, (last / SUMS_STAGES) & 1);
+  if (ok) {
+    tc_fence_after();
+    const int row = (warp & 3) * 32 + lane;
+    float* h = g.h + ((size_t)blockIdx.x * g.M + s.rows[row]) * PR + m0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int c = (warp >> 2) * 64 + q * 32;
+      if (c >= sums) break;                                   // (the whole warp)
+      uint32_t v[32];
+      tc_load32(s.tmem + ((uint32_t)(warp & 3) << 21) + c, v);
+      tc_load_wait();
+      if (row < item.z) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 4)
+          if (c + k < sums) *reinterpret_cast<uint4*>(h + c + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (tid < 32) tc_free(s.tmem, 128);
+}
+
+// Where the rests of a part's sums stand behind the sums, in elements; whole groups of 16 k
+__host__ __device__ inline int padded_rank(int R) { return (R + 15) & ~15; }
+
+// The sums over all of K, scaled, as pairs of bfloat16 numbers: four sums a thread.
+__global__ void __launch_bounds__(256) adapter_pairs_kernel(const AdapterArgs g) {
+  mi_pdl_wait();
+  mi_pdl_launch_dependents();
+  const int rp = padded_rank(g.R), quarter = rp / 4, per_row = g.P * quarter;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)g.M * per_row) return;
+  const int row = (int)(i / per_row), p = (int)(i % per_row) / quarter, r = (int)(i % per_row) % quarter * 4;
+  const int id = g.ids[row];
+  if (id < 0 || id >= g.n) return;
+  const int rank = rank_of(g, id), PR = g.P * g.R;
+  const float scale = g.scale ? g.scale[id] : 1.f;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (r < rank) {
+    const float* from = g.h + (size_t)row * PR + p * g.R + r;
+#pragma unroll 4
+    for (int k = 0; k < g.ks; ++k) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(from + (size_t)k * g.M * PR));
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+  }
+  const float f[4] = {s.x, s.y, s.z, s.w};
+  bf16 hi[4], lo[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) split_bf16(r + q < rank ? f[q] * scale : 0.f, hi[q], lo[q]);
+  bf16* to = g.pairs_of_h + ((size_t)row * g.P + p) * 2 * rp + r;
+  *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
+  *reinterpret_cast<uint2*>(to + rp) = *reinterpret_cast<uint2*>(lo);
+}
+
+// Shared memory of the second product: the item's sums, then stages of B and of y
+__host__ __device__ inline int sums_atoms(int R) { return (2 * padded_rank(R) + 63) / 64; }      // a part's sums and rests
+__host__ __device__ inline int b_atoms(int R) { return (padded_rank(R) + 63) / 64; }
+__host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_ATOM + TC_ROWS * ADD_COLS * 2; }
+
+// The second product and the sum with y, in tiles of 128 columns: the products run from shared memory into tensor memory, y
+// waits in shared memory in rows of 256 bytes (16-byte pieces permuted by the row, so that a thread of the sum, which has a row,
+// and a thread of the copies, which has a piece of it, both touch all banks), and the result leaves the way y came.
+template <int STAGES>
+__global__ void __launch_bounds__(TC_THREADS) adapter_add_tc_kernel(const AdapterArgs g) {
+  extern __shared__ unsigned char tc_smem[];
+  __shared__ TcBlock s;
+  mi_pdl_wait();
+  const uint32_t base = (smem_u32(tc_smem) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = g.R;
+  int4 item;
+  int rank, part, c_first, c_end;
+  const bool any = tc_begin(g, s, item, rank);
+  const bf16* y = (const bf16*)g.y;
+  bf16* out = (bf16*)g.out;
+  if (!find_chunk(g, blockIdx.x, g.span, part, c_first, c_end) || !any || (rank == 0 && out == y)) return;
+  c_end = min(c_end, c_first + g.span);
+  const int rows = item.z;
+  if (rank == 0) {                                            // rows without an adapter: 8 columns a thread
+    __syncthreads();
+    const int pieces = (c_end - c_first) / 8;
+    for (int i = tid; i < rows * pieces; i += TC_THREADS) {
+      const long long row = s.rows[i / pieces];
+      const int c = c_first + i % pieces * 8;
+      *reinterpret_cast<uint4*>(out + row * g.ldo + c) = load16(y + row * g.ldy + c);
+    }
+    return;
+  }
+  tc_ready(s, 128);
+  const int np = g.pairs ? 2 : 1, rp = padded_rank(R), ha = sums_atoms(R), ba = b_atoms(R);
+  const uint32_t h_at = base, stages_at = base + np * ha * TC_ATOM, stage_bytes = add_stage_bytes(R);
+
+  // the item's sums
+  const int h_pieces = 2 * rp / 8;
+  for (int i = tid; i < np * rows * h_pieces; i += TC_THREADS) {
+    const int q = i % h_pieces, row = i / h_pieces % rows, p = i / h_pieces / rows;
+    copy_piece(h_at + (p * ha + q / 8) * TC_ATOM + row * 128 + (((q & 7) ^ (row & 7)) << 4),
+               g.pairs_of_h + ((size_t)s.rows[row] * g.P + part + p) * 2 * rp + q * 8, 16);
+  }
+  const int tiles = (c_end - c_first + ADD_COLS - 1) / ADD_COLS, b_pieces = rp / 8;
+  const bf16* b = (const bf16*)g.b + (size_t)item.x * g.N * R;
+  const auto load = [&](int i) {
+    if (i < tiles) {
+      const int c = c_first + i * ADD_COLS;
+      const uint32_t to = stages_at + i % STAGES * stage_bytes;
+      // rows of B: the tile's columns, of pairs the first ones and then the second ones
+      for (int j = tid; j < ADD_COLS * b_pieces; j += TC_THREADS) {
+        const int q = j % b_pieces, col = j / b_pieces;
+        const int from = c + (g.pairs ? (col & 63) * 2 + (col >> 6) : col);
+        const int there = from < c_end ? max(0, min(8, rank - q * 8)) : 0;
+        copy_piece(to + q / 8 * TC_ATOM + col * 128 + (((q & 7) ^ (col & 7)) << 4), there ? b + (size_t)from * R + q * 8 : b, there * 2);
+      }
+      const uint32_t y_to = to + ba * TC_ATOM;
+#pragma unroll
+      for (int j = 0; j < TC_ROWS * 16 / TC_THREADS; ++j) {
+        const int row = (tid >> 4) + j * (TC_THREADS / 16), q = tid & 15;
+        if (row < rows && c + q * 8 < c_end)
+          copy_piece(y_to + row * 256 + ((q ^ (row & 15)) << 4), y + (long long)s.rows[row] * g.ldy + c + q * 8, 16);
+      }
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) load(i);
+  if (STAGES == 1) load(0);
+  const uint32_t desc = product_desc(g.pairs ? ADD_COLS / 2 : ADD_COLS);
+  bool ok = true;
+  for (int i = 0; i < tiles; ++i) {
+    copies_wait<(STAGES > 1 ? STAGES - 2 : 0)>();
+    smem_for_tensor_cores();
+    __syncthreads();
+    const int stage = i % STAGES;
+    const uint32_t at = stages_at + stage * stage_bytes;
+    if (tid == 0) {
+      tc_fence_after();
+      for (int p = 0; p < np; ++p)
+        for (int k = 0; k < rp; k += 16) {
+          const uint64_t bd = operand_desc(at + p * 64 * 128 + k / 64 * TC_ATOM + k % 64 * 2);
+          for (int lo = 0; lo < 2; ++lo) {
+            const int e = k + lo * rp;
+            tc_mma(s.tmem + p * 64, operand_desc(h_at + (p * ha + e / 64) * TC_ATOM + e % 64 * 2), bd, desc, k > 0 || lo > 0);
+          }
+        }
+      tc_commit(&s.bars[stage]);
+    }
+    if (STAGES > 1) load(i + STAGES - 1);
+    if (!tc_wait(s, stage, (i / STAGES) & 1)) {
+      ok = false;
+      break;
+    }
+    tc_fence_after();
+    // thread: a row and half of the tile's columns
+    const int row = (warp & 3) * 32 + lane, ch = warp >> 2;
+    const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21);
+    uint32_t v[2][32];
+    tc_load32(lanes + (g.pairs ? ch * 32 : ch * 64), v[0]);
+    tc_load32(lanes + (g.pairs ? 64 + ch * 32 : ch * 64 + 32), v[1]);
+    tc_load_wait();
+    tc_fence_before();
+    if (row < rows) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t place = at + ba * TC_ATOM + row * 256 + (((ch * 8 + q) ^ (row & 15)) << 4);
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place) : "memory");
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __nv_bfloat162 old = *reinterpret_cast<__nv_bfloat162*>(&w[e]);
+          const int k = q * 8 + 2 * e;                        // the pair's first column of this half
+          const float d0 = __uint_as_float(g.pairs ? v[0][k / 2] : k < 32 ? v[0][k & 31] : v[1][k & 31]);
+          const float d1 = __uint_as_float(g.pairs ? v[1][k / 2] : k < 32 ? v[0][(k + 1) & 31] : v[1][(k + 1) & 31]);
+          const float2 f = __bfloat1622float2(old);
+          __nv_bfloat162 sum = __floats2bfloat162_rn(f.x + d0, f.y + d1);
+          w[e] = *reinterpret_cast<uint32_t*>(&sum);
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+      }
+    }
+    __syncthreads();
+    const int c = c_first + i * ADD_COLS;
+#pragma unroll
+    for (int j = 0; j < TC_ROWS * 16 / TC_THREADS; ++j) {
+      const int r = (tid >> 4) + j * (TC_THREADS / 16), q = tid & 15;
+      if (r < rows && c + q * 8 < c_end) {
+        uint4 w;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                     : "r"(at + ba * TC_ATOM + r * 256 + ((q ^ (r & 15)) << 4))
+                     : "memory");
+        *reinterpret_cast<uint4*>(out + (long long)s.rows[r] * g.ldo + c + q * 8) = w;
+      }
+    }
+    if (STAGES == 1) {
+      __syncthreads();
+      load(i + 1);
+    }
+  }
+  copies_wait<0>();
+  __syncthreads();
+  if (tid < 32) tc_free(s.tmem, 128);
 }
 
 // ---- the plan: rows in the order of their adapters, and items of up to 64 of them
@@ -620,52 +947,94 @@ static cudaError_t allow_smem(K kernel, size_t bytes, size_t* allowed) {
   return e;
 }
 
-template <int NT>
-static cudaError_t launch_tiles(const AdapterArgs& g0, int max_items, cudaStream_t stream) {
-  AdapterArgs g = g0;
-  constexpr int KW = NT == 1 ? TILE_WARPS : TILE_WARPS / 2, TOK = 8 * NT;
-  static size_t allowed[4][64];
-  const size_t sums_bytes = (size_t)KW * TOK * (SUM_GROUP + 4) * 4;
-  cudaError_t e = allow_smem(adapter_sums_kernel<NT>, sums_bytes, allowed[0]);
-  if (e != cudaSuccess) return e;
+static cudaError_t launch_few(const AdapterArgs& g, int max_items, cudaStream_t stream) {
+  static size_t allowed[64];
   const int groups = (g.P * g.R + SUM_GROUP - 1) / SUM_GROUP;
-  e = MI_LAUNCH((adapter_sums_kernel<NT>), dim3(g.ks, max_items, groups), TILE_THREADS, sums_bytes, stream, g);
+  cudaError_t e = MI_LAUNCH((adapter_sums_kernel), dim3(g.ks, max_items, groups), TILE_THREADS, 0, stream, g);
   if (e != cudaSuccess) return e;
-  const size_t h_bytes = (size_t)(g.pairs ? 2 : 1) * 2 * TOK * h_stride(g.R) * 2;
+  const size_t bytes = (size_t)(g.pairs ? 2 : 1) * 2 * FEW_ROWS * h_stride(g.R) * 2;
   const dim3 grid(count_chunks(g, g.span), max_items);
-  if (g.R <= 16) return MI_LAUNCH((adapter_add_kernel<NT, 1, true>), grid, TILE_THREADS, h_bytes, stream, g);
-  if (g.R <= 32) return MI_LAUNCH((adapter_add_kernel<NT, 1, false>), grid, TILE_THREADS, h_bytes, stream, g);
-  if (g.R <= 64) {
-    e = allow_smem(adapter_add_kernel<NT, 2, false>, h_bytes, allowed[1]);
-    if (e != cudaSuccess) return e;
-    return MI_LAUNCH((adapter_add_kernel<NT, 2, false>), grid, TILE_THREADS, h_bytes, stream, g);
-  }
-  e = allow_smem(adapter_add_kernel<NT, 0, false>, h_bytes, allowed[2]);
+  if (g.R <= 16) return MI_LAUNCH((adapter_add_kernel<1, true>), grid, TILE_THREADS, bytes, stream, g);
+  if (g.R <= 32) return MI_LAUNCH((adapter_add_kernel<1, false>), grid, TILE_THREADS, bytes, stream, g);
+  if (g.R <= 64) return MI_LAUNCH((adapter_add_kernel<2, false>), grid, TILE_THREADS, bytes, stream, g);
+  e = allow_smem(adapter_add_kernel<0, false>, bytes, allowed);
   if (e != cudaSuccess) return e;
-  return MI_LAUNCH((adapter_add_kernel<NT, 0, false>), grid, TILE_THREADS, h_bytes, stream, g);
+  return MI_LAUNCH((adapter_add_kernel<0, false>), grid, TILE_THREADS, bytes, stream, g);
 }
 
-// Parts of the sum over K: enough blocks for the chip, at least one unit of 32 k for every warp.
-static int sum_parts(int M, int n, int K, int P, int R) {
-  const int units = (K + 31) / 32, groups = (P * R + SUM_GROUP - 1) / SUM_GROUP;
-  const int items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : (M + MAX_ROWS - 1) / MAX_ROWS;
-  int ks = 2 * 148 / (items * groups);
-  const int most = M <= FEW_MAX ? units / TILE_WARPS : units / (TILE_WARPS / 2) / 2;
-  ks = ks < most ? ks : most;
-  return ks < 1 ? 1 : ks > 16 ? 16 : ks;
+static int add_tc_stages(int R, int pairs) {
+  const int left = 225 * 1024 - (pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM;
+  const int n = left / add_stage_bytes(R);
+  return n > ADD_MAX_STAGES ? ADD_MAX_STAGES : n;
 }
 
-// Whether the tensor-core kernels take a call: rows of x, A and B in pieces of 16 bytes, a plan where there are many rows.
-static bool in_pieces(const void* x, long long ldx, const void* a, const void* b, int M, int K, int n, int P, int R, int dtype) {
-  return dtype == MI_DTYPE_BF16 && n > 0 && R > 0 && R <= 256 && K > 0 && R % 8 == 0 && K % 8 == 0 && mi_aligned(a, 16) &&
-         mi_aligned(b, 16) && mi_aligned(x, 16) && (M == 1 || ldx % 8 == 0) && P * R <= 65535 * SUM_GROUP;
+static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t stream) {
+  static size_t allowed[4][64];
+  const size_t sums_bytes = SUMS_STAGES * SUMS_STAGE_BYTES + 1024;
+  cudaError_t e = allow_smem(adapter_sums_tc_kernel, sums_bytes, allowed[0]);
+  if (e != cudaSuccess) return e;
+  e = MI_LAUNCH((adapter_sums_tc_kernel), dim3(g.ks, max_items, (g.P * g.R + 127) / 128), TC_THREADS, sums_bytes, stream, g);
+  if (e != cudaSuccess) return e;
+  const long long quarters = (long long)g.M * g.P * (padded_rank(g.R) / 4);
+  e = MI_LAUNCH((adapter_pairs_kernel), (unsigned)((quarters + 255) / 256), 256, 0, stream, g);
+  if (e != cudaSuccess) return e;
+  const int stages = add_tc_stages(g.R, g.pairs);
+  const size_t bytes = (size_t)(g.pairs ? 2 : 1) * sums_atoms(g.R) * TC_ATOM + (size_t)stages * add_stage_bytes(g.R) + 1024;
+  const dim3 grid(count_chunks(g, g.span), max_items);
+  if (stages >= 3) {
+    e = allow_smem(adapter_add_tc_kernel<3>, bytes, allowed[1]);
+    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<3>), grid, TC_THREADS, bytes, stream, g);
+  }
+  if (stages == 2) {
+    e = allow_smem(adapter_add_tc_kernel<2>, bytes, allowed[2]);
+    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<2>), grid, TC_THREADS, bytes, stream, g);
+  }
+  e = allow_smem(adapter_add_tc_kernel<1>, bytes, allowed[3]);
+  return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<1>), grid, TC_THREADS, bytes, stream, g);
 }
 
-// Floats of scratch memory (h) that a call needs.
-extern "C" long long mi_adapter_scratch(const void* x, long long ldx, const void* a, const void* b, int M, int K, int n, int P,
-                                        int R, int dtype) {
-  const long long one = (long long)M * P * R;
-  return in_pieces(x, ldx, a, b, M, K, n, P, R, dtype) ? one * sum_parts(M, n, K, P, R) : one;
+// How a call runs, and the scratch memory (h) that it takes.
+enum { BY_ELEMENTS, BY_FEW, BY_MANY };
+struct Route {
+  int way, items, ks;
+  long long floats, pair_floats;      // of h, and behind it of pairs_of_h
+};
+static Route route_of(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b, const void* out,
+                      long long ldo, int M, int N, int K, int n, int P, int R, const int* ends, int pairs, int dtype) {
+  Route r = {BY_ELEMENTS, 0, 1, (long long)M * P * R, 0};
+  // The tensor-core kernels take rows of x, A and B in pieces of 16 bytes.
+  if (dtype != MI_DTYPE_BF16 || n <= 0 || R <= 0 || R > 256 || K <= 0 || R % 8 || K % 8 || !mi_aligned(a, 16) ||
+      !mi_aligned(b, 16) || !mi_aligned(x, 16) || (M > 1 && ldx % 8))
+    return r;
+  bool whole = N % 8 == 0 && mi_aligned(y, 16) && mi_aligned(out, 16) && (M == 1 || (ldy % 8 == 0 && ldo % 8 == 0));
+  for (int p = 0; p + 1 < P && !pairs; ++p) whole = whole && ends[p] % 8 == 0;
+  if (M > FEW_MAX && whole && R <= 128 && add_tc_stages(R, pairs) >= 1) {
+    r.way = BY_MANY;
+    r.items = plan_items(M, n);
+    // Parts of the sum over K: enough blocks for the chip, four stages of 64 k for each
+    const int blocks = (K + 63) / 64, tiles = (M + TC_ROWS - 1) / TC_ROWS * ((P * R + 127) / 128);
+    r.ks = 2 * 148 / tiles;
+    if (r.ks > blocks / 4) r.ks = blocks / 4;
+    r.ks = r.ks < 1 ? 1 : r.ks > 16 ? 16 : r.ks;
+    r.pair_floats = (long long)M * P * padded_rank(R);
+  } else {
+    r.way = BY_FEW;
+    r.items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : plan_items(M, n) * SUB_ITEMS;
+    const int units = (K + 31) / 32, groups = (P * R + SUM_GROUP - 1) / SUM_GROUP;
+    r.ks = 2 * 148 / (r.items * groups);
+    if (r.ks > units / TILE_WARPS) r.ks = units / TILE_WARPS;
+    r.ks = r.ks < 1 ? 1 : r.ks > 16 ? 16 : r.ks;
+  }
+  r.floats *= r.ks;
+  return r;
+}
+
+extern "C" long long mi_adapter_scratch(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b,
+                                        const void* out, long long ldo, int M, int N, int K, int n, int P, int R, int end0,
+                                        int end1, int end2, int end3, int pairs, int dtype) {
+  const int ends[ADAPTER_MAX_PARTS] = {end0, end1, end2, end3};
+  const Route r = route_of(y, ldy, x, ldx, a, b, out, ldo, M, N, K, n, P, R, ends, pairs, dtype);
+  return r.floats + r.pair_floats;
 }
 
 extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b,
@@ -674,19 +1043,21 @@ extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long 
                               int end3, int pairs, int constant, int dtype, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   if (P < 1 || P > ADAPTER_MAX_PARTS) MI_REFUSE("adapter_add: %d parts, at most %d", P, ADAPTER_MAX_PARTS);
-  AdapterArgs g = {x, ldx, y, ldy, out, ldo, a, b, ids, ranks, scale, h, M, N, K, n, P, R, {end0, end1, end2, end3}, pairs, 0, 0, 1,
-                   order, (const int4*)items, constant};
-  if (in_pieces(x, ldx, a, b, M, K, n, P, R, dtype) && (M <= FEW_MAX || (order && items))) {
-    const int max_items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : plan_items(M, n);
-    if (max_items > 65535) MI_REFUSE("adapter_add: %d rows with %d adapters", M, n);
+  AdapterArgs g = {x, ldx, y, ldy, out, ldo, a, b, ids, ranks, scale, h, nullptr, M, N, K, n, P, R, {end0, end1, end2, end3}, pairs,
+                   0, 0, 1, order, (const int4*)items, constant};
+  const Route r = route_of(y, ldy, x, ldx, a, b, out, ldo, M, N, K, n, P, R, g.ends, pairs, dtype);
+  if (r.way != BY_ELEMENTS) {
+    if (r.items > 65535) MI_REFUSE("adapter_add: %d rows with %d adapters", M, n);
+    if (M > FEW_MAX && !(order && items)) MI_REFUSE("adapter_add: a plan of %d rows without their order", M);
+    g.ks = r.ks;
+    g.pairs_of_h = (bf16*)(h + r.floats);
     bool starts4 = true;
     for (int p = 0; p + 1 < P && !pairs; ++p) starts4 = starts4 && g.ends[p] % 4 == 0;
     g.vec = starts4 && mi_aligned(y, 8) && mi_aligned(out, 8) && (M == 1 || (ldy % 4 == 0 && ldo % 4 == 0));
-    g.ks = sum_parts(M, n, K, P, R);
     // Blocks with many columns look for their rows and sums once for all of them; a few waves of blocks fill the chip.
     g.span = 2048;
-    while (g.span > 256 && (long long)max_items * count_chunks(g, g.span) < (M <= FEW_MAX ? 3 : 4) * 148) g.span /= 2;
-    const cudaError_t e = M <= FEW_MAX ? launch_tiles<1>(g, max_items, stream) : launch_tiles<8>(g, max_items, stream);
+    while (g.span > 256 && (long long)r.items * count_chunks(g, g.span) < 3 * 148) g.span /= 2;
+    const cudaError_t e = r.way == BY_MANY ? launch_many(g, r.items, stream) : launch_few(g, r.items, stream);
     if (e != cudaSuccess) return refused_by_cuda(e);
     MI_RETURN_LAUNCH_STATUS();
   }

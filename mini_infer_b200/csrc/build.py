@@ -49,7 +49,7 @@ LIBRARIES: dict[str, tuple[list[str], list[str], list[str]]] = {
     "depth": (["depth.cu"], ["common.cuh"], []),
     "latent_decode": (["latent_decode.cu"], ["common.cuh"], []),
     "attention_stage": (["attention_stage.cu"], ["common.cuh"], []),
-    "adapters": (["adapters.cu"], ["common.cuh"], []),
+    "adapters": (["adapters.cu"], ["common.cuh", "bulk_copy.cuh"], []),
     "logits": (["logits.cu"], ["common.cuh"], []),
 }
 

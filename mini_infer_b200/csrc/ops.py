@@ -68,7 +68,7 @@ _configured: set[str] = set()
 # Libraries whose kernels have bounded waits.  Their give-ups are reported into one int32 word
 # per device (``status_word``), which the engine copies to the host with every step's result;
 # on their own the libraries would each keep a word that only a synchronising call can read.
-_WAITING_LIBRARIES = ("attention_mma", "attention_tc", "gemm_tma", "gemm_f32")
+_WAITING_LIBRARIES = ("attention_mma", "attention_tc", "gemm_tma", "gemm_f32", "adapters")
 _status_words: dict[int, torch.Tensor] = {}
 _status_shared: set[tuple[str, int]] = set()
 
@@ -441,10 +441,13 @@ def _sig_adapters(lib: ctypes.CDLL) -> None:
     lib.mi_adapter_add.argtypes = [c_void_p, ll, c_void_p, ll, c_void_p, c_void_p, c_void_p, ll, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                    c_int, c_int, c_int, c_int, c_void_p]
-    lib.mi_adapter_scratch.argtypes = [c_void_p, ll, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int]
+    lib.mi_adapter_scratch.argtypes = [c_void_p, ll, c_void_p, ll, c_void_p, c_void_p, c_void_p, ll, c_int, c_int, c_int, c_int,
+                                       c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]
     lib.mi_adapter_scratch.restype = ll
     lib.mi_adapter_plan_sizes.argtypes = [c_int, c_int, ctypes.POINTER(c_int)]
     lib.mi_adapter_plan.argtypes = [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]
+    lib.mi_adapters_status.argtypes = [c_int]
+    lib.mi_set_status_word.argtypes = [c_void_p]
 
 
 def _sig_logits(lib: ctypes.CDLL) -> None:
@@ -3090,9 +3093,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
         _same_device(what, x, y, a, b, plan.ids, scale, ranks, out)
     if M == 0 or N == 0:
         return out
-    lib = _lib("adapters")
-    h = torch.empty(lib.mi_adapter_scratch(_ptr(x), x.stride(0), _ptr(a), _ptr(b), M, K, n, P, R, code), dtype=torch.float32,
-                    device=x.device)
+    lib = _waiting_lib("adapters", x.device)
+    h = torch.empty(lib.mi_adapter_scratch(_ptr(y), y.stride(0), _ptr(x), x.stride(0), _ptr(a), _ptr(b), _ptr(out), out.stride(0), M,
+                                           N, K, n, P, R, *ends, 1 if pairs else 0, code), dtype=torch.float32, device=x.device)
     rc = lib.mi_adapter_add(_ptr(y), y.stride(0), _ptr(x), x.stride(0), _ptr(a), _ptr(b), _ptr(out), out.stride(0),
                             _ptr(plan.ids), _ptr(plan.order), _ptr(plan.items), _ptr(scale), _ptr(ranks), _ptr(h), M, N, K, n, P, R,
                             *ends, 1 if pairs else 0, 1 if w_constant else 0, code, _stream())
