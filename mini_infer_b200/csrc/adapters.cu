@@ -527,6 +527,14 @@ __device__ __forceinline__ void tc_load32(uint32_t from, uint32_t (&r)[32]) {   
       : "r"(from)
       : "memory");
 }
+__device__ __forceinline__ void tc_load16(uint32_t from, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(from)
+      : "memory");
+}
 __device__ __forceinline__ void tc_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 
 // Tensor memory for a block, by its first warp; the address is in `holder` behind a barrier of the block.  Only then may the next kernel's
@@ -700,8 +708,11 @@ __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_A
 // The second product and the sum with y, in tiles of 128 columns: the products run from shared memory into tensor memory, y
 // waits in shared memory in rows of 256 bytes (16-byte pieces permuted by the row, so that a thread of the sum, which has a row,
 // and a thread of the copies, which has a piece of it, both touch all banks), and the result leaves the way y came.
+#define ADD_THREADS 512
+#define ADD_ROW_STEP (ADD_THREADS / 16)
+
 template <int STAGES>
-__global__ void __launch_bounds__(TC_THREADS) adapter_add_tc_kernel(const AdapterArgs g) {
+__global__ void __launch_bounds__(ADD_THREADS, STAGES == 2 ? 2 : 1) adapter_add_tc_kernel(const AdapterArgs g) {
   extern __shared__ unsigned char tc_smem[];
   __shared__ TcBlock s;
   mi_pdl_wait();
@@ -718,7 +729,7 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_add_tc_kernel(const Adapte
   if (rank == 0) {                                            // rows without an adapter: 8 columns a thread
     __syncthreads();
     const int pieces = (c_end - c_first) / 8;
-    for (int i = tid; i < rows * pieces; i += TC_THREADS) {
+    for (int i = tid; i < rows * pieces; i += ADD_THREADS) {
       const long long row = s.rows[i / pieces];
       const int c = c_first + i % pieces * 8;
       *reinterpret_cast<uint4*>(out + row * g.ldo + c) = load16(y + row * g.ldy + c);
@@ -729,32 +740,46 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_add_tc_kernel(const Adapte
   const int np = g.pairs ? 2 : 1, rp = padded_rank(R), ha = sums_atoms(R), ba = b_atoms(R);
   const uint32_t h_at = base, stages_at = base + np * ha * TC_ATOM, stage_bytes = add_stage_bytes(R);
 
-  // the item's sums
-  const int h_pieces = 2 * rp / 8;
-  for (int i = tid; i < np * rows * h_pieces; i += TC_THREADS) {
-    const int q = i % h_pieces, row = i / h_pieces % rows, p = i / h_pieces / rows;
-    copy_piece(h_at + (p * ha + q / 8) * TC_ATOM + row * 128 + (((q & 7) ^ (row & 7)) << 4),
-               g.pairs_of_h + ((size_t)s.rows[row] * g.P + part + p) * 2 * rp + q * 8, 16);
+  // the item's sums: pieces of a row by as many threads, rounded up to a power of two
+  const int h_pieces = 2 * rp / 8, b_pieces = rp / 8, b_shift = b_pieces <= 2 ? 1 : b_pieces <= 4 ? 2 : b_pieces <= 8 ? 3 : 4;
+  {
+    const int q = tid & ((2 << b_shift) - 1);
+    if (q < h_pieces)
+      for (int row = tid >> (b_shift + 1); row < rows; row += ADD_THREADS >> (b_shift + 1))
+        for (int p = 0; p < np; ++p)
+          copy_piece(h_at + (p * ha + q / 8) * TC_ATOM + row * 128 + (((q & 7) ^ (row & 7)) << 4),
+                     g.pairs_of_h + ((size_t)s.rows[row] * g.P + part + p) * 2 * rp + q * 8, 16);
   }
-  const int tiles = (c_end - c_first + ADD_COLS - 1) / ADD_COLS, b_pieces = rp / 8;
-  const bf16* b = (const bf16*)g.b + (size_t)item.x * g.N * R;
+  const int tiles = (c_end - c_first + ADD_COLS - 1) / ADD_COLS;
+  // this thread's pieces: of y and the result, piece `tid % 16` of every 32nd row; of B, one of every so many columns
+  const int yq = tid & 15, yr = tid >> 4, bq = tid & ((1 << b_shift) - 1), b_col = tid >> b_shift, b_step = ADD_THREADS >> b_shift;
+  long long y_off[4], out_off[4];
+  uint32_t y_place[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = yr + j * ADD_ROW_STEP;
+    y_off[j] = s.rows[row] * g.ldy + c_first + yq * 8;
+    out_off[j] = s.rows[row] * g.ldo + c_first + yq * 8;
+    y_place[j] = ba * TC_ATOM + row * 256 + ((yq ^ (row & 15)) << 4);
+  }
+  const int b_there = bq < b_pieces ? 2 * max(0, min(8, rank - bq * 8)) : 0;
+  const bf16* b = (const bf16*)g.b + (size_t)item.x * g.N * R + bq * 8;
   const auto load = [&](int i) {
     if (i < tiles) {
-      const int c = c_first + i * ADD_COLS;
+      const int c = i * ADD_COLS;
       const uint32_t to = stages_at + i % STAGES * stage_bytes;
       // rows of B: the tile's columns, of pairs the first ones and then the second ones
-      for (int j = tid; j < ADD_COLS * b_pieces; j += TC_THREADS) {
-        const int q = j % b_pieces, col = j / b_pieces;
-        const int from = c + (g.pairs ? (col & 63) * 2 + (col >> 6) : col);
-        const int there = from < c_end ? max(0, min(8, rank - q * 8)) : 0;
-        copy_piece(to + q / 8 * TC_ATOM + col * 128 + (((q & 7) ^ (col & 7)) << 4), there ? b + (size_t)from * R + q * 8 : b, there * 2);
+      if (bq < b_pieces) {
+        for (int col = b_col; col < ADD_COLS; col += b_step) {
+          const int from = c_first + c + (g.pairs ? (col & 63) * 2 + (col >> 6) : col);
+          const int there = from < c_end ? b_there : 0;
+          copy_piece(to + bq / 8 * TC_ATOM + col * 128 + (((bq & 7) ^ (col & 7)) << 4), there ? b + (size_t)from * R : (const bf16*)g.b, there);
+        }
       }
-      const uint32_t y_to = to + ba * TC_ATOM;
+      if (c_first + c + yq * 8 < c_end) {
 #pragma unroll
-      for (int j = 0; j < TC_ROWS * 16 / TC_THREADS; ++j) {
-        const int row = (tid >> 4) + j * (TC_THREADS / 16), q = tid & 15;
-        if (row < rows && c + q * 8 < c_end)
-          copy_piece(y_to + row * 256 + ((q ^ (row & 15)) << 4), y + (long long)s.rows[row] * g.ldy + c + q * 8, 16);
+        for (int j = 0; j < 4; ++j)
+          if (yr + j * ADD_ROW_STEP < rows) copy_piece(to + y_place[j], y + y_off[j] + c, 16);
       }
     }
     copies_commit();
@@ -763,7 +788,9 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_add_tc_kernel(const Adapte
   for (int i = 0; i < STAGES - 1; ++i) load(i);
   if (STAGES == 1) load(0);
   const uint32_t desc = product_desc(g.pairs ? ADD_COLS / 2 : ADD_COLS);
-  bool ok = true;
+  // the sum: a row and a quarter of the tile's columns (of pairs, 16 of either sort)
+  const int row = (warp & 3) * 32 + lane, quarter = warp >> 2;
+  const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21) + (g.pairs ? quarter * 16 : quarter * 32);
   for (int i = 0; i < tiles; ++i) {
     copies_wait<(STAGES > 1 ? STAGES - 2 : 0)>();
     smem_for_tensor_cores();
@@ -783,32 +810,24 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_add_tc_kernel(const Adapte
       tc_commit(&s.bars[stage]);
     }
     if (STAGES > 1) load(i + STAGES - 1);
-    if (!tc_wait(s, stage, (i / STAGES) & 1)) {
-      ok = false;
-      break;
-    }
+    if (!tc_wait(s, stage, (i / STAGES) & 1)) break;
     tc_fence_after();
-    // thread: a row and half of the tile's columns
-    const int row = (warp & 3) * 32 + lane, ch = warp >> 2;
-    const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21);
-    uint32_t v[2][32];
-    tc_load32(lanes + (g.pairs ? ch * 32 : ch * 64), v[0]);
-    tc_load32(lanes + (g.pairs ? 64 + ch * 32 : ch * 64 + 32), v[1]);
+    uint32_t v[32];
+    tc_load16(lanes, v);
+    tc_load16(lanes + (g.pairs ? 64 : 16), v + 16);
     tc_load_wait();
     tc_fence_before();
     if (row < rows) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const uint32_t place = at + ba * TC_ATOM + row * 256 + (((ch * 8 + q) ^ (row & 15)) << 4);
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t place = at + ba * TC_ATOM + row * 256 + (((quarter * 4 + q) ^ (row & 15)) << 4);
         uint32_t w[4];
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place) : "memory");
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const __nv_bfloat162 old = *reinterpret_cast<__nv_bfloat162*>(&w[e]);
-          const int k = q * 8 + 2 * e;                        // the pair's first column of this half
-          const float d0 = __uint_as_float(g.pairs ? v[0][k / 2] : k < 32 ? v[0][k & 31] : v[1][k & 31]);
-          const float d1 = __uint_as_float(g.pairs ? v[1][k / 2] : k < 32 ? v[0][(k + 1) & 31] : v[1][(k + 1) & 31]);
-          const float2 f = __bfloat1622float2(old);
+          const int k = q * 8 + 2 * e;                        // the pair's first column of this quarter
+          const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[e]));
+          const float d0 = __uint_as_float(g.pairs ? v[k / 2] : v[k]), d1 = __uint_as_float(g.pairs ? v[16 + k / 2] : v[k + 1]);
           __nv_bfloat162 sum = __floats2bfloat162_rn(f.x + d0, f.y + d1);
           w[e] = *reinterpret_cast<uint32_t*>(&sum);
         }
@@ -816,18 +835,14 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_add_tc_kernel(const Adapte
       }
     }
     __syncthreads();
-    const int c = c_first + i * ADD_COLS;
+    if (c_first + i * ADD_COLS + yq * 8 < c_end) {
 #pragma unroll
-    for (int j = 0; j < TC_ROWS * 16 / TC_THREADS; ++j) {
-      const int r = (tid >> 4) + j * (TC_THREADS / 16), q = tid & 15;
-      if (r < rows && c + q * 8 < c_end) {
-        uint4 w;
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                     : "r"(at + ba * TC_ATOM + r * 256 + ((q ^ (r & 15)) << 4))
-                     : "memory");
-        *reinterpret_cast<uint4*>(out + (long long)s.rows[r] * g.ldo + c + q * 8) = w;
-      }
+      for (int j = 0; j < 4; ++j)
+        if (yr + j * ADD_ROW_STEP < rows) {
+          uint4 w;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at + y_place[j]) : "memory");
+          *reinterpret_cast<uint4*>(out + out_off[j] + i * ADD_COLS) = w;
+        }
     }
     if (STAGES == 1) {
       __syncthreads();
@@ -855,15 +870,27 @@ adapter_plan_kernel(const int* ids, int M, int n, int* order, int4* items, int m
   for (int i = tid; i <= n; i += PLAN_THREADS) count[i] = 0;
   if (tid < 2) carry[tid] = 0;
   __syncthreads();
-  const auto bucket = [&](int i) {
-    const int id = ids[i];
-    return id >= 0 && id < n ? id : n;
+  // (rows by the thousand are the usual case: eight loads under way at once)
+  const auto for_rows = [&](auto f) {
+    for (int i0 = 0; i0 < M; i0 += 8 * PLAN_THREADS) {
+      int id[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) id[u] = i0 + u * PLAN_THREADS + tid < M ? ids[i0 + u * PLAN_THREADS + tid] : 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (i0 + u * PLAN_THREADS >= M) break;
+        const int i = i0 + u * PLAN_THREADS + tid, b = i >= M ? -1 : id[u] >= 0 && id[u] < n ? id[u] : n;
+        // rows side by side are mostly of one request
+        int all;
+        unsigned same = __match_all_sync(0xffffffffu, b, &all);
+        if (!all) same = __match_any_sync(0xffffffffu, b);
+        f(i, b, same);
+      }
+    }
   };
-  for (int i0 = 0; i0 < M; i0 += PLAN_THREADS) {
-    const int i = i0 + tid, b = i < M ? bucket(i) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, b);
+  for_rows([&](int, int b, unsigned same) {
     if (b >= 0 && lane == __ffs(same) - 1) atomicAdd(&count[b], __popc(same));
-  }
+  });
   __syncthreads();
   // first rows and first items, from running sums over the adapters
   for (int i0 = 0; i0 <= n; i0 += PLAN_THREADS) {
@@ -901,14 +928,12 @@ adapter_plan_kernel(const int* ids, int M, int n, int* order, int4* items, int m
   }
   for (int i = carry[1] + tid; i < max_items; i += PLAN_THREADS) items[i] = make_int4(-1, 0, 0, 0);
   // rows into their order (which one of an adapter's rows comes first changes nothing that is computed)
-  for (int i0 = 0; i0 < M; i0 += PLAN_THREADS) {
-    const int i = i0 + tid, b = i < M ? bucket(i) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, b);
+  for_rows([&](int i, int b, unsigned same) {
     int at = 0;
     if (b >= 0 && lane == __ffs(same) - 1) at = atomicAdd(&next[b], __popc(same));
     at = __shfl_sync(0xffffffffu, at, __ffs(same) - 1) + __popc(same & ((1u << lane) - 1u));
     if (b >= 0) order[at] = i;
-  }
+  });
 }
 
 static int plan_items(int M, int n) { return M / MAX_ROWS + (M < n + 1 ? M : n + 1); }
@@ -965,6 +990,8 @@ static cudaError_t launch_few(const AdapterArgs& g, int max_items, cudaStream_t 
 static int add_tc_stages(int R, int pairs) {
   const int left = 225 * 1024 - (pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM;
   const int n = left / add_stage_bytes(R);
+  // two stages where that leaves room for another block on the SM, else all that fit
+  if ((pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM + 2 * add_stage_bytes(R) <= 112 * 1024) return 2;
   return n > ADD_MAX_STAGES ? ADD_MAX_STAGES : n;
 }
 
@@ -983,14 +1010,14 @@ static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t
   const dim3 grid(count_chunks(g, g.span), max_items);
   if (stages >= 3) {
     e = allow_smem(adapter_add_tc_kernel<3>, bytes, allowed[1]);
-    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<3>), grid, TC_THREADS, bytes, stream, g);
+    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<3>), grid, ADD_THREADS, bytes, stream, g);
   }
   if (stages == 2) {
     e = allow_smem(adapter_add_tc_kernel<2>, bytes, allowed[2]);
-    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<2>), grid, TC_THREADS, bytes, stream, g);
+    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<2>), grid, ADD_THREADS, bytes, stream, g);
   }
   e = allow_smem(adapter_add_tc_kernel<1>, bytes, allowed[3]);
-  return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<1>), grid, TC_THREADS, bytes, stream, g);
+  return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<1>), grid, ADD_THREADS, bytes, stream, g);
 }
 
 // How a call runs, and the scratch memory (h) that it takes.
