@@ -35,7 +35,8 @@ struct AdapterArgs {
   int span;                       // columns of a block
   int ks;                         // parts of the sum over K
   const int* order;
-  const int4* items;
+  const int4* items;              // (and behind the last one: how many there are)
+  int max_items, tiles;           // of the plan; of 128 columns in a row
   int constant;                   // no kernel in flight writes A and B
 };
 
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 3) adapter_add_kernel(const Adap
 #define SUMS_STAGES 3
 #define SUMS_STAGE_BYTES (2 * TC_ATOM)
 #define ADD_COLS 128                 // columns of a tile of the result
-#define ADD_MAX_STAGES 3
+#define ADD_MAX_STAGES 4
 
 __device__ __forceinline__ void copy_piece(uint32_t to, const void* from, int bytes) {      // the rest of 16 bytes: zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -548,7 +549,7 @@ __device__ __forceinline__ void tc_free(uint32_t at, int columns) {
 }
 
 struct TcBlock {
-  uint64_t bars[SUMS_STAGES > ADD_MAX_STAGES ? SUMS_STAGES : ADD_MAX_STAGES];      // the products that read a stage have ended
+  uint64_t bars[SUMS_STAGES];                                                           // the products that read a stage have ended
   uint32_t tmem;
   int give_up;
   int rows[TC_ROWS];
@@ -705,153 +706,259 @@ __host__ __device__ inline int sums_atoms(int R) { return (2 * padded_rank(R) + 
 __host__ __device__ inline int b_atoms(int R) { return (padded_rank(R) + 63) / 64; }
 __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_ATOM + TC_ROWS * ADD_COLS * 2; }
 
-// The second product and the sum with y, in tiles of 128 columns: the products run from shared memory into tensor memory, y
-// waits in shared memory in rows of 256 bytes (16-byte pieces permuted by the row, so that a thread of the sum, which has a row,
-// and a thread of the copies, which has a piece of it, both touch all banks), and the result leaves the way y came.
-#define ADD_THREADS 512
-#define ADD_ROW_STEP (ADD_THREADS / 16)
+// The second product and the sum with y, in tiles of 128 columns.  One block per SM takes an equal stretch of all items' tiles; its warps
+// have parts of their own and meet at mbarriers alone, so that copies, products and sums of different tiles run side by side:
+//
+//   four copy warps      bring B and y of a tile into a ring of stages, and an item's sums when it begins;
+//   one thread           issues a tile's products into one of two buffers in tensor memory;
+//   eight summing warps  add a buffer to y in shared memory (a thread has a row) and write the result (a lane has pieces of
+//                        rows).  y lies in rows of 256 bytes, 16-byte pieces permuted by the row, so that both ways touch all banks.
+//
+// Copies gather (rows of an item lie anywhere), which a tensor map does not; a copy warp says that a tile is there once its own
+// copies have landed and are visible to the tensor cores.
+#define ADD_SUM_WARPS 8
+#define ADD_COPY_WARPS 4
+#define ADD_COPY_THREADS (32 * ADD_COPY_WARPS)
+#define ADD_THREADS (32 * (ADD_SUM_WARPS + ADD_COPY_WARPS + 1))
+
+struct AddBlock {
+  uint64_t full[ADD_MAX_STAGES], empty[ADD_MAX_STAGES];      // a stage is there; the summing warps are through with it
+  uint64_t done[2], free_[2];                                // a buffer's products have ended; it has been read
+  uint64_t h_free;                                           // the products that read an item's sums have ended
+  uint32_t tmem;
+  int give_up;
+};
+
+// f(tile number of the block, item, rank, whether the item begins, whether it ends, chunk of columns) for a block's tiles in
+// order, until f returns false; items of which nothing changes are passed over.
+template <typename F>
+__device__ __forceinline__ void for_tiles(const AdapterArgs& g, F f) {
+  const int per_item = g.tiles;
+  const long long all = (long long)__ldcg(&g.items[g.max_items].x) * per_item;
+  const int t0 = (int)(all * blockIdx.x / gridDim.x), t1 = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  int count = 0;
+  for (int t = t0; t < t1;) {
+    const int index = t / per_item, end = min(t1, (index + 1) * per_item);
+    const int4 item = __ldcg(g.items + index);
+    const int rank = rank_of(g, item.x);
+    if (rank > 0 || g.out != g.y) {
+      for (int u = t; u < end; ++u)
+        if (!f(count++, item, rank, u == t, u + 1 == end, u - index * per_item)) return;
+    }
+    t = end;
+  }
+}
 
 template <int STAGES>
-__global__ void __launch_bounds__(ADD_THREADS, STAGES == 2 ? 2 : 1) adapter_add_tc_kernel(const AdapterArgs g) {
+__global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const AdapterArgs g) {
   extern __shared__ unsigned char tc_smem[];
-  __shared__ TcBlock s;
+  __shared__ AddBlock s;
   mi_pdl_wait();
   const uint32_t base = (smem_u32(tc_smem) + 1023) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = g.R;
-  int4 item;
-  int rank, part, c_first, c_end;
-  const bool any = tc_begin(g, s, item, rank);
-  const bf16* y = (const bf16*)g.y;
-  bf16* out = (bf16*)g.out;
-  if (!find_chunk(g, blockIdx.x, g.span, part, c_first, c_end) || !any || (rank == 0 && out == y)) return;
-  c_end = min(c_end, c_first + g.span);
-  const int rows = item.z;
-  if (rank == 0) {                                            // rows without an adapter: 8 columns a thread
-    __syncthreads();
-    const int pieces = (c_end - c_first) / 8;
-    for (int i = tid; i < rows * pieces; i += ADD_THREADS) {
-      const long long row = s.rows[i / pieces];
-      const int c = c_first + i % pieces * 8;
-      *reinterpret_cast<uint4*>(out + row * g.ldo + c) = load16(y + row * g.ldy + c);
-    }
-    return;
-  }
-  tc_ready(s, 128);
   const int np = g.pairs ? 2 : 1, rp = padded_rank(R), ha = sums_atoms(R), ba = b_atoms(R);
   const uint32_t h_at = base, stages_at = base + np * ha * TC_ATOM, stage_bytes = add_stage_bytes(R);
-
-  // the item's sums: pieces of a row by as many threads, rounded up to a power of two
-  const int h_pieces = 2 * rp / 8, b_pieces = rp / 8, b_shift = b_pieces <= 2 ? 1 : b_pieces <= 4 ? 2 : b_pieces <= 8 ? 3 : 4;
-  {
-    const int q = tid & ((2 << b_shift) - 1);
-    if (q < h_pieces)
-      for (int row = tid >> (b_shift + 1); row < rows; row += ADD_THREADS >> (b_shift + 1))
-        for (int p = 0; p < np; ++p)
-          copy_piece(h_at + (p * ha + q / 8) * TC_ATOM + row * 128 + (((q & 7) ^ (row & 7)) << 4),
-                     g.pairs_of_h + ((size_t)s.rows[row] * g.P + part + p) * 2 * rp + q * 8, 16);
-  }
-  const int tiles = (c_end - c_first + ADD_COLS - 1) / ADD_COLS;
-  // this thread's pieces: of y and the result, piece `tid % 16` of every 32nd row; of B, one of every so many columns
-  const int yq = tid & 15, yr = tid >> 4, bq = tid & ((1 << b_shift) - 1), b_col = tid >> b_shift, b_step = ADD_THREADS >> b_shift;
-  long long y_off[4], out_off[4];
-  uint32_t y_place[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = yr + j * ADD_ROW_STEP;
-    y_off[j] = s.rows[row] * g.ldy + c_first + yq * 8;
-    out_off[j] = s.rows[row] * g.ldo + c_first + yq * 8;
-    y_place[j] = ba * TC_ATOM + row * 256 + ((yq ^ (row & 15)) << 4);
-  }
-  const int b_there = bq < b_pieces ? 2 * max(0, min(8, rank - bq * 8)) : 0;
-  const bf16* b = (const bf16*)g.b + (size_t)item.x * g.N * R + bq * 8;
-  const auto load = [&](int i) {
-    if (i < tiles) {
-      const int c = i * ADD_COLS;
-      const uint32_t to = stages_at + i % STAGES * stage_bytes;
-      // rows of B: the tile's columns, of pairs the first ones and then the second ones
-      if (bq < b_pieces) {
-        for (int col = b_col; col < ADD_COLS; col += b_step) {
-          const int from = c_first + c + (g.pairs ? (col & 63) * 2 + (col >> 6) : col);
-          const int there = from < c_end ? b_there : 0;
-          copy_piece(to + bq / 8 * TC_ATOM + col * 128 + (((bq & 7) ^ (col & 7)) << 4), there ? b + (size_t)from * R : (const bf16*)g.b, there);
-        }
+  if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) {
+    if (lane == 0) {
+      for (int i = 0; i < STAGES; ++i) {
+        mbar_init(&s.full[i], ADD_COPY_THREADS);
+        mbar_init(&s.empty[i], ADD_SUM_WARPS);
       }
-      if (c_first + c + yq * 8 < c_end) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (yr + j * ADD_ROW_STEP < rows) copy_piece(to + y_place[j], y + y_off[j] + c, 16);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s.done[i], 1);
+        mbar_init(&s.free_[i], ADD_SUM_WARPS);
       }
+      mbar_init(&s.h_free, 1);
+      s.give_up = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    copies_commit();
-  };
+    __syncwarp();
+    tc_alloc(&s.tmem, 2 * ADD_COLS);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  mi_pdl_launch_dependents();
+  const uint32_t tmem = s.tmem;
+  const bf16* y = (const bf16*)g.y;
+  bf16* out = (bf16*)g.out;
+
+  if (warp >= ADD_SUM_WARPS && warp < ADD_SUM_WARPS + ADD_COPY_WARPS) {
+    // ---- copies.  Pieces of a row by as many threads, rounded up to a power of two
+    constexpr int LAG = STAGES > 2 ? STAGES - 2 : 0;          // tiles under way behind the one just asked for
+    const int ct = tid - 32 * ADD_SUM_WARPS;
+    const int h_pieces = 2 * rp / 8, b_pieces = rp / 8, b_shift = b_pieces <= 2 ? 1 : b_pieces <= 4 ? 2 : b_pieces <= 8 ? 3 : 4;
+    const int bq = ct & ((1 << b_shift) - 1), b_col = ct >> b_shift, b_step = ADD_COPY_THREADS >> b_shift;
+    const int hq = ct & ((2 << b_shift) - 1), h_row = ct >> (b_shift + 1), h_step = ADD_COPY_THREADS >> (b_shift + 1);
+    const int yq = ct & 15, yr = ct >> 4;                     // piece `yq` of every 8th row
+    constexpr int YN = TC_ROWS * 16 / ADD_COPY_THREADS;
+    long long y_off[YN];
+    uint32_t y_in = 0;
+    int items = 0, asked = 0, told = 0;                       // begun so far, of those with an adapter; tiles asked for, and said to be there
+    const auto tell = [&](int upto) {
+      if (told < upto) smem_for_tensor_cores();
+      for (; told < upto; ++told) mbar_arrive(&s.full[told % STAGES]);
+    };
+    for_tiles(g, [&](int j, const int4& item, int rank, bool begins, bool, int chunk) {
+      const int stage = j % STAGES;
+      const uint32_t to = stages_at + stage * stage_bytes;
+      if (begins) {
+        y_in = 0;
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load(i);
-  if (STAGES == 1) load(0);
-  const uint32_t desc = product_desc(g.pairs ? ADD_COLS / 2 : ADD_COLS);
-  // the sum: a row and a quarter of the tile's columns (of pairs, 16 of either sort)
-  const int row = (warp & 3) * 32 + lane, quarter = warp >> 2;
-  const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21) + (g.pairs ? quarter * 16 : quarter * 32);
-  for (int i = 0; i < tiles; ++i) {
-    copies_wait<(STAGES > 1 ? STAGES - 2 : 0)>();
-    smem_for_tensor_cores();
-    __syncthreads();
-    const int stage = i % STAGES;
-    const uint32_t at = stages_at + stage * stage_bytes;
-    if (tid == 0) {
-      tc_fence_after();
-      for (int p = 0; p < np; ++p)
-        for (int k = 0; k < rp; k += 16) {
-          const uint64_t bd = operand_desc(at + p * 64 * 128 + k / 64 * TC_ATOM + k % 64 * 2);
-          for (int lo = 0; lo < 2; ++lo) {
-            const int e = k + lo * rp;
-            tc_mma(s.tmem + p * 64, operand_desc(h_at + (p * ha + e / 64) * TC_ATOM + e % 64 * 2), bd, desc, k > 0 || lo > 0);
+        for (int i = 0; i < YN; ++i) {
+          const int row = yr + i * (TC_ROWS / YN);
+          if (row < item.z) {
+            y_off[i] = __ldcg(g.order + item.y + row) * g.ldy + yq * 8;
+            y_in |= 1u << i;
           }
         }
-      tc_commit(&s.bars[stage]);
-    }
-    if (STAGES > 1) load(i + STAGES - 1);
-    if (!tc_wait(s, stage, (i / STAGES) & 1)) break;
-    tc_fence_after();
-    uint32_t v[32];
-    tc_load16(lanes, v);
-    tc_load16(lanes + (g.pairs ? 64 : 16), v + 16);
-    tc_load_wait();
-    tc_fence_before();
-    if (row < rows) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t place = at + ba * TC_ATOM + row * 256 + (((quarter * 4 + q) ^ (row & 15)) << 4);
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place) : "memory");
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = q * 8 + 2 * e;                        // the pair's first column of this quarter
-          const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[e]));
-          const float d0 = __uint_as_float(g.pairs ? v[k / 2] : v[k]), d1 = __uint_as_float(g.pairs ? v[16 + k / 2] : v[k + 1]);
-          __nv_bfloat162 sum = __floats2bfloat162_rn(f.x + d0, f.y + d1);
-          w[e] = *reinterpret_cast<uint32_t*>(&sum);
-        }
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
       }
-    }
-    __syncthreads();
-    if (c_first + i * ADD_COLS + yq * 8 < c_end) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (yr + j * ADD_ROW_STEP < rows) {
-          uint4 w;
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at + y_place[j]) : "memory");
-          *reinterpret_cast<uint4*>(out + out_off[j] + i * ADD_COLS) = w;
+      if (j >= STAGES && !mbar_wait(&s.empty[stage], (j / STAGES - 1) & 1, &s.give_up)) return false;
+      int part, c, c_end;
+      find_chunk(g, chunk, ADD_COLS, part, c, c_end);
+      if (begins && rank > 0) {
+        // the last item's products have to end first, and for that to be told of all their tiles
+        copies_wait<0>();
+        tell(j);
+        if (items > 0 && !mbar_wait(&s.h_free, (items - 1) & 1, &s.give_up)) return false;
+        ++items;
+        if (hq < h_pieces)
+          for (int row = h_row; row < item.z; row += h_step) {
+            const bf16* from = g.pairs_of_h + (size_t)__ldcg(g.order + item.y + row) * g.P * 2 * rp + hq * 8;
+            for (int p = 0; p < np; ++p)
+              copy_piece(h_at + (p * ha + hq / 8) * TC_ATOM + row * 128 + (((hq & 7) ^ (row & 7)) << 4), from + (size_t)(part + p) * 2 * rp, 16);
+          }
+      }
+      if (rank > 0 && bq < b_pieces) {
+        // rows of B: the tile's columns, of pairs the first ones and then the second ones
+        const int there = 2 * max(0, min(8, rank - bq * 8));
+        const bf16* b = (const bf16*)g.b + (size_t)item.x * g.N * R + bq * 8;
+        for (int col = b_col; col < ADD_COLS; col += b_step) {
+          const int from = c + (g.pairs ? (col & 63) * 2 + (col >> 6) : col);
+          const bool in = there && from < c_end;
+          copy_piece(to + bq / 8 * TC_ATOM + col * 128 + (((bq & 7) ^ (col & 7)) << 4), in ? b + (size_t)from * R : (const bf16*)g.b, in ? there : 0);
         }
+      }
+      if (c + yq * 8 < c_end) {
+#pragma unroll
+        for (int i = 0; i < YN; ++i) {
+          const int row = yr + i * (TC_ROWS / YN);
+          if ((y_in >> i) & 1u) copy_piece(to + ba * TC_ATOM + row * 256 + ((yq ^ (row & 15)) << 4), y + y_off[i] + c, 16);
+        }
+      }
+      copies_commit();
+      asked = j + 1;
+      copies_wait<LAG>();
+      tell(asked - LAG);
+      return true;
+    });
+    copies_wait<0>();
+    tell(asked);
+  } else if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) {
+    // ---- products
+    if (lane == 0) {
+      const uint32_t desc = product_desc(g.pairs ? ADD_COLS / 2 : ADD_COLS);
+      for_tiles(g, [&](int j, const int4&, int rank, bool, bool ends, int) {
+        const int stage = j % STAGES, buf = j & 1;
+        if (!mbar_wait(&s.full[stage], (j / STAGES) & 1, &s.give_up)) return false;
+        if (j >= 2 && !mbar_wait(&s.free_[buf], (j / 2 - 1) & 1, &s.give_up)) return false;
+        tc_fence_after();
+        const uint32_t at = stages_at + stage * stage_bytes;
+        for (int p = 0; p < np && rank > 0; ++p)
+          for (int k = 0; k < rp; k += 16) {
+            const uint64_t bd = operand_desc(at + p * 64 * 128 + k / 64 * TC_ATOM + k % 64 * 2);
+            for (int lo = 0; lo < 2; ++lo) {
+              const int e = k + lo * rp;
+              tc_mma(tmem + buf * ADD_COLS + p * 64, operand_desc(h_at + (p * ha + e / 64) * TC_ATOM + e % 64 * 2), bd, desc, k > 0 || lo > 0);
+            }
+          }
+        tc_commit(&s.done[buf]);
+        if (ends && rank > 0) tc_commit(&s.h_free);
+        return true;
+      });
     }
-    if (STAGES == 1) {
-      __syncthreads();
-      load(i + 1);
-    }
+    __syncwarp();
+  } else {
+    // ---- sums: a warp has 32 rows and half of a tile's columns
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21) + (g.pairs ? half * 32 : half * 64);
+    const int q0 = lane & 7, r0 = (warp & 3) * 32 + (lane >> 3);       // the result: a piece of every 4th row
+    long long out_off[8];
+    uint32_t out_in = 0;
+    for_tiles(g, [&](int j, const int4& item, int rank, bool begins, bool, int chunk) {
+      const int stage = j % STAGES, buf = j & 1;
+      if (begins) {
+        out_in = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (r0 + 4 * i < item.z) {
+            out_off[i] = __ldcg(g.order + item.y + r0 + 4 * i) * g.ldo + half * 64 + q0 * 8;
+            out_in |= 1u << i;
+          }
+      }
+      int part, c, c_end;
+      find_chunk(g, chunk, ADD_COLS, part, c, c_end);
+      const uint32_t y_at = stages_at + stage * stage_bytes + ba * TC_ATOM;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.full[stage], (j / STAGES) & 1, &s.give_up))) return false;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.done[buf], (j / 2) & 1, &s.give_up))) return false;
+      if (rank > 0) {
+        tc_fence_after();
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {                         // 32 columns at a time
+          uint32_t v[32];
+          tc_load16(lanes + buf * ADD_COLS + (g.pairs ? o * 16 : o * 32), v);
+          tc_load16(lanes + buf * ADD_COLS + (g.pairs ? 64 + o * 16 : o * 32 + 16), v + 16);
+          tc_load_wait();
+          if (o == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.free_[buf]);
+          }
+          if (row < item.z) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t place = y_at + row * 256 + (((half * 8 + o * 4 + q) ^ (row & 15)) << 4);
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place) : "memory");
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int k = q * 8 + 2 * e;                  // the pair's first column of the 32
+                const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[e]));
+                const float d0 = __uint_as_float(g.pairs ? v[k / 2] : v[k]), d1 = __uint_as_float(g.pairs ? v[16 + k / 2] : v[k + 1]);
+                __nv_bfloat162 sum = __floats2bfloat162_rn(f.x + d0, f.y + d1);
+                w[e] = *reinterpret_cast<uint32_t*>(&sum);
+              }
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+            }
+          }
+        }
+      } else if (lane == 0) {
+        mbar_arrive(&s.free_[buf]);
+      }
+      __syncwarp();
+      if (c + half * 64 + q0 * 8 < c_end) {
+        uint4 w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((out_in >> i) & 1u) {
+            const int r = r0 + 4 * i;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                         : "r"(y_at + r * 256 + (((half * 8 + q0) ^ (r & 15)) << 4))
+                         : "memory");
+          }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((out_in >> i) & 1u) *reinterpret_cast<uint4*>(out + out_off[i] + c) = w[i];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.empty[stage]);
+      return true;
+    });
   }
-  copies_wait<0>();
+  tc_fence_before();
   __syncthreads();
-  if (tid < 32) tc_free(s.tmem, 128);
+  if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) tc_free(tmem, 2 * ADD_COLS);
 }
 
 // ---- the plan: rows in the order of their adapters, and items of up to 64 of them
@@ -927,6 +1034,7 @@ adapter_plan_kernel(const int* ids, int M, int n, int* order, int4* items, int m
     __syncthreads();
   }
   for (int i = carry[1] + tid; i < max_items; i += PLAN_THREADS) items[i] = make_int4(-1, 0, 0, 0);
+  if (tid == 0) items[max_items] = make_int4(min(carry[1], max_items), 0, 0, 0);
   // rows into their order (which one of an adapter's rows comes first changes nothing that is computed)
   for_rows([&](int i, int b, unsigned same) {
     int at = 0;
@@ -937,13 +1045,13 @@ adapter_plan_kernel(const int* ids, int M, int n, int* order, int4* items, int m
 }
 
 static int plan_items(int M, int n) { return M / MAX_ROWS + (M < n + 1 ? M : n + 1); }
-extern "C" int mi_adapter_plan_sizes(int M, int n, int* max_items) {
+extern "C" int mi_adapter_plan_sizes(int M, int n, int* items) {
   if (M <= FEW_MAX) {
-    *max_items = 0;
+    *items = 0;
     return 0;
   }
   if (n > PLAN_MAX_ADAPTERS) MI_REFUSE("adapter_plan: %d adapters, at most %d with more than %d rows", n, PLAN_MAX_ADAPTERS, FEW_MAX);
-  *max_items = plan_items(M, n);
+  *items = plan_items(M, n) + 1;
   return 0;
 }
 extern "C" int mi_adapter_plan(const int* ids, int M, int n, int* order, void* items, cudaStream_t stream) {
@@ -990,13 +1098,11 @@ static cudaError_t launch_few(const AdapterArgs& g, int max_items, cudaStream_t 
 static int add_tc_stages(int R, int pairs) {
   const int left = 225 * 1024 - (pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM;
   const int n = left / add_stage_bytes(R);
-  // two stages where that leaves room for another block on the SM, else all that fit
-  if ((pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM + 2 * add_stage_bytes(R) <= 112 * 1024) return 2;
   return n > ADD_MAX_STAGES ? ADD_MAX_STAGES : n;
 }
 
 static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t stream) {
-  static size_t allowed[4][64];
+  static size_t allowed[5][64];
   const size_t sums_bytes = SUMS_STAGES * SUMS_STAGE_BYTES + 1024;
   cudaError_t e = allow_smem(adapter_sums_tc_kernel, sums_bytes, allowed[0]);
   if (e != cudaSuccess) return e;
@@ -1007,16 +1113,21 @@ static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t
   if (e != cudaSuccess) return e;
   const int stages = add_tc_stages(g.R, g.pairs);
   const size_t bytes = (size_t)(g.pairs ? 2 : 1) * sums_atoms(g.R) * TC_ATOM + (size_t)stages * add_stage_bytes(g.R) + 1024;
-  const dim3 grid(count_chunks(g, g.span), max_items);
-  if (stages >= 3) {
-    e = allow_smem(adapter_add_tc_kernel<3>, bytes, allowed[1]);
+  const long long tiles = (long long)max_items * g.tiles;
+  const int grid = tiles < 148 ? (int)tiles : 148;
+  if (stages == 4) {
+    e = allow_smem(adapter_add_tc_kernel<4>, bytes, allowed[1]);
+    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<4>), grid, ADD_THREADS, bytes, stream, g);
+  }
+  if (stages == 3) {
+    e = allow_smem(adapter_add_tc_kernel<3>, bytes, allowed[2]);
     return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<3>), grid, ADD_THREADS, bytes, stream, g);
   }
   if (stages == 2) {
-    e = allow_smem(adapter_add_tc_kernel<2>, bytes, allowed[2]);
+    e = allow_smem(adapter_add_tc_kernel<2>, bytes, allowed[3]);
     return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<2>), grid, ADD_THREADS, bytes, stream, g);
   }
-  e = allow_smem(adapter_add_tc_kernel<1>, bytes, allowed[3]);
+  e = allow_smem(adapter_add_tc_kernel<1>, bytes, allowed[4]);
   return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<1>), grid, ADD_THREADS, bytes, stream, g);
 }
 
@@ -1071,10 +1182,13 @@ extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long 
   if (M <= 0 || N <= 0) return 0;
   if (P < 1 || P > ADAPTER_MAX_PARTS) MI_REFUSE("adapter_add: %d parts, at most %d", P, ADAPTER_MAX_PARTS);
   AdapterArgs g = {x, ldx, y, ldy, out, ldo, a, b, ids, ranks, scale, h, nullptr, M, N, K, n, P, R, {end0, end1, end2, end3}, pairs,
-                   0, 0, 1, order, (const int4*)items, constant};
+                   0, 0, 1, order, (const int4*)items, 0, 0, constant};
   const Route r = route_of(y, ldy, x, ldx, a, b, out, ldo, M, N, K, n, P, R, g.ends, pairs, dtype);
   if (r.way != BY_ELEMENTS) {
     if (r.items > 65535) MI_REFUSE("adapter_add: %d rows with %d adapters", M, n);
+    g.max_items = r.way == BY_MANY ? r.items : 0;
+    g.tiles = count_chunks(g, ADD_COLS);
+    if ((long long)r.items * g.tiles > 0x7fffffffLL) MI_REFUSE("adapter_add: %d rows of %d columns", M, N);
     if (M > FEW_MAX && !(order && items)) MI_REFUSE("adapter_add: a plan of %d rows without their order", M);
     g.ks = r.ks;
     g.pairs_of_h = (bf16*)(h + r.floats);
