@@ -27,7 +27,7 @@ struct AdapterArgs {
   const int* ranks;
   const float* scale;
   float* h;                       // [parts of the sum over K][M][P R] the sums of the first product
-  bf16* pairs_of_h;               // [M][P][2][R up to 16s] the same over all of K, as pairs of bfloat16 numbers (many rows)
+  bf16* held;                     // [M][P][held_sums] the same over all of K, in bfloat16 (many rows)
   int M, N, K, n, P, R;
   int ends[ADAPTER_MAX_PARTS];    // where each part's columns end (side by side)
   int pairs;
@@ -665,11 +665,16 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_sums_tc_kernel(const Adapt
   if (tid < 32) tc_free(s.tmem, 128);
 }
 
-// Where the rests of a part's sums stand behind the sums, in elements; whole groups of 16 k
+// A part's sums for the second product: whole groups of 16 k, and behind them their rests for ranks up to 32, where they cost
+// nothing.  Beyond, a sum is rounded to bfloat16 once (off by up to 2^-8 of it; the result, rounded too, is off by as much):
+// with the rests the products double and a stage of the ring goes, and 8192 rows of rank 64 at 4096 x 28672 take 299 us instead of
+// 283.
 __host__ __device__ inline int padded_rank(int R) { return (R + 15) & ~15; }
+__host__ __device__ inline int with_rests(int R) { return R <= 32; }
+__host__ __device__ inline int held_sums(int R) { return (with_rests(R) ? 2 : 1) * padded_rank(R); }
 
-// The sums over all of K, scaled, as pairs of bfloat16 numbers: four sums a thread.
-__global__ void __launch_bounds__(256) adapter_pairs_kernel(const AdapterArgs g) {
+// The sums over all of K, scaled, in bfloat16: four sums a thread.
+__global__ void __launch_bounds__(256) adapter_held_kernel(const AdapterArgs g) {
   mi_pdl_wait();
   mi_pdl_launch_dependents();
   const int rp = padded_rank(g.R), quarter = rp / 4, per_row = g.P * quarter;
@@ -696,13 +701,13 @@ __global__ void __launch_bounds__(256) adapter_pairs_kernel(const AdapterArgs g)
   bf16 hi[4], lo[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) split_bf16(r + q < rank ? f[q] * scale : 0.f, hi[q], lo[q]);
-  bf16* to = g.pairs_of_h + ((size_t)row * g.P + p) * 2 * rp + r;
+  bf16* to = g.held + ((size_t)row * g.P + p) * held_sums(g.R) + r;
   *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
-  *reinterpret_cast<uint2*>(to + rp) = *reinterpret_cast<uint2*>(lo);
+  if (with_rests(g.R)) *reinterpret_cast<uint2*>(to + rp) = *reinterpret_cast<uint2*>(lo);
 }
 
 // Shared memory of the second product: the item's sums, then stages of B and of y
-__host__ __device__ inline int sums_atoms(int R) { return (2 * padded_rank(R) + 63) / 64; }      // a part's sums and rests
+__host__ __device__ inline int sums_atoms(int R) { return (held_sums(R) + 63) / 64; }      // a part's sums and rests
 __host__ __device__ inline int b_atoms(int R) { return (padded_rank(R) + 63) / 64; }
 __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_ATOM + TC_ROWS * ADD_COLS * 2; }
 
@@ -787,14 +792,14 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
     // ---- copies.  Pieces of a row by as many threads, rounded up to a power of two
     constexpr int LAG = STAGES > 2 ? STAGES - 2 : 0;          // tiles under way behind the one just asked for
     const int ct = tid - 32 * ADD_SUM_WARPS;
-    const int h_pieces = 2 * rp / 8, b_pieces = rp / 8, b_shift = b_pieces <= 2 ? 1 : b_pieces <= 4 ? 2 : b_pieces <= 8 ? 3 : 4;
+    const int hp = held_sums(R), h_pieces = hp / 8, b_pieces = rp / 8, b_shift = b_pieces <= 2 ? 1 : b_pieces <= 4 ? 2 : b_pieces <= 8 ? 3 : 4;
     const int bq = ct & ((1 << b_shift) - 1), b_col = ct >> b_shift, b_step = ADD_COPY_THREADS >> b_shift;
-    const int hq = ct & ((2 << b_shift) - 1), h_row = ct >> (b_shift + 1), h_step = ADD_COPY_THREADS >> (b_shift + 1);
+    const int h_shift = b_shift + with_rests(R), hq = ct & ((1 << h_shift) - 1), h_row = ct >> h_shift, h_step = ADD_COPY_THREADS >> h_shift;
     const int yq = ct & 15, yr = ct >> 4;                     // piece `yq` of every 8th row
     constexpr int YN = TC_ROWS * 16 / ADD_COPY_THREADS;
     long long y_off[YN];
     uint32_t y_in = 0;
-    int items = 0, asked = 0, told = 0;                       // begun so far, of those with an adapter; tiles asked for, and said to be there
+    int items = 0, asked = 0, told = 0, last_part = -1;                       // begun so far, of those with an adapter; tiles asked for, and said to be there
     const auto tell = [&](int upto) {
       if (told < upto) smem_for_tensor_cores();
       for (; told < upto; ++told) mbar_arrive(&s.full[told % STAGES]);
@@ -816,7 +821,8 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
       if (j >= STAGES && !mbar_wait(&s.empty[stage], (j / STAGES - 1) & 1, &s.give_up)) return false;
       int part, c, c_end;
       find_chunk(g, chunk, ADD_COLS, part, c, c_end);
-      if (begins && rank > 0) {
+      if ((begins || part != last_part) && rank > 0) {
+        last_part = part;
         // the last item's products have to end first, and for that to be told of all their tiles
         copies_wait<0>();
         tell(j);
@@ -824,9 +830,9 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         ++items;
         if (hq < h_pieces)
           for (int row = h_row; row < item.z; row += h_step) {
-            const bf16* from = g.pairs_of_h + (size_t)__ldcg(g.order + item.y + row) * g.P * 2 * rp + hq * 8;
+            const bf16* from = g.held + (size_t)__ldcg(g.order + item.y + row) * g.P * hp + hq * 8;
             for (int p = 0; p < np; ++p)
-              copy_piece(h_at + (p * ha + hq / 8) * TC_ATOM + row * 128 + (((hq & 7) ^ (row & 7)) << 4), from + (size_t)(part + p) * 2 * rp, 16);
+              copy_piece(h_at + (p * ha + hq / 8) * TC_ATOM + row * 128 + (((hq & 7) ^ (row & 7)) << 4), from + (size_t)(part + p) * hp, 16);
           }
       }
       if (rank > 0 && bq < b_pieces) {
@@ -858,7 +864,8 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
     // ---- products
     if (lane == 0) {
       const uint32_t desc = product_desc(g.pairs ? ADD_COLS / 2 : ADD_COLS);
-      for_tiles(g, [&](int j, const int4&, int rank, bool, bool ends, int) {
+      const int rests = with_rests(R);
+      for_tiles(g, [&](int j, const int4&, int rank, bool, bool ends, int chunk) {
         const int stage = j % STAGES, buf = j & 1;
         if (!mbar_wait(&s.full[stage], (j / STAGES) & 1, &s.give_up)) return false;
         if (j >= 2 && !mbar_wait(&s.free_[buf], (j / 2 - 1) & 1, &s.give_up)) return false;
@@ -867,13 +874,17 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         for (int p = 0; p < np && rank > 0; ++p)
           for (int k = 0; k < rp; k += 16) {
             const uint64_t bd = operand_desc(at + p * 64 * 128 + k / 64 * TC_ATOM + k % 64 * 2);
-            for (int lo = 0; lo < 2; ++lo) {
+            for (int lo = 0; lo <= rests; ++lo) {
               const int e = k + lo * rp;
               tc_mma(tmem + buf * ADD_COLS + p * 64, operand_desc(h_at + (p * ha + e / 64) * TC_ATOM + e % 64 * 2), bd, desc, k > 0 || lo > 0);
             }
           }
         tc_commit(&s.done[buf]);
-        if (ends && rank > 0) tc_commit(&s.h_free);
+        int part, next, c, c_end;
+        find_chunk(g, chunk, ADD_COLS, part, c, c_end);
+        next = part;
+        if (!ends) find_chunk(g, chunk + 1, ADD_COLS, next, c, c_end);
+        if ((ends || next != part) && rank > 0) tc_commit(&s.h_free);
         return true;
       });
     }
@@ -1109,7 +1120,7 @@ static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t
   e = MI_LAUNCH((adapter_sums_tc_kernel), dim3(g.ks, max_items, (g.P * g.R + 127) / 128), TC_THREADS, sums_bytes, stream, g);
   if (e != cudaSuccess) return e;
   const long long quarters = (long long)g.M * g.P * (padded_rank(g.R) / 4);
-  e = MI_LAUNCH((adapter_pairs_kernel), (unsigned)((quarters + 255) / 256), 256, 0, stream, g);
+  e = MI_LAUNCH((adapter_held_kernel), (unsigned)((quarters + 255) / 256), 256, 0, stream, g);
   if (e != cudaSuccess) return e;
   const int stages = add_tc_stages(g.R, g.pairs);
   const size_t bytes = (size_t)(g.pairs ? 2 : 1) * sums_atoms(g.R) * TC_ATOM + (size_t)stages * add_stage_bytes(g.R) + 1024;
@@ -1135,7 +1146,7 @@ static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t
 enum { BY_ELEMENTS, BY_FEW, BY_MANY };
 struct Route {
   int way, items, ks;
-  long long floats, pair_floats;      // of h, and behind it of pairs_of_h
+  long long floats, held_floats;      // of h, and behind it of `held`
 };
 static Route route_of(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b, const void* out,
                       long long ldo, int M, int N, int K, int n, int P, int R, const int* ends, int pairs, int dtype) {
@@ -1149,12 +1160,12 @@ static Route route_of(const void* y, long long ldy, const void* x, long long ldx
   if (M > FEW_MAX && whole && R <= 128 && add_tc_stages(R, pairs) >= 1) {
     r.way = BY_MANY;
     r.items = plan_items(M, n);
-    // Parts of the sum over K: enough blocks for the chip, four stages of 64 k for each
+    // Parts of the sum over K: enough blocks for the chip, eight stages of 64 k for each
     const int blocks = (K + 63) / 64, tiles = (M + TC_ROWS - 1) / TC_ROWS * ((P * R + 127) / 128);
     r.ks = 2 * 148 / tiles;
-    if (r.ks > blocks / 4) r.ks = blocks / 4;
+    if (r.ks > blocks / 8) r.ks = blocks / 8;
     r.ks = r.ks < 1 ? 1 : r.ks > 16 ? 16 : r.ks;
-    r.pair_floats = (long long)M * P * padded_rank(R);
+    r.held_floats = (long long)M * P * held_sums(R) / 2;
   } else {
     r.way = BY_FEW;
     r.items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : plan_items(M, n) * SUB_ITEMS;
@@ -1172,7 +1183,7 @@ extern "C" long long mi_adapter_scratch(const void* y, long long ldy, const void
                                         int end1, int end2, int end3, int pairs, int dtype) {
   const int ends[ADAPTER_MAX_PARTS] = {end0, end1, end2, end3};
   const Route r = route_of(y, ldy, x, ldx, a, b, out, ldo, M, N, K, n, P, R, ends, pairs, dtype);
-  return r.floats + r.pair_floats;
+  return r.floats + r.held_floats;
 }
 
 extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b,
@@ -1191,7 +1202,7 @@ extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long 
     if ((long long)r.items * g.tiles > 0x7fffffffLL) MI_REFUSE("adapter_add: %d rows of %d columns", M, N);
     if (M > FEW_MAX && !(order && items)) MI_REFUSE("adapter_add: a plan of %d rows without their order", M);
     g.ks = r.ks;
-    g.pairs_of_h = (bf16*)(h + r.floats);
+    g.held = (bf16*)(h + r.floats);
     bool starts4 = true;
     for (int p = 0; p + 1 < P && !pairs; ++p) starts4 = starts4 && g.ends[p] % 4 == 0;
     g.vec = starts4 && mi_aligned(y, 8) && mi_aligned(out, 8) && (M == 1 || (ldy % 4 == 0 && ldo % 4 == 0));

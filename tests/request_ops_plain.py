@@ -6,14 +6,15 @@ import torch
 
 
 def adapter_rows(y, x, a, b, ids, scale=None, ranks=None, parts=None, pairs=False):
-    """``(result, magnitude)`` in float64 on the CPU: the magnitude is the same sum with every term's absolute value."""
+    """``(result, magnitude, products)`` in float64 on the CPU: the magnitude is the same sum with every term's absolute value,
+    the products are the second product alone with the first one's sums as they are and every term's absolute value."""
     y, x, a, b = (t.detach().cpu().double() for t in (y, x, a, b))
     n, P, R, _ = a.shape
     N = y.shape[1]
     parts = list(parts) if parts is not None else [N // P] * P if pairs else [N]
     ends = torch.tensor(parts).cumsum(0)
     part_of = torch.arange(N) % 2 if pairs else torch.bucketize(torch.arange(N), ends, right=True)
-    out, mag = y.clone(), y.abs()
+    out, mag, products = y.clone(), y.abs(), torch.zeros_like(y)
     for t, i in enumerate(ids.tolist()):
         if not 0 <= i < n:
             continue
@@ -25,7 +26,8 @@ def adapter_rows(y, x, a, b, ids, scale=None, ranks=None, parts=None, pairs=Fals
         hm = a[i, :, :r].abs() @ x[t].abs()
         out[t] += s * (b[i, :, :r] * h[part_of]).sum(1)
         mag[t] += abs(s) * (b[i, :, :r].abs() * hm[part_of]).sum(1)
-    return out, mag
+        products[t] += abs(s) * (b[i, :, :r].abs() * h.abs()[part_of]).sum(1)
+    return out, mag, products
 
 
 def unpacked(words, V):
