@@ -1178,34 +1178,66 @@ static Route route_of(const void* y, long long ldy, const void* x, long long ldx
   return r;
 }
 
-extern "C" long long mi_adapter_scratch(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b,
-                                        const void* out, long long ldo, int M, int N, int K, int n, int P, int R, int end0,
-                                        int end1, int end2, int end3, int pairs, int dtype) {
-  const int ends[ADAPTER_MAX_PARTS] = {end0, end1, end2, end3};
-  const Route r = route_of(y, ldy, x, ldx, a, b, out, ldo, M, N, K, n, P, R, ends, pairs, dtype);
+// The arguments of a call as one block of 64-bit numbers.
+struct AdapterCall {
+  long long y, ldy, x, ldx, a, b, out, ldo, ids, order, items, scale, ranks, M, N, K, n, P, R, ends[ADAPTER_MAX_PARTS], pairs, constant,
+      dtype, unused;
+};
+static Route route_of(const AdapterCall& c) {
+  const int ends[ADAPTER_MAX_PARTS] = {(int)c.ends[0], (int)c.ends[1], (int)c.ends[2], (int)c.ends[3]};
+  return route_of((const void*)c.y, c.ldy, (const void*)c.x, c.ldx, (const void*)c.a, (const void*)c.b, (const void*)c.out, c.ldo,
+                  (int)c.M, (int)c.N, (int)c.K, (int)c.n, (int)c.P, (int)c.R, ends, (int)c.pairs, (int)c.dtype);
+}
+
+// Floats of scratch memory that a call takes.
+extern "C" long long mi_adapter_scratch(const AdapterCall* c) {
+  const Route r = route_of(*c);
   return r.floats + r.held_floats;
 }
 
-extern "C" int mi_adapter_add(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b,
-                              void* out, long long ldo, const int* ids, const int* order, const void* items, const float* scale,
-                              const int* ranks, float* h, int M, int N, int K, int n, int P, int R, int end0, int end1, int end2,
-                              int end3, int pairs, int constant, int dtype, cudaStream_t stream) {
+extern "C" int mi_adapter_add(const AdapterCall* call, float* h, cudaStream_t stream) {
+  const AdapterCall& c = *call;
+  const long long most = 0x7fffffff;
+  if (c.M > most || c.N > most || c.K > most || c.n > most || c.R > most) MI_REFUSE("adapter_add: sizes beyond 31 bits");
+  const int M = (int)c.M, N = (int)c.N, K = (int)c.K, n = (int)c.n, P = (int)c.P, R = (int)c.R, pairs = c.pairs != 0, dtype = (int)c.dtype;
   if (M <= 0 || N <= 0) return 0;
   if (P < 1 || P > ADAPTER_MAX_PARTS) MI_REFUSE("adapter_add: %d parts, at most %d", P, ADAPTER_MAX_PARTS);
-  AdapterArgs g = {x, ldx, y, ldy, out, ldo, a, b, ids, ranks, scale, h, nullptr, M, N, K, n, P, R, {end0, end1, end2, end3}, pairs,
-                   0, 0, 1, order, (const int4*)items, 0, 0, constant};
-  const Route r = route_of(y, ldy, x, ldx, a, b, out, ldo, M, N, K, n, P, R, g.ends, pairs, dtype);
+  AdapterArgs g = {};
+  g.x = (const void*)c.x;
+  g.ldx = c.ldx;
+  g.y = (const void*)c.y;
+  g.ldy = c.ldy;
+  g.out = (void*)c.out;
+  g.ldo = c.ldo;
+  g.a = (const void*)c.a;
+  g.b = (const void*)c.b;
+  g.ids = (const int*)c.ids;
+  g.order = (const int*)c.order;
+  g.items = (const int4*)c.items;
+  g.ranks = (const int*)c.ranks;
+  g.scale = (const float*)c.scale;
+  g.h = h;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.n = n;
+  g.P = P;
+  g.R = R;
+  for (int p = 0; p < ADAPTER_MAX_PARTS; ++p) g.ends[p] = (int)c.ends[p];
+  g.pairs = pairs;
+  g.constant = c.constant != 0;
+  const Route r = route_of(c);
   if (r.way != BY_ELEMENTS) {
     if (r.items > 65535) MI_REFUSE("adapter_add: %d rows with %d adapters", M, n);
     g.max_items = r.way == BY_MANY ? r.items : 0;
     g.tiles = count_chunks(g, ADD_COLS);
     if ((long long)r.items * g.tiles > 0x7fffffffLL) MI_REFUSE("adapter_add: %d rows of %d columns", M, N);
-    if (M > FEW_MAX && !(order && items)) MI_REFUSE("adapter_add: a plan of %d rows without their order", M);
+    if (M > FEW_MAX && !(g.order && g.items)) MI_REFUSE("adapter_add: a plan of %d rows without their order", M);
     g.ks = r.ks;
     g.held = (bf16*)(h + r.floats);
     bool starts4 = true;
     for (int p = 0; p + 1 < P && !pairs; ++p) starts4 = starts4 && g.ends[p] % 4 == 0;
-    g.vec = starts4 && mi_aligned(y, 8) && mi_aligned(out, 8) && (M == 1 || (ldy % 4 == 0 && ldo % 4 == 0));
+    g.vec = starts4 && mi_aligned(g.y, 8) && mi_aligned(g.out, 8) && (M == 1 || (g.ldy % 4 == 0 && g.ldo % 4 == 0));
     // Blocks with many columns look for their rows and sums once for all of them; a few waves of blocks fill the chip.
     g.span = 2048;
     while (g.span > 256 && (long long)r.items * count_chunks(g, g.span) < 3 * 148) g.span /= 2;

@@ -195,21 +195,26 @@ __global__ void __launch_bounds__(ADJUST_THREADS) adjust_logits_kernel(const Adj
   }
 }
 
-extern "C" int mi_adjust_logits(const float* logits, long long ld_in, float* out, long long ld_out, int B, int V,
-                                const int* slots, const uint32_t* seen, const int* counts, int n_slots,
-                                const float* repetition, const float* presence, const float* frequency,
-                                const int* bias_starts, const int* bias_ids, const float* bias_values, int n_bias,
-                                const uint32_t* masks, const int* mask_rows, int n_masks, cudaStream_t stream) {
+// The arguments of a call as one block of 64-bit numbers.
+struct AdjustCall {
+  long long logits, ld_in, out, ld_out, B, V, slots, seen, counts, n_slots, repetition, presence, frequency, bias_starts, bias_ids,
+      bias_values, n_bias, masks, mask_rows, n_masks;
+};
+
+extern "C" int mi_adjust_logits(const AdjustCall* call, cudaStream_t stream) {
+  const AdjustCall& c = *call;
+  const long long B = c.B, V = c.V, n_bias = c.n_bias;
   if (B <= 0 || V <= 0) return 0;
-  if (n_bias > 0x7fffffff - 65536) MI_REFUSE("adjust_logits: %d biases", n_bias);
-  if (B > 65535) MI_REFUSE("adjust_logits: %d rows, at most 65535", B);
-  if (V > 0x7fffffff - 65536) MI_REFUSE("adjust_logits: vocabulary %d", V);
-  const bool in_place = out == logits;
-  AdjustArgs a = {logits, out, ld_in, ld_out, V, (int)(((long long)V + 31) / 32), slots, seen, counts, n_slots, repetition,
-                  presence, frequency, bias_starts, bias_ids, bias_values, n_bias, masks, mask_rows, n_masks};
-  // (a row whose first columns lie before a boundary may need no more blocks for it: the first block's stretch is the longer)
+  if (n_bias > 0x7fffffff - 65536) MI_REFUSE("adjust_logits: %lld biases", n_bias);
+  if (B > 65535) MI_REFUSE("adjust_logits: %lld rows, at most 65535", B);
+  if (V > 0x7fffffff - 65536) MI_REFUSE("adjust_logits: vocabulary %lld", V);
+  const bool in_place = c.out == c.logits;
+  const AdjustArgs a = {(const float*)c.logits, (float*)c.out, c.ld_in, c.ld_out, (int)V, (int)((V + 31) / 32), (const int*)c.slots,
+                        (const uint32_t*)c.seen, (const int*)c.counts, (int)c.n_slots, (const float*)c.repetition,
+                        (const float*)c.presence, (const float*)c.frequency, (const int*)c.bias_starts, (const int*)c.bias_ids,
+                        (const float*)c.bias_values, (int)n_bias, (const uint32_t*)c.masks, (const int*)c.mask_rows, (int)c.n_masks};
   const int cols = ADJUST_WARP_COLS * (ADJUST_THREADS / 32);
-  const dim3 grid((V + cols - 1) / cols, B);
+  const dim3 grid((unsigned)((V + cols - 1) / cols), (unsigned)B);
   if (in_place)
     MI_LAUNCH((adjust_logits_kernel<true>), grid, ADJUST_THREADS, 0, stream, a);
   else
@@ -332,12 +337,20 @@ record_more_kernel(int* counts, uint32_t* seen, int n_slots, int V, int words, c
   }
 }
 
-extern "C" int mi_record_tokens(int* counts, uint32_t* seen, int n_slots, int V, const int* slots, const int* starts,
-                                const int* tokens, int n_tokens, const int* n_prompt, int B, int fresh,
-                                cudaStream_t stream) {
+struct RecordCall {
+  long long counts, seen, n_slots, V, slots, starts, tokens, n_tokens, n_prompt, B, fresh;
+};
+
+extern "C" int mi_record_tokens(const RecordCall* call, cudaStream_t stream) {
+  const RecordCall& c = *call;
+  if (c.B > 65535) MI_REFUSE("record_tokens: %lld requests, at most 65535", c.B);
+  if (c.V > 0x7fffffff - 65536 || c.n_tokens > 0x7fffffff - 65536 || c.n_slots > 0x7fffffff)
+    MI_REFUSE("record_tokens: vocabulary %lld, %lld tokens, %lld histories", c.V, c.n_tokens, c.n_slots);
+  int* counts = (int*)c.counts;
+  uint32_t* seen = (uint32_t*)c.seen;
+  const int *slots = (const int*)c.slots, *starts = (const int*)c.starts, *tokens = (const int*)c.tokens, *n_prompt = (const int*)c.n_prompt;
+  const int n_slots = (int)c.n_slots, V = (int)c.V, n_tokens = (int)c.n_tokens, B = (int)c.B, fresh = c.fresh != 0;
   if (B <= 0 || V <= 0) return 0;
-  if (B > 65535) MI_REFUSE("record_tokens: %d requests, at most 65535", B);
-  if (V > 0x7fffffff - 65536 || n_tokens > 0x7fffffff - 65536) MI_REFUSE("record_tokens: vocabulary %d, %d tokens", V, n_tokens);
   const int words = (int)(((long long)V + 31) / 32);
   if (!fresh) {
     const int blocks = (n_tokens + RECORD_THREADS * RECORD_EACH - 1) / (RECORD_THREADS * RECORD_EACH);

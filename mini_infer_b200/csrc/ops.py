@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from contextlib import contextmanager
 from ctypes import c_float, c_int, c_void_p
@@ -437,13 +438,9 @@ def _sig_attention_stage(lib: ctypes.CDLL) -> None:
 
 
 def _sig_adapters(lib: ctypes.CDLL) -> None:
-    ll = ctypes.c_longlong
-    lib.mi_adapter_add.argtypes = [c_void_p, ll, c_void_p, ll, c_void_p, c_void_p, c_void_p, ll, c_void_p, c_void_p, c_void_p,
-                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                   c_int, c_int, c_int, c_int, c_void_p]
-    lib.mi_adapter_scratch.argtypes = [c_void_p, ll, c_void_p, ll, c_void_p, c_void_p, c_void_p, ll, c_int, c_int, c_int, c_int,
-                                       c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]
-    lib.mi_adapter_scratch.restype = ll
+    lib.mi_adapter_add.argtypes = [ctypes.c_char_p, c_void_p, c_void_p]
+    lib.mi_adapter_scratch.argtypes = [ctypes.c_char_p]
+    lib.mi_adapter_scratch.restype = ctypes.c_longlong
     lib.mi_adapter_plan_sizes.argtypes = [c_int, c_int, ctypes.POINTER(c_int)]
     lib.mi_adapter_plan.argtypes = [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]
     lib.mi_adapters_status.argtypes = [c_int]
@@ -451,12 +448,8 @@ def _sig_adapters(lib: ctypes.CDLL) -> None:
 
 
 def _sig_logits(lib: ctypes.CDLL) -> None:
-    ll = ctypes.c_longlong
-    lib.mi_adjust_logits.argtypes = [c_void_p, ll, c_void_p, ll, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
-                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
-                                     c_void_p]
-    lib.mi_record_tokens.argtypes = [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
-                                     c_int, c_void_p]
+    lib.mi_adjust_logits.argtypes = [ctypes.c_char_p, c_void_p]
+    lib.mi_record_tokens.argtypes = [ctypes.c_char_p, c_void_p]
 
 
 _SIGNATURES = {
@@ -2967,17 +2960,27 @@ def branch_norm_then_norm(stream: torch.Tensor, branch: torch.Tensor, gain_y: to
 # --------------------------------------------------------------------------------------- what a request brings of its own
 
 
+# Calls of these operators are short, and there is one for every projection of a step: what costs the host is asked once per
+# tensor, and the arguments go to the library as one block of 64-bit numbers, in the order of its structures.
+_ADAPTER_BLOCK = struct.Struct("27q").pack
+_ADJUST_BLOCK = struct.Struct("20q").pack
+_RECORD_BLOCK = struct.Struct("11q").pack
+
+
 def _same_device(what: str, *tensors: torch.Tensor | None) -> None:
     """Every tensor on the current CUDA device: the kernels are launched on its current stream."""
     here = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at == here:
+            continue
+        if at < 0:
             raise KernelError(f"{what}: kernels run on CUDA tensors only (got a tensor on {t.device})")
         if here is None:
             here = torch._C._cuda_getDevice()
-        if t.get_device() != here:
+        if at != here:
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
 
 
@@ -2995,7 +2998,7 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _vector(what: str, name: str, t: torch.Tensor | None, dtype: torch.dtype, n: int) -> None:
-    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous()):
+    if t is not None and (t.dtype is not dtype or t.numel() != n or t.dim() != 1 or not t.is_contiguous()):
         raise KernelError(f"{what}: {name} must be a contiguous {dtype} vector of {n}")
 
 
@@ -3094,12 +3097,13 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     if M == 0 or N == 0:
         return out
     lib = _waiting_lib("adapters", x.device)
-    h = torch.empty(lib.mi_adapter_scratch(_ptr(y), y.stride(0), _ptr(x), x.stride(0), _ptr(a), _ptr(b), _ptr(out), out.stride(0), M,
-                                           N, K, n, P, R, *ends, 1 if pairs else 0, code), dtype=torch.float32, device=x.device)
-    rc = lib.mi_adapter_add(_ptr(y), y.stride(0), _ptr(x), x.stride(0), _ptr(a), _ptr(b), _ptr(out), out.stride(0),
-                            _ptr(plan.ids), _ptr(plan.order), _ptr(plan.items), _ptr(scale), _ptr(ranks), _ptr(h), M, N, K, n, P, R,
-                            *ends, 1 if pairs else 0, 1 if w_constant else 0, code, _stream())
-    _finish(lib, rc, what)
+    order, items = plan.order, plan.items
+    block = _ADAPTER_BLOCK(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), out.data_ptr(),
+                           out.stride(0), plan.ids.data_ptr(), 0 if order is None else order.data_ptr(),
+                           0 if items is None else items.data_ptr(), 0 if scale is None else scale.data_ptr(),
+                           0 if ranks is None else ranks.data_ptr(), M, N, K, n, P, R, *ends, pairs, w_constant, code, 0)
+    h = torch.empty(lib.mi_adapter_scratch(block), dtype=torch.float32, device=x.device)
+    _finish(lib, lib.mi_adapter_add(block, h.data_ptr(), _stream()), what)
     return out
 
 
@@ -3178,11 +3182,14 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor | None = None, *, slot
             raise KernelError(f"{what}: out overlaps the logits without being them")
     if B == 0 or V == 0:
         return out
+    def at(t):
+        return 0 if t is None else t.data_ptr()
+
     lib = _lib("logits")
-    rc = lib.mi_adjust_logits(_ptr(logits), logits.stride(0), _ptr(out), out.stride(0), B, V, _ptr(slots), _ptr(seen),
-                              _ptr(counts), n_slots, _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(starts), _ptr(ids),
-                              _ptr(values), n_bias, _ptr(masks), _ptr(mask_rows), n_masks, _stream())
-    _finish(lib, rc, what)
+    block = _ADJUST_BLOCK(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), B, V, at(slots), at(seen), at(counts),
+                          n_slots, at(repetition), at(presence), at(frequency), at(starts), at(ids), at(values), n_bias, at(masks),
+                          at(mask_rows), n_masks)
+    _finish(lib, lib.mi_adjust_logits(block, _stream()), what)
     return out
 
 
@@ -3217,6 +3224,7 @@ def record_tokens(counts: torch.Tensor, seen: torch.Tensor, slots: torch.Tensor 
     if B == 0 or V == 0:
         return
     lib = _lib("logits")
-    rc = lib.mi_record_tokens(_ptr(counts), _ptr(seen), n_slots, V, _ptr(slots), _ptr(starts), _ptr(tokens), tokens.shape[0],
-                              _ptr(n_prompt), B, 1 if fresh else 0, _stream())
-    _finish(lib, rc, what)
+    block = _RECORD_BLOCK(counts.data_ptr(), seen.data_ptr(), n_slots, V, 0 if slots is None else slots.data_ptr(),
+                          0 if starts is None else starts.data_ptr(), tokens.data_ptr(), tokens.shape[0],
+                          0 if n_prompt is None else n_prompt.data_ptr(), B, fresh)
+    _finish(lib, lib.mi_record_tokens(block, _stream()), what)
