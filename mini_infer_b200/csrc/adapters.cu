@@ -320,8 +320,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) adapter_sums_kernel(const Ada
 //
 // KG: groups of 32 k (0: as many as there are).  Sums and their rests take two passes, but for items of up to four rows, where the rests
 // stand in the place of four more tokens, and (FOLD) for up to 16 k, where they stand in the place of 16 more.
-template <int KG, bool FOLD>
-__global__ void __launch_bounds__(TILE_THREADS, 3) adapter_add_kernel(const AdapterArgs g) {
+// BLOCKS: of an SM.  A grid that fits at two has the registers of two: 16 rows, ranks 4 to 32, 14336 x 4096 13.0 us become 9.9, one row
+// at 4096 x 6144 7.3 become 6.5; 128 rows at 4096 x 28672, which does not, would take 31.4 instead of 22.8.
+template <int KG, bool FOLD, int BLOCKS>
+__global__ void __launch_bounds__(TILE_THREADS, BLOCKS) adapter_add_kernel(const AdapterArgs g) {
   extern __shared__ __align__(16) unsigned char add_smem[];
   bf16* h = (bf16*)add_smem;                                  // [parts of the block][hi, lo][FEW_ROWS][stride]
   __shared__ int rows[FEW_ROWS];
@@ -1092,18 +1094,21 @@ static cudaError_t allow_smem(K kernel, size_t bytes, size_t* allowed) {
 }
 
 static cudaError_t launch_few(const AdapterArgs& g, int max_items, cudaStream_t stream) {
-  static size_t allowed[64];
+  static size_t allowed[8][64];
   const int groups = (g.P * g.R + SUM_GROUP - 1) / SUM_GROUP;
   cudaError_t e = MI_LAUNCH((adapter_sums_kernel), dim3(g.ks, max_items, groups), TILE_THREADS, 0, stream, g);
   if (e != cudaSuccess) return e;
   const size_t bytes = (size_t)(g.pairs ? 2 : 1) * 2 * FEW_ROWS * h_stride(g.R) * 2;
   const dim3 grid(count_chunks(g, g.span), max_items);
-  if (g.R <= 16) return MI_LAUNCH((adapter_add_kernel<1, true>), grid, TILE_THREADS, bytes, stream, g);
-  if (g.R <= 32) return MI_LAUNCH((adapter_add_kernel<1, false>), grid, TILE_THREADS, bytes, stream, g);
-  if (g.R <= 64) return MI_LAUNCH((adapter_add_kernel<2, false>), grid, TILE_THREADS, bytes, stream, g);
-  e = allow_smem(adapter_add_kernel<0, false>, bytes, allowed);
-  if (e != cudaSuccess) return e;
-  return MI_LAUNCH((adapter_add_kernel<0, false>), grid, TILE_THREADS, bytes, stream, g);
+  const auto run = [&](auto two, auto three, size_t* room) {
+    const bool few = (long long)grid.x * grid.y <= 2 * 148;
+    const cudaError_t e = allow_smem(few ? two : three, bytes, room + (few ? 0 : 64));
+    return e != cudaSuccess ? e : MI_LAUNCH((few ? two : three), grid, TILE_THREADS, bytes, stream, g);
+  };
+  if (g.R <= 16) return run(adapter_add_kernel<1, true, 2>, adapter_add_kernel<1, true, 3>, allowed[0]);
+  if (g.R <= 32) return run(adapter_add_kernel<1, false, 2>, adapter_add_kernel<1, false, 3>, allowed[2]);
+  if (g.R <= 64) return run(adapter_add_kernel<2, false, 2>, adapter_add_kernel<2, false, 3>, allowed[4]);
+  return run(adapter_add_kernel<0, false, 2>, adapter_add_kernel<0, false, 3>, allowed[6]);
 }
 
 static int add_tc_stages(int R, int pairs) {

@@ -3086,7 +3086,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
         _vector(what, "ranks", ranks, torch.int32, n)
     if out is None:
         _same_device(what, x, y, a, b, plan.ids, scale, ranks)
-        out = torch.empty((M, N), dtype=dtype, device=x.device)
+        out = torch.empty_like(y) if y.is_contiguous() else torch.empty((M, N), dtype=dtype, device=x.device)
     else:
         if out.shape != y.shape or out.dtype != dtype or (N and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise KernelError(f"{what}: out must be [M, N] in the operands' dtype, rows apart, with unit inner stride")
@@ -3173,7 +3173,7 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor | None = None, *, slot
         raise KernelError(f"{what}: the rows of the logits overlap")
     _same_device(what, logits, out, slots, seen, counts, repetition, presence, frequency, starts, ids, values, masks, mask_rows)
     if out is None:
-        out = torch.empty((B, V), dtype=torch.float32, device=logits.device)
+        out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((B, V), dtype=torch.float32, device=logits.device)
     else:
         if out.dtype != torch.float32 or out.shape != logits.shape or (V and out.stride(1) != 1) or (B > 1 and out.stride(0) < V):
             raise KernelError(f"{what}: out must be fp32 [B, V], rows apart, with unit inner stride")
