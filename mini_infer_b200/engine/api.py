@@ -19,21 +19,27 @@ from .scheduler import ContinuousScheduler, GenerationResult, Request
 
 def generate(runner: ModelRunner, prompts: Sequence[Sequence[int]], *, max_tokens: int = 16,
              sampling_params: SamplingParams | Sequence[SamplingParams] | None = None,
+             adapters: str | None | Sequence[str | None] = None,
              max_concurrent: int = 16, chunk_size: int | None = None, max_tokens_per_step: int = 2048,
              decode_headroom_blocks: int = 8, eos_token_ids: Sequence[int] = ()) -> list[GenerationResult]:
-    """Generate for every prompt (token ids) with continuous batching; results in order."""
+    """Generate for every prompt (token ids) with continuous batching; results in order.  ``adapters``: the name of a low-rank adapter
+    that the runner has loaded, for all prompts or one each (None: none)."""
     if sampling_params is None:
         sampling_params = SamplingParams()
     if isinstance(sampling_params, SamplingParams):
         sampling_params = [sampling_params] * len(prompts)
+    if adapters is None or isinstance(adapters, str):
+        adapters = [adapters] * len(prompts)
+    if len(adapters) != len(prompts):
+        raise ValueError(f"{len(adapters)} adapters for {len(prompts)} prompts")
     scheduler = ContinuousScheduler(
         runner, max_concurrent=max_concurrent, chunk_size=chunk_size,
         max_tokens_per_step=max_tokens_per_step, decode_headroom_blocks=decode_headroom_blocks,
         eos_token_ids=eos_token_ids,
     )
     return scheduler.generate(
-        [Request(prompt=list(p), sampling_params=sp, max_tokens=max_tokens)
-         for p, sp in zip(prompts, sampling_params)]
+        [Request(prompt=list(p), sampling_params=sp, max_tokens=max_tokens, adapter=a)
+         for p, sp, a in zip(prompts, sampling_params, adapters)]
     )
 
 

@@ -15,8 +15,10 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..config.registry import load_config
+from ..parts.adapters import AdapterBank
 from ..parts.model import DecoderModel
-from ..weights.loader import bind_state_dict, load_weights
+from ..weights.adapters import adapter_scale, pair_matrices, read_adapter
+from ..weights.loader import WeightLoadError, bind_state_dict, load_weights
 from .step import StepEntry, StepResult, StepRunner
 
 DTYPES = {
@@ -63,6 +65,7 @@ class ModelRunner:
         self.max_positions = model.spec.max_positions
         self.num_blocks = num_blocks
         self.block_size = block_size
+        self._adapter_names: list[str | None] | None = None      # by index; None: adapters are off
 
     @classmethod
     def from_pretrained(cls, model_dir: str | os.PathLike, *, device="cuda:0", dtype="bfloat16",
@@ -109,6 +112,96 @@ class ModelRunner:
         bind_random(model, seed, tdtype, device, std=std, gain_std=gain_std, std_overrides=std_overrides)
         return cls(model, cfg, num_blocks=num_blocks, block_size=block_size, max_requests=max_requests,
                    cuda_graph=cuda_graph)
+
+    # -- adapters -----------------------------------------------------------------------
+
+    def enable_adapters(self, count: int = 8, rank: int = 16) -> None:
+        """Make room for ``count`` low-rank adapters of rank up to ``rank`` beside every product of the model that takes them
+        (``Part.adapted``).  Once, before the first is loaded."""
+        if self._adapter_names is not None:
+            raise ValueError("adapters are enabled already")
+        if count <= 0 or rank <= 0:
+            raise ValueError(f"room for {count} adapters of rank {rank}")
+        if rank > 256:
+            raise ValueError(f"adapters of rank {rank}: at most 256")
+        held = -(-rank // 8) * 8          # whole pieces of 16 bytes
+        parts = [p for p in self.model.all_parts() if p.adapted()]
+        if not parts:
+            raise ValueError("no part of this model takes adapters")
+        for p in parts:
+            p.banks = {q.name: AdapterBank(q, count, held, self.dtype, self.device) for q in p.adapted()}
+        self._adapter_names = [None] * count
+        self._adapter_users = [0] * count
+        self._adapter_rank = rank
+        self.stepper.adapter_count = count
+
+    def load_adapter(self, name: str, source, config: Mapping[str, Any] | None = None) -> int:
+        """Load an adapter under ``name`` and return its index: ``source`` is a folder (``weights.read_adapter``), or the adapter's
+        tensors by name with ``config`` (``r``, ``lora_alpha``).  Adapters need not be enabled before: room for eight of this
+        one's rank is then made."""
+        if isinstance(source, (str, os.PathLike)):
+            if config is not None:
+                raise ValueError("a folder brings its own configuration")
+            config, source = read_adapter(source)
+        if config is None:
+            raise ValueError("an adapter's tensors need its configuration")
+        matrices, scale = pair_matrices(source), adapter_scale(config)
+        rank = max(a.shape[0] for a, _ in matrices.values())
+        takes: dict[str, tuple[int, int]] = {}
+        for p in self.model.all_parts():
+            for q in p.adapted():
+                for local, width in zip(q.tensors, q.widths):
+                    takes[p.spec.tensor_name(local)] = (width, q.inputs)
+        unknown = sorted(n for n in matrices if n not in takes)
+        wrong = sorted((n, takes[n], (b.shape[0], a.shape[1])) for n, (a, b) in matrices.items()
+                       if n in takes and takes[n] != (b.shape[0], a.shape[1]))
+        if unknown or wrong:
+            raise WeightLoadError(f"adapter {name!r} does not fit the model: "
+                                  + "; ".join(filter(None, [f"no product that takes adapters: {unknown}" if unknown else "",
+                                                            f"sizes (expected, found): {wrong}" if wrong else ""])),
+                                  unexpected=unknown, mismatched=wrong)
+        if self._adapter_names is None:
+            self.enable_adapters(rank=rank)
+        if rank > self._adapter_rank:
+            raise ValueError(f"adapter {name!r} has rank {rank}, room is for {self._adapter_rank}")
+        if name in self._adapter_names:
+            raise ValueError(f"an adapter {name!r} is loaded already")
+        if None not in self._adapter_names:
+            raise ValueError(f"all {len(self._adapter_names)} places for adapters are taken")
+        index = self._adapter_names.index(None)
+        with torch.inference_mode():
+            for p in self.model.all_parts():
+                for q in (p.adapted() if p.banks is not None else ()):
+                    mine = {local: matrices[p.spec.tensor_name(local)] for local in q.tensors
+                            if p.spec.tensor_name(local) in matrices}
+                    p.banks[q.name].put(index, mine, scale)
+        self._adapter_names[index] = name
+        return index
+
+    def unload_adapter(self, name: str) -> None:
+        """Give an adapter's place back; refused while requests use it."""
+        index = self.adapter_index(name)
+        if self._adapter_users[index]:
+            raise ValueError(f"adapter {name!r} is in use by {self._adapter_users[index]} requests")
+        with torch.inference_mode():
+            for p in self.model.all_parts():
+                for bank in (p.banks or {}).values():
+                    bank.clear(index)
+        self._adapter_names[index] = None
+
+    def adapter_index(self, name: str) -> int:
+        if self._adapter_names is None or name is None or name not in self._adapter_names:
+            raise ValueError(f"no adapter {name!r} is loaded")
+        return self._adapter_names.index(name)
+
+    def hold_adapter(self, name: str) -> int:
+        """The adapter's index, for a request that uses it until ``release_adapter``."""
+        index = self.adapter_index(name)
+        self._adapter_users[index] += 1
+        return index
+
+    def release_adapter(self, index: int) -> None:
+        self._adapter_users[index] -= 1
 
     # -- requests -----------------------------------------------------------------------
 

@@ -38,9 +38,12 @@ import enum
 import json
 import threading
 import time
-from typing import Callable, Hashable, Sequence
+from typing import Any, Callable, Hashable, Sequence
+
+import numpy as np
 
 from ..cache.manager import CacheManager, OutOfPages
+from ..sampling.adjust import AdjustedRow, LogitsAdjuster, mask_any, mask_words
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import default_seed
 from .step import StepEntry
@@ -64,6 +67,10 @@ class Request:
     prompt: Sequence[int] | str
     sampling_params: SamplingParams = dataclasses.field(default_factory=SamplingParams)
     max_tokens: int = 16
+    adapter: str | None = None      # name of a low-rank adapter that the runner has loaded
+    # a grammar: given the tokens generated so far, the ids of the tokens that may come next, or their bits (a numpy int32
+    # array of ceil(V / 32) words); None: any token.  No token at all ends the request as "stop".
+    token_mask: Callable[[list[int]], Any] | None = None
 
 
 @dataclasses.dataclass
@@ -112,6 +119,8 @@ class RunningRequest:
         self.on_token: Callable[[int], None] | None = None
         self.cancel_requested = False
         self.in_flight_after_done = False       # finished while a step launched ahead still writes its pages
+        self.adapter = -1                       # the runner's index of the request's adapter
+        self.mask_ended = False                 # the grammar allows no further token
 
     def result(self, detokenize=None) -> GenerationResult:
         text = detokenize(self.generated) if detokenize else ""
@@ -219,6 +228,7 @@ class ContinuousScheduler:
         self.lookahead = lookahead
         self._inflight: _InFlightStep | None = None
         self.wasted_tokens = 0
+        self._adjuster: LogitsAdjuster | None = None      # made by the first request that needs one
 
     # ------------------------------------------------------------------ public
 
@@ -232,12 +242,21 @@ class ContinuousScheduler:
             prompt_ids = [int(t) for t in prompt]
         if request.max_tokens <= 0:
             raise ValueError("max_tokens must be positive")
+        vocab_size = getattr(self.runner, "vocab_size", None)
+        if vocab_size is not None:
+            request.sampling_params.check_vocabulary(vocab_size)
         with self._lock:
+            adapter = -1
+            if request.adapter is not None:
+                if not hasattr(self.runner, "hold_adapter"):
+                    raise ValueError(f"no adapter {request.adapter!r}: this runner takes none")
+                adapter = self.runner.hold_adapter(request.adapter)
             rid = self._next_rid
             self._next_rid += 1
             seed = request.sampling_params.seed
             rr = RunningRequest(rid, request, prompt_ids, default_seed(rid) if seed is None else seed)
             rr.on_token = on_token
+            rr.adapter = adapter
             if not prompt_ids:
                 self._finish(rr, "stop")        # nothing to condition on (reference :703-707)
             elif self.max_positions is not None and len(prompt_ids) >= self.max_positions:
@@ -348,12 +367,15 @@ class ContinuousScheduler:
         self.steps += 1
         wanting = [rr for rr, e in zip(owners, entries) if e.want]
         if wanting:
+            rows = self._adjust(result.logits, wanting)
             ids = self.sampler.sample(
                 result.logits,
                 [rr.request.sampling_params for rr in wanting],
                 [rr.seed for rr in wanting],
                 [len(rr.generated) for rr in wanting],
             )
+            if rows is not None:
+                self._adjuster.record(ids, rows)
             health = self._queue_health_read()
             ids = [int(t) for t in (ids.tolist() if hasattr(ids, "tolist") else ids)]
         else:
@@ -448,12 +470,15 @@ class ContinuousScheduler:
         self.steps += 1
         # the draw index counts the tokens a request has been given, the one in flight included
         ahead = 0 if device_tokens is None else 1
+        rows = self._adjust(result.logits, owners)
         sampled = self.sampler.sample(
             result.logits,
             [rr.request.sampling_params for rr in owners],
             [rr.seed for rr in owners],
             [len(rr.generated) + ahead for rr in owners],
         )
+        if rows is not None:
+            self._adjuster.record(sampled, rows)
         ready = None
         if isinstance(sampled, torch.Tensor) and sampled.is_cuda:
             host = torch.empty(sampled.shape, dtype=sampled.dtype, pin_memory=True)
@@ -481,8 +506,8 @@ class ContinuousScheduler:
             return None
         with self._lock:
             if self._waiting or any(rr.cancel_requested or rr.state is not RequestState.DECODING
-                                    for rr in self._live):
-                return None
+                                    or rr.request.token_mask is not None for rr in self._live):
+                return None                      # (a grammar has to see a token before it says what may follow)
             keep: list[int] = []
             for i, rr in enumerate(cur.owners):
                 if rr.in_flight_after_done or rr.state is not RequestState.DECODING:
@@ -502,7 +527,7 @@ class ContinuousScheduler:
             if cur.sampled.is_cuda:
                 index = index.pin_memory().to(cur.sampled.device, non_blocking=True)
             tokens = cur.sampled.index_select(0, index)
-        entries = [StepEntry(rr.rid, [0], [0]) for rr in owners]
+        entries = [StepEntry(rr.rid, [0], [0], rr.adapter) for rr in owners]
         return self._launch(entries, owners, tokens.to(torch.int32))
 
     def _collect(self, cur: _InFlightStep, check: bool = True) -> None:
@@ -637,13 +662,15 @@ class ContinuousScheduler:
             else:
                 tokens = rr.feed[rr.fed:rr.fed + n]
                 want = [n - 1] if rr.fed + n == len(rr.feed) else []
-            entries.append(StepEntry(rr.rid, tokens, want))
+            entries.append(StepEntry(rr.rid, tokens, want, rr.adapter))
             owners.append(rr)
         return entries, owners
 
     def _preempt(self, rr: RunningRequest) -> None:
         self._release(rr)
         self._live.remove(rr)
+        if self._adjuster is not None:
+            self._adjuster.forget(rr.rid)       # its history is written anew when it comes back
         rr.feed = list(rr.prompt_ids) + list(rr.generated)
         # (a decoding request's pending token is the last of ``generated``, so it is in ``feed``)
         rr.fed = 0
@@ -662,7 +689,7 @@ class ContinuousScheduler:
         ``still_in_flight`` a step launched ahead holds the request: if it ends here, its
         pages stay until that step has been read.  The request's streaming callback is not
         called here (the lock is held) but noted in ``emitted`` for ``_emit``."""
-        if token in self.eos_token_ids:
+        if token in self.eos_token_ids or rr.mask_ended:
             self._retire(rr, "stop", still_in_flight)
             return
         rr.generated.append(token)
@@ -685,7 +712,34 @@ class ContinuousScheduler:
             self._live.remove(rr)
         self._finish(rr, reason)
 
+    def _adjust(self, logits, rrs: Sequence[RunningRequest]) -> "list[AdjustedRow] | None":
+        """What the requests ask of their rows of ``logits``, in place; None where none asks for anything."""
+        if all(not rr.request.sampling_params.adjusted and rr.request.token_mask is None for rr in rrs):
+            return None
+        if self._adjuster is None:
+            self._adjuster = LogitsAdjuster(self.runner.device, self.runner.vocab_size, self.max_concurrent)
+        V = self.runner.vocab_size
+        rows = []
+        for rr in rrs:
+            row = AdjustedRow(rr.rid, rr.request.sampling_params, rr.prompt_ids, rr.generated)
+            if rr.request.token_mask is not None:
+                said = rr.request.token_mask(list(rr.generated))
+                if said is not None:
+                    row.words = said if getattr(said, "dtype", None) == np.int32 else mask_words(said, V)
+                    if row.words.shape != (-(-V // 32),):
+                        raise ValueError(f"a mask of {row.words.shape} words for {V} tokens")
+                    row.words = self._adjuster.mask_of(row)
+                    rr.mask_ended = not mask_any(row.words, V)
+            rows.append(row)
+        self._adjuster.apply(logits, rows)
+        return rows
+
     def _finish(self, rr: RunningRequest, reason: str) -> None:
+        if self._adjuster is not None:
+            self._adjuster.forget(rr.rid)
+        if rr.adapter >= 0:
+            self.runner.release_adapter(rr.adapter)
+            rr.adapter = -1
         rr.state = RequestState.DONE
         rr.finish_reason = reason
         rr.done.set()

@@ -36,6 +36,7 @@ class StepEntry:
     rid: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = field(default_factory=tuple)
+    adapter: int = -1      # index of the low-rank adapter that the request's tokens use (-1: none)
 
 
 @dataclass
@@ -81,7 +82,7 @@ class StepRunner:
     how decode attention spreads its keys over blocks are all read from device memory when the
     graph runs); the reference keeps such graphs per batch bucket (``engine/paged_decode_graph.py:67-225``).
     Everything else runs kernel by kernel, and so does every step of a model one of whose parts
-    is not ``graph_safe``.
+    is not ``graph_safe``.  Steps of which a request has an adapter are other graphs than those of which none has.
 
     The block tables live on the device (``CacheManager.block_tables``); a step uploads only
     the page ids the host has just handed out and scatters them in before its first kernel,
@@ -102,6 +103,7 @@ class StepRunner:
         self.sm_count = ops.sm_count(self.device) if self.device is not None and self.device.type == "cuda" else 148
         self.steps_run = 0
         self.last_h2d_bytes = 0
+        self.adapter_count = 0      # adapters that the model's parts hold (0: no step may use one)
 
     # ------------------------------------------------------------------ planning
 
@@ -123,6 +125,8 @@ class StepRunner:
                     if not 0 <= int(t) < V:
                         raise StepError(f"request {e.rid!r}: token id {t} is outside [0, {V})")
             arrays.append(None if check else ids)
+            if not -1 <= e.adapter < self.adapter_count:
+                raise StepError(f"request {e.rid!r}: adapter {e.adapter} of {self.adapter_count}")
             for w in e.want:
                 if not 0 <= int(w) < len(e.tokens):
                     raise StepError(f"request {e.rid!r}: wanted place {w} is outside its {len(e.tokens)} tokens")
@@ -172,6 +176,8 @@ class StepRunner:
             ("q_len", q_len), ("kv_len", kv_len), ("state_slot", plan.state_slots),
             ("want_rows", want_rows),
         ]
+        if any(e.adapter >= 0 for e in entries):
+            parts.append(("adapter_ids", np.repeat([e.adapter for e in entries], q_len)))
         n_groups = len(self.cache.groups)
         capacity, overflow = [0] * n_groups, [[] for _ in range(n_groups)]
         for gi, g in enumerate(self.cache.groups):
@@ -247,7 +253,7 @@ class StepRunner:
         host.numpy()[:] = hp.buffer
         slot = None
         if graphed:
-            key = (B,)
+            key = (B,) if "adapter_ids" not in hp.offsets else (B, "adapters")
             slot = self._graphs.get(key)
             if slot is None:
                 slot = GraphSlot(device_buffer=torch.empty(host.numel(), dtype=torch.int32, device=self.device))
@@ -289,6 +295,8 @@ class StepRunner:
             # the longest context its block tables can hold
             max_kv_len=(max(self.cache.table_width, default=1) * self.cache.page_size) if graphed else max(hp.kv_len),
         )
+        if "adapter_ids" in hp.offsets:
+            ctx.adapter_ids = view("adapter_ids")
         ctx.table_updates = [(view(f"updates{gi}"), view(f"update_count{gi}"), hp.update_capacity[gi])
                              for gi in range(len(self.cache.groups))]
         if self._layer_caches is None:     # the views never change: build them once
@@ -329,6 +337,8 @@ class StepRunner:
     def _run(self, ctx: StepContext, caches, want, n_want: int) -> torch.Tensor:
         """The device work of a step: the new page ids into the block tables, then the model."""
         ctx.scratch.clear()   # what the parts share within a step is made anew in every run (and in a capture)
+        if ctx.adapter_ids is not None:
+            ctx.adapters = ops.adapter_plan(ctx.adapter_ids, self.adapter_count)
         self.apply_table_updates(ctx)
         return self.model.forward(ctx, caches, want, n_want)
 

@@ -46,6 +46,13 @@ def main(argv=None) -> int:
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--sampling-seed", type=int, default=None)
+    ap.add_argument("--repetition-penalty", type=float, default=1.0)
+    ap.add_argument("--frequency-penalty", type=float, default=0.0)
+    ap.add_argument("--presence-penalty", type=float, default=0.0)
+    ap.add_argument("--logit-bias", action="append", default=[], metavar="ID:NUMBER",
+                    help="added to a token's logit (-inf: never; repeatable)")
+    ap.add_argument("--allowed-token-ids", help="no other token is chosen (comma or space separated)")
+    ap.add_argument("--adapter", help="folder of a low-rank adapter (adapter_config.json + adapter_model.safetensors)")
     ap.add_argument("--num-blocks", type=int, default=int(env.get("MINI_INFER_NUM_BLOCKS", 1024)))
     ap.add_argument("--block-size", type=int, default=int(env.get("MINI_INFER_BLOCK_SIZE", 16)))
     ap.add_argument("--max-concurrent", type=int, default=16)
@@ -95,9 +102,15 @@ def main(argv=None) -> int:
         max_tokens_per_step=args.max_tokens_per_step, decode_headroom_blocks=args.decode_headroom_blocks,
         eos_token_ids=eos, tokenizer=tokenizer, trace_out=args.trace_out,
     )
+    if args.adapter:
+        runner.load_adapter("adapter", args.adapter)
+    bias = {int(t): float(b) for t, b in (item.split(":", 1) for item in args.logit_bias)}
     params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
-                            seed=args.sampling_seed)
-    results = scheduler.generate([Request(p, params, args.max_tokens) for p in prompts])
+                            seed=args.sampling_seed, repetition_penalty=args.repetition_penalty,
+                            frequency_penalty=args.frequency_penalty, presence_penalty=args.presence_penalty,
+                            logit_bias=bias or None,
+                            allowed_token_ids=parse_ids(args.allowed_token_ids) if args.allowed_token_ids else None)
+    results = scheduler.generate([Request(p, params, args.max_tokens, "adapter" if args.adapter else None) for p in prompts])
     scheduler.stop()
     for r in results:
         print(json.dumps({"tokens": r.tokens, "text": r.text, "finish_reason": r.finish_reason,

@@ -1,5 +1,6 @@
 """Parts a decoder is put together from (see ``base`` for the interfaces)."""
 
+from .adapters import AdaptedProduct, AdapterBank  # noqa: F401
 from .base import (  # noqa: F401
     Arrangement,
     DeferredNorm,

@@ -151,6 +151,10 @@ class StepContext:
     # what parts of different layers share within one step (a table that depends on the step's
     # positions only, say): filled by whoever needs it first (two parts side by side, ``Part.alone``: each for itself)
     scratch: dict = field(default_factory=dict)
+    # the low-rank adapter of every token (int32, -1: none), and the plan that is made of it in front of the model; None where no
+    # request of the step has an adapter
+    adapter_ids: torch.Tensor | None = None
+    adapters: Any = None
 
     def q_tiles(self, tokens: int) -> tuple[torch.Tensor, torch.Tensor, int]:
         """``(tile_request, tile_first_token, n_tiles)`` for tiles of ``tokens`` tokens."""
@@ -200,6 +204,19 @@ class Part:
              device: torch.device) -> None:
         """Receive the declared tensors (already on ``device``); ``dtype`` is the compute
         dtype of activations (float32 or bfloat16)."""
+
+    # the banks of low-rank adapters beside the part's products, by the names that ``adapted`` gives them (None: adapters are off)
+    banks: dict | None = None
+
+    def adapted(self) -> tuple:
+        """The part's products that low-rank adapters may stand beside (``parts.adapters.AdaptedProduct``)."""
+        return ()
+
+    def add_adapters(self, name: str, y: torch.Tensor, x: torch.Tensor, ctx: "StepContext") -> torch.Tensor:
+        """``y``, the product ``name`` of ``x``, with what the adapters of the step's requests add to it (in place)."""
+        if ctx.adapters is None or self.banks is None or name not in self.banks:
+            return y
+        return self.banks[name].add(y, x, ctx.adapters)
 
     def param(self, name: str, default: Any = None) -> Any:
         if name in self.spec.params:

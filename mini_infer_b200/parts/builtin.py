@@ -12,6 +12,7 @@ import math
 import torch
 
 from ..csrc import ops
+from .adapters import AdaptedProduct
 from .base import (
     Arrangement,
     BranchSum,
@@ -539,6 +540,11 @@ class GroupedQueryAttention(Mixer):
         self.qkv_proj = Linear(qkv)
         self.o_proj = Linear(_as_compute(tensors["o_proj.weight"], dtype).contiguous())
 
+    def adapted(self):
+        nq, nkv, d = self.nq, self.nkv, self.d
+        return (AdaptedProduct("qkv", ("q_proj.weight", "k_proj.weight", "v_proj.weight"), (nq * d, nkv * d, nkv * d), self.hidden),
+                AdaptedProduct("o", ("o_proj.weight",), (self.hidden,), nq * d))
+
     def takes_deferred_norm(self, n_rows, kind):
         return self.qkv_proj.fusable(n_rows, kind)
 
@@ -547,7 +553,7 @@ class GroupedQueryAttention(Mixer):
 
     def forward(self, x, ctx: StepContext, cache: LayerCache, position, into=None):
         nq, nkv, d = self.nq, self.nkv, self.d
-        qkv = self.qkv_proj(x)
+        qkv = self.add_adapters("qkv", self.qkv_proj(x), x, ctx)
         table = None
         if (position is not None and cache.k is not None
                 and ops.decode_rope_fusable(x.dtype, d, ctx.decode_only, ctx.n_requests)):
@@ -562,7 +568,9 @@ class GroupedQueryAttention(Mixer):
         out = torch.empty((ctx.n_tokens, nq * d), dtype=x.dtype, device=x.device)
         ops.attention(qkv, qkv.stride(0), out, cache, ctx, nq, nkv, d, self.scale, self.window or 0,
                       rope_table=table)
-        return self.o_proj(out) if into is None else self.o_proj.into_stream(out, into)
+        if into is not None:
+            return self.o_proj.into_stream(out, into)
+        return self.add_adapters("o", self.o_proj(out), out, ctx)
 
 
 # ----------------------------------------------------------------------------- feed-forward
@@ -602,6 +610,11 @@ class SwiGLU(FeedForward):
         self.gate_up_proj = Linear(gate_up)
         self.down_proj = Linear(_as_compute(tensors["down_proj.weight"], dtype).contiguous())
 
+    def adapted(self):
+        H, I = int(self.param("hidden_size")), int(self.param("intermediate_size"))
+        return (AdaptedProduct("gate_up", ("gate_proj.weight", "up_proj.weight"), (I, I), H, pairs=True),
+                AdaptedProduct("down", ("down_proj.weight",), (H,), I))
+
     def takes_deferred_norm(self, n_rows, kind):
         return self.gate_up_proj.fusable(n_rows, kind)
 
@@ -613,9 +626,14 @@ class SwiGLU(FeedForward):
             if x.kind != "rms":
                 raise ValueError(f"this product cannot finish a norm of kind {x.kind!r}")
             h = ops.linear_swiglu(x.x, self.gate_up_proj.weight, row_stats=x.stats, act=self.activation)
+        elif ctx.adapters is not None and self.banks is not None:      # the activation runs behind what the adapters add
+            y = self.add_adapters("gate_up", self.gate_up_proj(x), x, ctx)
+            h = ops.silu_mul(y, pairs=True) if self.activation == "silu" else ops.glu_mul_pairs(y, self.activation)
         else:
             h = ops.linear_swiglu(x, self.gate_up_proj.weight, act=self.activation, w_constant=True)
-        return self.down_proj(h) if into is None else self.down_proj.into_stream(h, into)
+        if into is not None:
+            return self.down_proj.into_stream(h, into)
+        return self.add_adapters("down", self.down_proj(h), h, ctx)
 
 
 class ClampedGLU(FeedForward):
@@ -784,13 +802,15 @@ class PreNormBlock(Arrangement):
         a, residual = self.mixer_norm.forward(x, residual)
         if isinstance(self.feed_forward, NoFeedForward):
             return self.mixer.forward(a, ctx, cache, self.position), residual
-        sink = self._sink(self.mixer, self.feed_forward_norm, self.feed_forward, residual, n)
+        # (with adapters a branch ends behind what they add to its last product, and a branch's first product reads a whole norm)
+        fused = ctx.adapters is None
+        sink = self._sink(self.mixer, self.feed_forward_norm, self.feed_forward, residual, n) if fused else None
         if sink is None:
             h = self.mixer.forward(a, ctx, cache, self.position)
         else:
             h = self.mixer.forward(a, ctx, cache, self.position, into=sink)
         b, residual = self.feed_forward_norm.forward(h, residual)
-        sink = self._sink(self.feed_forward, following[0], following[1], residual, n) if following else None
+        sink = self._sink(self.feed_forward, following[0], following[1], residual, n) if following and fused else None
         if sink is None:
             f = self.feed_forward.forward(b, ctx)
         else:

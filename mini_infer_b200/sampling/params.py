@@ -2,7 +2,15 @@
 
 Names, defaults and checks are the reference's (``engine/sampler.py:7-21``):
 ``temperature`` 0 means greedy, ``top_k`` 0 and ``top_p`` 1.0 switch the filters off.
-``seed`` is this engine's addition: the reference draws from torch's global generator,
+What follows ``seed`` is this engine's addition, and applies to the logits in this order before everything else:
+
+* ``repetition_penalty``: a token of the prompt or the answer has its logit divided by it (multiplied where negative); 1 is off;
+* ``frequency_penalty``, ``presence_penalty``: the logit of a token that the answer holds ``c > 0`` times loses
+  ``frequency_penalty * c + presence_penalty``; 0 is off;
+* ``logit_bias``: a number added to the logits of given tokens (minus infinity: never);
+* ``allowed_token_ids``: no other token is ever chosen.
+
+``seed`` is an addition too: the reference draws from torch's global generator,
 here every request has a seed of its own and token ``n`` of a request is drawn from
 ``(seed, n)`` alone, so results do not depend on what else is in the batch.
 """
@@ -10,6 +18,8 @@ here every request has a seed of its own and token ``n`` of a request is drawn f
 from __future__ import annotations
 
 import dataclasses
+import math
+from typing import Mapping, Sequence
 
 
 @dataclasses.dataclass(frozen=True)
@@ -18,6 +28,11 @@ class SamplingParams:
     top_k: int = 0
     top_p: float = 1.0
     seed: int | None = None
+    repetition_penalty: float = 1.0
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    logit_bias: Mapping[int, float] | None = None
+    allowed_token_ids: Sequence[int] | None = None
 
     def __post_init__(self) -> None:
         if self.temperature < 0:
@@ -28,7 +43,39 @@ class SamplingParams:
             raise ValueError(f"top_p must be in [0, 1], got {self.top_p}")
         if self.seed is not None and not 0 <= self.seed < 2 ** 64:
             raise ValueError(f"seed must fit 64 bits, got {self.seed}")
+        if not (self.repetition_penalty > 0 and math.isfinite(self.repetition_penalty)):
+            raise ValueError(f"repetition_penalty must be positive, got {self.repetition_penalty}")
+        for name in ("frequency_penalty", "presence_penalty"):
+            if not math.isfinite(getattr(self, name)):
+                raise ValueError(f"{name} must be a number, got {getattr(self, name)}")
+        if self.logit_bias is not None:
+            items = tuple((int(t), float(b)) for t, b in dict(self.logit_bias).items())
+            if any(t < 0 or math.isnan(b) or b == math.inf for t, b in items):
+                raise ValueError(f"logit_bias gives numbers (or minus infinity) to token ids, got {self.logit_bias}")
+            object.__setattr__(self, "logit_bias", items)       # hashable, and nobody's to change
+        if self.allowed_token_ids is not None:
+            ids = tuple(sorted({int(t) for t in self.allowed_token_ids}))
+            if not ids or ids[0] < 0:
+                raise ValueError("allowed_token_ids must name at least one token")
+            object.__setattr__(self, "allowed_token_ids", ids)
 
     @property
     def greedy(self) -> bool:
         return self.temperature == 0.0
+
+    @property
+    def penalised(self) -> bool:
+        """Whether the logits depend on the tokens so far."""
+        return self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0
+
+    @property
+    def adjusted(self) -> bool:
+        """Whether the logits are changed at all before a token is chosen."""
+        return self.penalised or bool(self.logit_bias) or self.allowed_token_ids is not None
+
+    def check_vocabulary(self, vocab_size: int) -> None:
+        for t, _ in self.logit_bias or ():
+            if t >= vocab_size:
+                raise ValueError(f"logit_bias names token {t} of {vocab_size}")
+        if self.allowed_token_ids is not None and self.allowed_token_ids[-1] >= vocab_size:
+            raise ValueError(f"allowed_token_ids names token {self.allowed_token_ids[-1]} of {vocab_size}")
