@@ -214,7 +214,7 @@ class Part:
 
     def add_adapters(self, name: str, y: torch.Tensor, x: torch.Tensor, ctx: "StepContext") -> torch.Tensor:
         """``y``, the product ``name`` of ``x``, with what the adapters of the step's requests add to it (in place)."""
-        if ctx.adapters is None or self.banks is None or name not in self.banks:
+        if self.banks is None or ctx.adapters is None or name not in self.banks:
             return y
         return self.banks[name].add(y, x, ctx.adapters)
 

@@ -626,7 +626,7 @@ class SwiGLU(FeedForward):
             if x.kind != "rms":
                 raise ValueError(f"this product cannot finish a norm of kind {x.kind!r}")
             h = ops.linear_swiglu(x.x, self.gate_up_proj.weight, row_stats=x.stats, act=self.activation)
-        elif ctx.adapters is not None and self.banks is not None:      # the activation runs behind what the adapters add
+        elif self.banks is not None and ctx.adapters is not None:      # the activation runs behind what the adapters add
             y = self.add_adapters("gate_up", self.gate_up_proj(x), x, ctx)
             h = ops.silu_mul(y, pairs=True) if self.activation == "silu" else ops.glu_mul_pairs(y, self.activation)
         else:
