@@ -12,7 +12,6 @@ MI_DEFINE_ERROR_API()
 MI_DEFINE_STATUS_API(mi_adapters_status)
 
 #define ADAPTER_MAX_PARTS 4
-#define ADAPTER_THREADS 256
 
 struct AdapterArgs {
   const void* x;
@@ -39,48 +38,6 @@ struct AdapterArgs {
   int max_items, tiles;           // of the plan; of 128 columns in a row
   int constant;                   // no kernel in flight writes A and B
 };
-
-// One warp per (row, part and rank).
-template <typename T>
-__global__ void __launch_bounds__(ADAPTER_THREADS) adapter_shrink_kernel(const AdapterArgs g) {
-  mi_pdl_enter();
-  const int PR = g.P * g.R, lane = threadIdx.x & 31;
-  const long long unit = (long long)blockIdx.x * (ADAPTER_THREADS / 32) + (threadIdx.x >> 5);
-  if (unit >= (long long)g.M * PR) return;
-  const int t = (int)(unit / PR), pr = (int)(unit % PR);
-  const int id = g.ids[t];
-  if (id < 0 || id >= g.n) return;
-  const int rank = g.ranks ? min(g.ranks[id], g.R) : g.R;
-  if (pr % g.R >= rank) return;
-  const T* x = (const T*)g.x + t * g.ldx;
-  const T* a = (const T*)g.a + ((size_t)id * PR + pr) * g.K;
-  float s = 0.f;
-  for (int k = lane; k < g.K; k += 32) s = fmaf(mi_to_float(x[k]), mi_to_float(a[k]), s);
-  s = mi_warp_sum(s);
-  if (lane == 0) g.h[(size_t)t * PR + pr] = s * (g.scale ? g.scale[id] : 1.f);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(ADAPTER_THREADS) adapter_expand_kernel(const AdapterArgs g) {
-  mi_pdl_enter();
-  const int t = blockIdx.y, c = blockIdx.x * ADAPTER_THREADS + threadIdx.x;
-  if (c >= g.N) return;
-  const int id = g.ids[t];
-  float s = mi_to_float(((const T*)g.y)[t * g.ldy + c]);
-  if (id >= 0 && id < g.n) {
-    const int rank = g.ranks ? min(g.ranks[id], g.R) : g.R;
-    int p = 0;
-    if (g.pairs) p = c & 1;
-    else
-      while (p + 1 < g.P && c >= g.ends[p]) ++p;
-    const float* h = g.h + ((size_t)t * g.P + p) * g.R;
-    const T* b = (const T*)g.b + ((size_t)id * g.N + c) * g.R;
-    float d = 0.f;
-    for (int r = 0; r < rank; ++r) d = fmaf(h[r], mi_to_float(b[r]), d);
-    s += d;
-  }
-  ((T*)g.out)[t * g.ldo + c] = mi_from_float<T>(s);
-}
 
 // ---------------------------------------------------------------------------------------------- tensor cores, bfloat16
 //
@@ -171,7 +128,7 @@ inline int count_chunks(const AdapterArgs& g, int size) {
 
 #define TILE_THREADS 256
 #define TILE_WARPS (TILE_THREADS / 32)
-#define FEW_MAX 128           // rows of a call whose items the blocks find by themselves
+#define FEW_MAX 256           // rows of a call whose items the blocks find by themselves
 #define FEW_ROWS 8            // rows of an item
 #define SUM_GROUP 64          // sums of the first product that a block makes
 #define MAX_ROWS 128          // rows of an item of a plan
@@ -476,6 +433,141 @@ __global__ void __launch_bounds__(TILE_THREADS, BLOCKS) adapter_add_kernel(const
       }
     }
   }
+}
+
+// ---- the same on CUDA cores: float32, and operands that are not in pieces of 16 bytes
+//
+// Four values from `k` on, zeros behind `n`.  VEC: they are one access (float32 rows of whole pieces).
+template <typename T, bool VEC>
+__device__ __forceinline__ float4 four_values(const T* row, int k, int n) {
+  if (k >= n) return make_float4(0.f, 0.f, 0.f, 0.f);
+  if (VEC && sizeof(T) == 4) return *reinterpret_cast<const float4*>(row + k);
+  float4 v;
+  v.x = mi_to_float(row[k]);
+  v.y = k + 1 < n ? mi_to_float(row[k + 1]) : 0.f;
+  v.z = k + 2 < n ? mi_to_float(row[k + 2]) : 0.f;
+  v.w = k + 3 < n ? mi_to_float(row[k + 3]) : 0.f;
+  return v;
+}
+
+// The first product: a warp makes four sums of an item's up to eight rows over a share of K, its lanes four values of k each; the 32
+// totals are shared out over the lanes while they are added up.
+#define PLAIN_SUMS 4
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(TILE_THREADS) adapter_sums_plain_kernel(const AdapterArgs g) {
+  mi_pdl_wait();
+  mi_pdl_launch_dependents();
+  __shared__ int rows[FEW_ROWS];
+  __shared__ __align__(16) int ids[FEW_MAX + TILE_WARPS];
+  __shared__ int found[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Item item = get_item(g, blockIdx.y, rows, ids, found);
+  const int rank = rank_of(g, item.id), PR = g.P * g.R, first = (blockIdx.z * TILE_WARPS + warp) * PLAIN_SUMS;
+  if (item.count == 0 || rank == 0 || first >= PR) return;
+  const int units = (g.K + 127) / 128;
+  const int u0 = (int)((long long)units * blockIdx.x / g.ks), u1 = (int)((long long)units * (blockIdx.x + 1) / g.ks);
+  const T* x[FEW_ROWS];
+#pragma unroll
+  for (int t = 0; t < FEW_ROWS; ++t) x[t] = (const T*)g.x + (long long)rows[t < item.count ? t : 0] * g.ldx;
+  const T* a = (const T*)g.a + ((size_t)item.id * PR + first) * g.K;
+  float acc[PLAIN_SUMS * FEW_ROWS];
+#pragma unroll
+  for (int i = 0; i < PLAIN_SUMS * FEW_ROWS; ++i) acc[i] = 0.f;
+  for (int u = u0; u < u1; ++u) {
+    const int k = u * 128 + lane * 4;
+    float4 av[PLAIN_SUMS];
+#pragma unroll
+    for (int j = 0; j < PLAIN_SUMS; ++j)
+      av[j] = first + j < PR && (first + j) % g.R < rank ? four_values<T, VEC>(a + (size_t)j * g.K, k, g.K) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int t = 0; t < FEW_ROWS; ++t) {
+      if (t >= item.count) break;
+      const float4 xv = four_values<T, VEC>(x[t], k, g.K);
+#pragma unroll
+      for (int j = 0; j < PLAIN_SUMS; ++j) {
+        float& s = acc[j * FEW_ROWS + t];
+        s = fmaf(xv.x, av[j].x, fmaf(xv.y, av[j].y, fmaf(xv.z, av[j].z, fmaf(xv.w, av[j].w, s))));
+      }
+    }
+  }
+  // lane l ends with the total of acc[l]
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float give = upper ? acc[i] : acc[i + o], keep = upper ? acc[i + o] : acc[i];
+      acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  const int sum = first + lane / FEW_ROWS, tok = lane % FEW_ROWS;
+  if (sum < PR && tok < item.count) g.h[((size_t)blockIdx.x * g.M + rows[tok]) * PR + sum] = acc[0];
+}
+
+// The second product and the sum with y: a thread has a column and the item's rows.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(TILE_THREADS) adapter_add_plain_kernel(const AdapterArgs g) {
+  extern __shared__ __align__(16) float plain_h[];            // [parts of the block][R up to 4s][FEW_ROWS]
+  __shared__ int rows[FEW_ROWS];
+  __shared__ __align__(16) int ids[FEW_MAX + TILE_WARPS];
+  __shared__ int found[2];
+  mi_pdl_launch_dependents();
+  const Item item = get_item(g, blockIdx.y, rows, ids, found);
+  const int rank = rank_of(g, item.id), R = g.R, r4 = (R + 3) & ~3, np = g.pairs ? 2 : 1;
+  const T* y = (const T*)g.y;
+  T* out = (T*)g.out;
+  int part, c_first, c_end;
+  const bool there = find_chunk(g, blockIdx.x, TILE_THREADS, part, c_first, c_end) && item.count > 0 && (rank > 0 || out != y);
+  mi_pdl_wait();
+  if (!there) return;
+  const int c = c_first + threadIdx.x;
+  float acc[FEW_ROWS];
+#pragma unroll
+  for (int t = 0; t < FEW_ROWS; ++t) acc[t] = c < c_end && t < item.count ? mi_to_float(y[rows[t] * g.ldy + c]) : 0.f;
+  if (rank > 0) {
+    const float scale = g.scale ? g.scale[item.id] : 1.f;
+    for (int i = threadIdx.x; i < np * r4 * FEW_ROWS; i += TILE_THREADS) {
+      const int t = i % FEW_ROWS, r = i / FEW_ROWS % r4, p = i / FEW_ROWS / r4;
+      float s = 0.f;
+      if (t < item.count && r < rank)
+        for (int k = 0; k < g.ks; ++k) s += __ldcg(g.h + ((size_t)k * g.M + rows[t]) * g.P * R + (part + p) * R + r);
+      plain_h[i] = s * scale;
+    }
+    __syncthreads();
+    if (c < c_end) {
+      const T* b = (const T*)g.b + ((size_t)item.id * g.N + c) * R;
+      const float* h = plain_h + (g.pairs ? c & 1 : 0) * r4 * FEW_ROWS;
+      float d[FEW_ROWS];
+#pragma unroll
+      for (int t = 0; t < FEW_ROWS; ++t) d[t] = 0.f;
+      for (int r = 0; r < rank; r += 4) {
+        // (a whole piece is loaded, and what lies behind the rank left out)
+        const float4 v = VEC ? four_values<T, VEC>(b, r, R) : four_values<T, VEC>(b, r, rank);
+        const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (r + q >= rank) break;
+          const float4 h0 = *reinterpret_cast<const float4*>(h + (r + q) * FEW_ROWS), h1 = *reinterpret_cast<const float4*>(h + (r + q) * FEW_ROWS + 4);
+          d[0] = fmaf(w[q], h0.x, d[0]);
+          d[1] = fmaf(w[q], h0.y, d[1]);
+          d[2] = fmaf(w[q], h0.z, d[2]);
+          d[3] = fmaf(w[q], h0.w, d[3]);
+          d[4] = fmaf(w[q], h1.x, d[4]);
+          d[5] = fmaf(w[q], h1.y, d[5]);
+          d[6] = fmaf(w[q], h1.z, d[6]);
+          d[7] = fmaf(w[q], h1.w, d[7]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < FEW_ROWS; ++t) acc[t] += d[t];
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < FEW_ROWS; ++t)
+    if (c < c_end && t < item.count) {
+      if (rank > 0) out[rows[t] * g.ldo + c] = mi_from_float<T>(acc[t]);
+      else out[rows[t] * g.ldo + c] = y[rows[t] * g.ldy + c];
+    }
 }
 
 // ---- many rows: both products on tcgen05, items of up to 128 rows
@@ -977,7 +1069,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
 // ---- the plan: rows in the order of their adapters, and items of up to 64 of them
 
 #define PLAN_THREADS 1024
-#define PLAN_MAX_ADAPTERS 4096
+#define PLAN_MAX_ADAPTERS 2048
 
 __global__ void __launch_bounds__(PLAN_THREADS)
 adapter_plan_kernel(const int* ids, int M, int n, int* order, int4* items, int max_items) {
@@ -1111,6 +1203,19 @@ static cudaError_t launch_few(const AdapterArgs& g, int max_items, cudaStream_t 
   return run(adapter_add_kernel<0, false, 2>, adapter_add_kernel<0, false, 3>, allowed[6]);
 }
 
+template <typename T, bool VEC>
+static cudaError_t launch_plain(const AdapterArgs& g, int max_items, cudaStream_t stream) {
+  static size_t allowed[64];
+  const int groups = (g.P * g.R + TILE_WARPS * PLAIN_SUMS - 1) / (TILE_WARPS * PLAIN_SUMS);
+  cudaError_t e = cudaSuccess;
+  if (g.n > 0 && g.R > 0) e = MI_LAUNCH((adapter_sums_plain_kernel<T, VEC>), dim3(g.ks, max_items, groups), TILE_THREADS, 0, stream, g);
+  if (e != cudaSuccess) return e;
+  const size_t bytes = (size_t)(g.pairs ? 2 : 1) * ((g.R + 3) & ~3) * FEW_ROWS * 4;
+  e = allow_smem(adapter_add_plain_kernel<T, VEC>, bytes, allowed);
+  if (e != cudaSuccess) return e;
+  return MI_LAUNCH((adapter_add_plain_kernel<T, VEC>), dim3(count_chunks(g, TILE_THREADS), max_items), TILE_THREADS, bytes, stream, g);
+}
+
 static int add_tc_stages(int R, int pairs) {
   const int left = 225 * 1024 - (pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM;
   const int n = left / add_stage_bytes(R);
@@ -1156,10 +1261,17 @@ struct Route {
 static Route route_of(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b, const void* out,
                       long long ldo, int M, int N, int K, int n, int P, int R, const int* ends, int pairs, int dtype) {
   Route r = {BY_ELEMENTS, 0, 1, (long long)M * P * R, 0};
+  r.items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : plan_items(M, n) * SUB_ITEMS;
   // The tensor-core kernels take rows of x, A and B in pieces of 16 bytes.
   if (dtype != MI_DTYPE_BF16 || n <= 0 || R <= 0 || R > 256 || K <= 0 || R % 8 || K % 8 || !mi_aligned(a, 16) ||
-      !mi_aligned(b, 16) || !mi_aligned(x, 16) || (M > 1 && ldx % 8))
+      !mi_aligned(b, 16) || !mi_aligned(x, 16) || (M > 1 && ldx % 8)) {
+    const int groups = (P * R + TILE_WARPS * PLAIN_SUMS - 1) / (TILE_WARPS * PLAIN_SUMS), units = (K + 127) / 128;
+    r.ks = 4 * 148 / (r.items * groups + 1);
+    if (r.ks > units / 4) r.ks = units / 4;
+    r.ks = r.ks < 1 ? 1 : r.ks > 16 ? 16 : r.ks;
+    r.floats *= r.ks;
     return r;
+  }
   bool whole = N % 8 == 0 && mi_aligned(y, 16) && mi_aligned(out, 16) && (M == 1 || (ldy % 8 == 0 && ldo % 8 == 0));
   for (int p = 0; p + 1 < P && !pairs; ++p) whole = whole && ends[p] % 8 == 0;
   if (M > FEW_MAX && whole && R <= 128 && add_tc_stages(R, pairs) >= 1) {
@@ -1173,7 +1285,6 @@ static Route route_of(const void* y, long long ldy, const void* x, long long ldx
     r.held_floats = (long long)M * P * held_sums(R) / 2;
   } else {
     r.way = BY_FEW;
-    r.items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : plan_items(M, n) * SUB_ITEMS;
     const int units = (K + 31) / 32, groups = (P * R + SUM_GROUP - 1) / SUM_GROUP;
     r.ks = 2 * 148 / (r.items * groups);
     if (r.ks > units / TILE_WARPS) r.ks = units / TILE_WARPS;
@@ -1232,13 +1343,15 @@ extern "C" int mi_adapter_add(const AdapterCall* call, float* h, cudaStream_t st
   g.pairs = pairs;
   g.constant = c.constant != 0;
   const Route r = route_of(c);
+  if (r.items > 65535) MI_REFUSE("adapter_add: %d rows with %d adapters", M, n);
+  if (M > FEW_MAX && !(g.order && g.items)) MI_REFUSE("adapter_add: a plan of %d rows without their order", M);
+  if (M <= FEW_MAX) g.items = nullptr;
+  g.ks = r.ks;
   if (r.way != BY_ELEMENTS) {
-    if (r.items > 65535) MI_REFUSE("adapter_add: %d rows with %d adapters", M, n);
     g.max_items = r.way == BY_MANY ? r.items : 0;
     g.tiles = count_chunks(g, ADD_COLS);
     if ((long long)r.items * g.tiles > 0x7fffffffLL) MI_REFUSE("adapter_add: %d rows of %d columns", M, N);
     if (M > FEW_MAX && !(g.order && g.items)) MI_REFUSE("adapter_add: a plan of %d rows without their order", M);
-    g.ks = r.ks;
     g.held = (bf16*)(h + r.floats);
     bool starts4 = true;
     for (int p = 0; p + 1 < P && !pairs; ++p) starts4 = starts4 && g.ends[p] % 4 == 0;
@@ -1250,17 +1363,11 @@ extern "C" int mi_adapter_add(const AdapterCall* call, float* h, cudaStream_t st
     if (e != cudaSuccess) return refused_by_cuda(e);
     MI_RETURN_LAUNCH_STATUS();
   }
-  if (M > 65535) MI_REFUSE("adapter_add: %d rows, at most 65535 of operands that are not in pieces of 16 bytes", M);
-  const long long units = (long long)M * P * R, per = ADAPTER_THREADS / 32;
-  if ((units + per - 1) / per > 0x7fffffffLL) MI_REFUSE("adapter_add: %lld sums of the first product", units);
-  const unsigned blocks = n > 0 ? (unsigned)((units + per - 1) / per) : 0u;
-  const dim3 grid((N + ADAPTER_THREADS - 1) / ADAPTER_THREADS, M);
-  if (dtype == MI_DTYPE_F32) {
-    if (blocks) MI_LAUNCH((adapter_shrink_kernel<float>), blocks, ADAPTER_THREADS, 0, stream, g);
-    MI_LAUNCH((adapter_expand_kernel<float>), grid, ADAPTER_THREADS, 0, stream, g);
-  } else {
-    if (blocks) MI_LAUNCH((adapter_shrink_kernel<bf16>), blocks, ADAPTER_THREADS, 0, stream, g);
-    MI_LAUNCH((adapter_expand_kernel<bf16>), grid, ADAPTER_THREADS, 0, stream, g);
-  }
+  if (R > 3000) MI_REFUSE("adapter_add: rank %d, at most 3000", R);
+  const cudaError_t e = dtype != MI_DTYPE_F32 ? launch_plain<bf16, false>(g, r.items, stream)
+                        : K % 4 || R % 4 || !mi_aligned(g.x, 16) || !mi_aligned(g.a, 16) || !mi_aligned(g.b, 16) || (M > 1 && g.ldx % 4)
+                            ? launch_plain<float, false>(g, r.items, stream)
+                            : launch_plain<float, true>(g, r.items, stream);
+  if (e != cudaSuccess) return refused_by_cuda(e);
   MI_RETURN_LAUNCH_STATUS();
 }

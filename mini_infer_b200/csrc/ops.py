@@ -3017,7 +3017,7 @@ class AdapterPlan:
         self.order = self.items = None
 
 
-ADAPTER_FEW_ROWS = 128       # rows whose adapters the kernels look through by themselves
+ADAPTER_FEW_ROWS = 256       # rows whose adapters the kernels look through by themselves
 
 
 def adapter_plan(ids: torch.Tensor, adapters: int) -> AdapterPlan:
