@@ -454,7 +454,7 @@ __device__ __forceinline__ float4 four_values(const T* row, int k, int n) {
 // totals are shared out over the lanes while they are added up.
 #define PLAIN_SUMS 4
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(TILE_THREADS) adapter_sums_plain_kernel(const AdapterArgs g) {
+__global__ void __launch_bounds__(TILE_THREADS, 3) adapter_sums_plain_kernel(const AdapterArgs g) {
   mi_pdl_wait();
   mi_pdl_launch_dependents();
   __shared__ int rows[FEW_ROWS];
@@ -478,16 +478,19 @@ __global__ void __launch_bounds__(TILE_THREADS) adapter_sums_plain_kernel(const 
     float4 av[PLAIN_SUMS];
 #pragma unroll
     for (int j = 0; j < PLAIN_SUMS; ++j)
-      av[j] = first + j < PR && (first + j) % g.R < rank ? four_values<T, VEC>(a + (size_t)j * g.K, k, g.K) : make_float4(0.f, 0.f, 0.f, 0.f);
+      av[j] = four_values<T, VEC>(a + (size_t)j * g.K, first + j < PR && (first + j) % g.R < rank ? k : g.K, g.K);
 #pragma unroll
-    for (int t = 0; t < FEW_ROWS; ++t) {
-      if (t >= item.count) break;
-      const float4 xv = four_values<T, VEC>(x[t], k, g.K);
+    for (int t0 = 0; t0 < FEW_ROWS; t0 += 4) {                // four rows under way at once
+      float4 xv[4];
 #pragma unroll
-      for (int j = 0; j < PLAIN_SUMS; ++j) {
-        float& s = acc[j * FEW_ROWS + t];
-        s = fmaf(xv.x, av[j].x, fmaf(xv.y, av[j].y, fmaf(xv.z, av[j].z, fmaf(xv.w, av[j].w, s))));
-      }
+      for (int t = 0; t < 4; ++t) xv[t] = four_values<T, VEC>(x[t0 + t], t0 + t < item.count ? k : g.K, g.K);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < PLAIN_SUMS; ++j) {
+          float& s = acc[j * FEW_ROWS + t0 + t];
+          s = fmaf(xv[t].x, av[j].x, fmaf(xv[t].y, av[j].y, fmaf(xv[t].z, av[j].z, fmaf(xv[t].w, av[j].w, s))));
+        }
     }
   }
   // lane l ends with the total of acc[l]
@@ -517,57 +520,60 @@ __global__ void __launch_bounds__(TILE_THREADS) adapter_add_plain_kernel(const A
   const T* y = (const T*)g.y;
   T* out = (T*)g.out;
   int part, c_first, c_end;
-  const bool there = find_chunk(g, blockIdx.x, TILE_THREADS, part, c_first, c_end) && item.count > 0 && (rank > 0 || out != y);
+  const bool there = find_chunk(g, blockIdx.x, g.span, part, c_first, c_end) && item.count > 0 && (rank > 0 || out != y);
   mi_pdl_wait();
   if (!there) return;
-  const int c = c_first + threadIdx.x;
-  float acc[FEW_ROWS];
-#pragma unroll
-  for (int t = 0; t < FEW_ROWS; ++t) acc[t] = c < c_end && t < item.count ? mi_to_float(y[rows[t] * g.ldy + c]) : 0.f;
+  c_end = min(c_end, c_first + g.span);
   if (rank > 0) {
     const float scale = g.scale ? g.scale[item.id] : 1.f;
     for (int i = threadIdx.x; i < np * r4 * FEW_ROWS; i += TILE_THREADS) {
       const int t = i % FEW_ROWS, r = i / FEW_ROWS % r4, p = i / FEW_ROWS / r4;
       float s = 0.f;
-      if (t < item.count && r < rank)
-        for (int k = 0; k < g.ks; ++k) s += __ldcg(g.h + ((size_t)k * g.M + rows[t]) * g.P * R + (part + p) * R + r);
+      if (t < item.count && r < rank) {
+        const float* from = g.h + (size_t)rows[t] * g.P * R + (part + p) * R + r;
+#pragma unroll 8
+        for (int k = 0; k < g.ks; ++k) s += __ldcg(from + (size_t)k * g.M * g.P * R);
+      }
       plain_h[i] = s * scale;
     }
     __syncthreads();
-    if (c < c_end) {
-      const T* b = (const T*)g.b + ((size_t)item.id * g.N + c) * R;
-      const float* h = plain_h + (g.pairs ? c & 1 : 0) * r4 * FEW_ROWS;
-      float d[FEW_ROWS];
-#pragma unroll
-      for (int t = 0; t < FEW_ROWS; ++t) d[t] = 0.f;
-      for (int r = 0; r < rank; r += 4) {
-        // (a whole piece is loaded, and what lies behind the rank left out)
-        const float4 v = VEC ? four_values<T, VEC>(b, r, R) : four_values<T, VEC>(b, r, rank);
-        const float w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (r + q >= rank) break;
-          const float4 h0 = *reinterpret_cast<const float4*>(h + (r + q) * FEW_ROWS), h1 = *reinterpret_cast<const float4*>(h + (r + q) * FEW_ROWS + 4);
-          d[0] = fmaf(w[q], h0.x, d[0]);
-          d[1] = fmaf(w[q], h0.y, d[1]);
-          d[2] = fmaf(w[q], h0.z, d[2]);
-          d[3] = fmaf(w[q], h0.w, d[3]);
-          d[4] = fmaf(w[q], h1.x, d[4]);
-          d[5] = fmaf(w[q], h1.y, d[5]);
-          d[6] = fmaf(w[q], h1.z, d[6]);
-          d[7] = fmaf(w[q], h1.w, d[7]);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < FEW_ROWS; ++t) acc[t] += d[t];
-    }
   }
-#pragma unroll
-  for (int t = 0; t < FEW_ROWS; ++t)
-    if (c < c_end && t < item.count) {
-      if (rank > 0) out[rows[t] * g.ldo + c] = mi_from_float<T>(acc[t]);
-      else out[rows[t] * g.ldo + c] = y[rows[t] * g.ldy + c];
+  for (int c = c_first + threadIdx.x; c < c_end; c += TILE_THREADS) {
+    if (rank == 0) {
+      for (int t = 0; t < item.count; ++t) out[rows[t] * g.ldo + c] = y[rows[t] * g.ldy + c];
+      continue;
     }
+    float acc[FEW_ROWS], d[FEW_ROWS];
+#pragma unroll
+    for (int t = 0; t < FEW_ROWS; ++t) {
+      acc[t] = t < item.count ? mi_to_float(y[rows[t] * g.ldy + c]) : 0.f;
+      d[t] = 0.f;
+    }
+    const T* b = (const T*)g.b + ((size_t)item.id * g.N + c) * R;
+    const float* h = plain_h + (g.pairs ? c & 1 : 0) * r4 * FEW_ROWS;
+#pragma unroll 2
+    for (int r = 0; r < rank; r += 4) {
+      // (a whole piece is loaded, and what lies behind the rank left out)
+      const float4 v = VEC ? four_values<T, VEC>(b, r, R) : four_values<T, VEC>(b, r, rank);
+      const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (r + q >= rank) break;
+        const float4 h0 = *reinterpret_cast<const float4*>(h + (r + q) * FEW_ROWS), h1 = *reinterpret_cast<const float4*>(h + (r + q) * FEW_ROWS + 4);
+        d[0] = fmaf(w[q], h0.x, d[0]);
+        d[1] = fmaf(w[q], h0.y, d[1]);
+        d[2] = fmaf(w[q], h0.z, d[2]);
+        d[3] = fmaf(w[q], h0.w, d[3]);
+        d[4] = fmaf(w[q], h1.x, d[4]);
+        d[5] = fmaf(w[q], h1.y, d[5]);
+        d[6] = fmaf(w[q], h1.z, d[6]);
+        d[7] = fmaf(w[q], h1.w, d[7]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < FEW_ROWS; ++t)
+      if (t < item.count) out[rows[t] * g.ldo + c] = mi_from_float<T>(acc[t] + d[t]);
+  }
 }
 
 // ---- many rows: both products on tcgen05, items of up to 128 rows
@@ -852,7 +858,8 @@ template <int STAGES>
 __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const AdapterArgs g) {
   extern __shared__ unsigned char tc_smem[];
   __shared__ AddBlock s;
-  mi_pdl_wait();
+  // (The kernel in front, which holds the sums, started this one once the first product's had ended: everything that was before that
+  // is there, tensor memory is nobody's any more, and the copy warps alone wait, before they take the sums.)
   const uint32_t base = (smem_u32(tc_smem) + 1023) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = g.R;
   const int np = g.pairs ? 2 : 1, rp = padded_rank(R), ha = sums_atoms(R), ba = b_atoms(R);
@@ -891,7 +898,10 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
     const int h_shift = b_shift + with_rests(R), hq = ct & ((1 << h_shift) - 1), h_row = ct >> h_shift, h_step = ADD_COPY_THREADS >> h_shift;
     const int yq = ct & 15, yr = ct >> 4;                     // piece `yq` of every 8th row
     constexpr int YN = TC_ROWS * 16 / ADD_COPY_THREADS;
-    long long y_off[YN];
+    const uint32_t y_row = ba * TC_ATOM + yr * 256, y_place[2] = {y_row + ((yq ^ yr) << 4), y_row + ((yq ^ (yr + 8)) << 4)};
+    const uint32_t b_place = bq / 8 * TC_ATOM + b_col * 128 + (((bq & 7) ^ (b_col & 7)) << 4);
+    const int b_stride = (g.pairs ? 2 : 1) * b_step * R;      // elements between a thread's columns
+    const bf16* y_from[YN];
     uint32_t y_in = 0;
     int items = 0, asked = 0, told = 0, last_part = -1;                       // begun so far, of those with an adapter; tiles asked for, and said to be there
     const auto tell = [&](int upto) {
@@ -907,7 +917,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         for (int i = 0; i < YN; ++i) {
           const int row = yr + i * (TC_ROWS / YN);
           if (row < item.z) {
-            y_off[i] = __ldcg(g.order + item.y + row) * g.ldy + yq * 8;
+            y_from[i] = y + __ldcg(g.order + item.y + row) * g.ldy + yq * 8;
             y_in |= 1u << i;
           }
         }
@@ -921,7 +931,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         copies_wait<0>();
         tell(j);
         if (items > 0 && !mbar_wait(&s.h_free, (items - 1) & 1, &s.give_up)) return false;
-        ++items;
+        if (items++ == 0) mi_pdl_wait();
         if (hq < h_pieces)
           for (int row = h_row; row < item.z; row += h_step) {
             const bf16* from = g.held + (size_t)__ldcg(g.order + item.y + row) * g.P * hp + hq * 8;
@@ -933,17 +943,30 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         // rows of B: the tile's columns, of pairs the first ones and then the second ones
         const int there = 2 * max(0, min(8, rank - bq * 8));
         const bf16* b = (const bf16*)g.b + (size_t)item.x * g.N * R + bq * 8;
-        for (int col = b_col; col < ADD_COLS; col += b_step) {
-          const int from = c + (g.pairs ? (col & 63) * 2 + (col >> 6) : col);
-          const bool in = there && from < c_end;
-          copy_piece(to + bq / 8 * TC_ATOM + col * 128 + (((bq & 7) ^ (col & 7)) << 4), in ? b + (size_t)from * R : (const bf16*)g.b, in ? there : 0);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int first = g.pairs ? c + 2 * b_col + half : c + half * 64 + b_col;
+          const bf16* from = b + (size_t)first * R;
+          uint32_t at = to + b_place + half * (TC_ATOM / 2);
+          if (c + ADD_COLS <= c_end && there == 16) {
+            for (int col = b_col; col < 64; col += b_step, from += b_stride, at += b_step * 128) copy_piece(at, from, 16);
+          } else {
+            int column = first;
+            for (int col = b_col; col < 64; col += b_step, from += b_stride, at += b_step * 128, column += (g.pairs ? 2 : 1) * b_step) {
+              const bool in = there && column < c_end;
+              copy_piece(at, in ? from : (const bf16*)g.b, in ? there : 0);
+            }
+          }
         }
       }
       if (c + yq * 8 < c_end) {
+        if (y_in == (1u << YN) - 1u) {
 #pragma unroll
-        for (int i = 0; i < YN; ++i) {
-          const int row = yr + i * (TC_ROWS / YN);
-          if ((y_in >> i) & 1u) copy_piece(to + ba * TC_ATOM + row * 256 + ((yq ^ (row & 15)) << 4), y + y_off[i] + c, 16);
+          for (int i = 0; i < YN; ++i) copy_piece(to + y_place[i & 1] + i * 2048, y_from[i] + c, 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < YN; ++i)
+            if ((y_in >> i) & 1u) copy_piece(to + y_place[i & 1] + i * 2048, y_from[i] + c, 16);
         }
       }
       copies_commit();
@@ -954,6 +977,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
     });
     copies_wait<0>();
     tell(asked);
+    mi_pdl_wait();
   } else if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) {
     // ---- products
     if (lane == 0) {
@@ -1213,7 +1237,7 @@ static cudaError_t launch_plain(const AdapterArgs& g, int max_items, cudaStream_
   const size_t bytes = (size_t)(g.pairs ? 2 : 1) * ((g.R + 3) & ~3) * FEW_ROWS * 4;
   e = allow_smem(adapter_add_plain_kernel<T, VEC>, bytes, allowed);
   if (e != cudaSuccess) return e;
-  return MI_LAUNCH((adapter_add_plain_kernel<T, VEC>), dim3(count_chunks(g, TILE_THREADS), max_items), TILE_THREADS, bytes, stream, g);
+  return MI_LAUNCH((adapter_add_plain_kernel<T, VEC>), dim3(count_chunks(g, g.span), max_items), TILE_THREADS, bytes, stream, g);
 }
 
 static int add_tc_stages(int R, int pairs) {
@@ -1266,8 +1290,9 @@ static Route route_of(const void* y, long long ldy, const void* x, long long ldx
   if (dtype != MI_DTYPE_BF16 || n <= 0 || R <= 0 || R > 256 || K <= 0 || R % 8 || K % 8 || !mi_aligned(a, 16) ||
       !mi_aligned(b, 16) || !mi_aligned(x, 16) || (M > 1 && ldx % 8)) {
     const int groups = (P * R + TILE_WARPS * PLAIN_SUMS - 1) / (TILE_WARPS * PLAIN_SUMS), units = (K + 127) / 128;
-    r.ks = 4 * 148 / (r.items * groups + 1);
-    if (r.ks > units / 4) r.ks = units / 4;
+    const int likely = M <= FEW_MAX ? r.items : M / FEW_ROWS + n;      // (a plan has room for more items than there are)
+    r.ks = 12 * 148 / (likely * groups + 1);
+    if (r.ks > units) r.ks = units;
     r.ks = r.ks < 1 ? 1 : r.ks > 16 ? 16 : r.ks;
     r.floats *= r.ks;
     return r;
@@ -1363,6 +1388,8 @@ extern "C" int mi_adapter_add(const AdapterCall* call, float* h, cudaStream_t st
     if (e != cudaSuccess) return refused_by_cuda(e);
     MI_RETURN_LAUNCH_STATUS();
   }
+  g.span = 2048;
+  while (g.span > 256 && (long long)(M <= FEW_MAX ? r.items : M / FEW_ROWS + n) * count_chunks(g, g.span) < 6 * 148) g.span /= 2;
   if (R > 3000) MI_REFUSE("adapter_add: rank %d, at most 3000", R);
   const cudaError_t e = dtype != MI_DTYPE_F32 ? launch_plain<bf16, false>(g, r.items, stream)
                         : K % 4 || R % 4 || !mi_aligned(g.x, 16) || !mi_aligned(g.a, 16) || !mi_aligned(g.b, 16) || (M > 1 && g.ldx % 4)
