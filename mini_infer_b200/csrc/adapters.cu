@@ -585,8 +585,7 @@ __global__ void __launch_bounds__(TILE_THREADS) adapter_add_plain_kernel(const A
 #define TC_THREADS 256
 #define TC_ROWS 128
 #define TC_ATOM (TC_ROWS * 128)      // bytes of 128 rows of 64 k
-#define SUMS_STAGES 3
-#define SUMS_STAGE_BYTES (2 * TC_ATOM)
+#define SUMS_MAX_STAGES 4
 #define ADD_COLS 128                 // columns of a tile of the result
 #define ADD_MAX_STAGES 4
 
@@ -648,8 +647,11 @@ __device__ __forceinline__ void tc_free(uint32_t at, int columns) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(at), "r"(columns) : "memory");
 }
 
+// A stage of the first product: 64 k of 128 rows and of a block's sums
+__host__ __device__ inline uint32_t sums_stage_bytes(int PR) { return TC_ATOM + (uint32_t)((PR < 128 ? PR + 15 : 128 + 15) / 16 * 16) * 128; }
+
 struct TcBlock {
-  uint64_t bars[SUMS_STAGES];                                                           // the products that read a stage have ended
+  uint64_t bars[SUMS_MAX_STAGES];        // the products that read a stage have ended
   uint32_t tmem;
   int give_up;
   int rows[TC_ROWS];
@@ -679,6 +681,7 @@ __device__ __forceinline__ bool tc_wait(TcBlock& s, int stage, uint32_t parity) 
 }
 
 // The first product: up to 128 sums of an item over a share of K, through a ring of stages of 64 k.
+template <int STAGES>
 __global__ void __launch_bounds__(TC_THREADS) adapter_sums_tc_kernel(const AdapterArgs g) {
   mi_pdl_wait();
   extern __shared__ unsigned char tc_smem[];
@@ -692,6 +695,7 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_sums_tc_kernel(const Adapt
   const int PR = g.P * g.R, m0 = blockIdx.z * 128, sums = min(128, PR - m0), n = (sums + 15) & ~15;
   const int blocks = (g.K + 63) / 64;
   const int u0 = (int)((long long)blocks * blockIdx.x / g.ks), u1 = (int)((long long)blocks * (blockIdx.x + 1) / g.ks);
+  const uint32_t stage_bytes = sums_stage_bytes(PR);
 
   // piece `tid % 8` of four rows of x and of A, 32 rows apart
   const int piece = tid & 7, r0 = tid >> 3;
@@ -705,7 +709,7 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_sums_tc_kernel(const Adapt
   }
   const auto load = [&](int u) {
     if (u < u1) {
-      const uint32_t to = base + (u - u0) % SUMS_STAGES * SUMS_STAGE_BYTES + place;
+      const uint32_t to = base + (u - u0) % STAGES * stage_bytes + place;
       const bool in = u * 64 + piece * 8 < g.K;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -717,31 +721,31 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_sums_tc_kernel(const Adapt
     copies_commit();
   };
 #pragma unroll
-  for (int i = 0; i < SUMS_STAGES - 1; ++i) load(u0 + i);
+  for (int i = 0; i < STAGES - 1; ++i) load(u0 + i);
   const uint32_t desc = product_desc(n);
   bool ok = true;
   for (int u = u0; u < u1; ++u) {
-    copies_wait<SUMS_STAGES - 2>();
+    copies_wait<STAGES - 2>();
     smem_for_tensor_cores();
-    __syncthreads();
-    const int i = u - u0, stage = i % SUMS_STAGES;
+    if (__syncthreads_or(*(volatile int*)&s.give_up)) {       // (a wait of the last round ran out)
+      ok = false;
+      break;
+    }
+    const int i = u - u0, stage = i % STAGES;
     if (tid == 0) {
       tc_fence_after();
-      const uint32_t at = base + stage * SUMS_STAGE_BYTES;
+      const uint32_t at = base + stage * stage_bytes;
 #pragma unroll
       for (int k = 0; k < 4; ++k) tc_mma(s.tmem, operand_desc(at + k * 32), operand_desc(at + TC_ATOM + k * 32), desc, i > 0 || k > 0);
       tc_commit(&s.bars[stage]);
     }
     // the stage of the products before these is free once they have ended
-    if (i > 0 && !tc_wait(s, (i - 1) % SUMS_STAGES, ((i - 1) / SUMS_STAGES) & 1)) {
-      ok = false;
-      break;
-    }
-    load(u + SUMS_STAGES - 1);
+    if (i > 0) mbar_wait(&s.bars[(i - 1) % STAGES], ((i - 1) / STAGES) & 1, &s.give_up);
+    load(u + STAGES - 1);
   }
   copies_wait<0>();
   const int last = u1 - u0 - 1;
-  if (ok) ok = tc_wait(s, last % SUMS_STAGES, (last / SUMS_STAGES) & 1);
+  if (ok) ok = tc_wait(s, last % STAGES, (last / STAGES) & 1);
   if (ok) {
     tc_fence_after();
     const int row = (warp & 3) * 32 + lane;
@@ -925,20 +929,6 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
       if (j >= STAGES && !mbar_wait(&s.empty[stage], (j / STAGES - 1) & 1, &s.give_up)) return false;
       int part, c, c_end;
       find_chunk(g, chunk, ADD_COLS, part, c, c_end);
-      if ((begins || part != last_part) && rank > 0) {
-        last_part = part;
-        // the last item's products have to end first, and for that to be told of all their tiles
-        copies_wait<0>();
-        tell(j);
-        if (items > 0 && !mbar_wait(&s.h_free, (items - 1) & 1, &s.give_up)) return false;
-        if (items++ == 0) mi_pdl_wait();
-        if (hq < h_pieces)
-          for (int row = h_row; row < item.z; row += h_step) {
-            const bf16* from = g.held + (size_t)__ldcg(g.order + item.y + row) * g.P * hp + hq * 8;
-            for (int p = 0; p < np; ++p)
-              copy_piece(h_at + (p * ha + hq / 8) * TC_ATOM + row * 128 + (((hq & 7) ^ (row & 7)) << 4), from + (size_t)(part + p) * hp, 16);
-          }
-      }
       if (rank > 0 && bq < b_pieces) {
         // rows of B: the tile's columns, of pairs the first ones and then the second ones
         const int there = 2 * max(0, min(8, rank - bq * 8));
@@ -970,6 +960,21 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         }
       }
       copies_commit();
+      if ((begins || part != last_part) && rank > 0) {
+        last_part = part;
+        // the last item's products have to end first, and for that to be told of all their tiles
+        copies_wait<1>();
+        tell(j);
+        if (items > 0 && !mbar_wait(&s.h_free, (items - 1) & 1, &s.give_up)) return false;
+        if (items++ == 0) mi_pdl_wait();
+        if (hq < h_pieces)
+          for (int row = h_row; row < item.z; row += h_step) {
+            const bf16* from = g.held + (size_t)__ldcg(g.order + item.y + row) * g.P * hp + hq * 8;
+            for (int p = 0; p < np; ++p)
+              copy_piece(h_at + (p * ha + hq / 8) * TC_ATOM + row * 128 + (((hq & 7) ^ (row & 7)) << 4), from + (size_t)(part + p) * hp, 16);
+          }
+        copies_commit();                                      // (one group more than tiles: waits for tiles wait for no less)
+      }
       asked = j + 1;
       copies_wait<LAG>();
       tell(asked - LAG);
@@ -1247,11 +1252,16 @@ static int add_tc_stages(int R, int pairs) {
 }
 
 static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t stream) {
-  static size_t allowed[5][64];
-  const size_t sums_bytes = SUMS_STAGES * SUMS_STAGE_BYTES + 1024;
-  cudaError_t e = allow_smem(adapter_sums_tc_kernel, sums_bytes, allowed[0]);
+  static size_t allowed[6][64];
+  const int PR = g.P * g.R;
+  const dim3 sums_grid(g.ks, max_items, (PR + 127) / 128);
+  // two blocks on an SM: four stages of up to 96 sums, three of more
+  const int sums_stages = PR <= 96 ? 4 : 3;
+  const size_t sums_bytes = (size_t)sums_stages * sums_stage_bytes(PR) + 1024;
+  const auto sums = sums_stages == 4 ? adapter_sums_tc_kernel<4> : adapter_sums_tc_kernel<3>;
+  cudaError_t e = allow_smem(sums, sums_bytes, allowed[sums_stages == 4 ? 5 : 0]);
   if (e != cudaSuccess) return e;
-  e = MI_LAUNCH((adapter_sums_tc_kernel), dim3(g.ks, max_items, (g.P * g.R + 127) / 128), TC_THREADS, sums_bytes, stream, g);
+  e = MI_LAUNCH((sums), sums_grid, TC_THREADS, sums_bytes, stream, g);
   if (e != cudaSuccess) return e;
   const long long quarters = (long long)g.M * g.P * (padded_rank(g.R) / 4);
   e = MI_LAUNCH((adapter_held_kernel), (unsigned)((quarters + 255) / 256), 256, 0, stream, g);
