@@ -35,6 +35,7 @@ struct AdapterArgs {
   int ks;                         // parts of the sum over K
   const int* order;
   const int4* items;              // (and behind the last one: how many there are)
+  int item_rows;                  // rows of an item of few rows, at most FEW_ROWS
   int max_items, tiles;           // of the plan; of 128 columns in a row
   int constant;                   // no kernel in flight writes A and B
 };
@@ -132,13 +133,12 @@ inline int count_chunks(const AdapterArgs& g, int size) {
 #define FEW_ROWS 8            // rows of an item
 #define SUM_GROUP 64          // sums of the first product that a block makes
 #define MAX_ROWS 128          // rows of an item of a plan
-#define SUB_ITEMS (MAX_ROWS / FEW_ROWS)
 
 struct Item {
   int id, count;              // adapter (-1: none), rows
 };
 
-// Item `index` of a call of few rows, 8 rows each: rows with one adapter are put together in their order, and items are in the order of
+// Item `index` of a call of few rows: rows with one adapter are put together in their order, and items are in the order of
 // their first rows.  `rows` and `ids` are shared memory; count 0: there is no such item.
 __device__ __forceinline__ Item few_item(const AdapterArgs& g, int index, int* rows, int* ids, int* found) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -159,7 +159,7 @@ __device__ __forceinline__ Item few_item(const AdapterArgs& g, int index, int* r
     }
     for (int j = tid & ~3; j < tid; ++j) before += ids[j] == id;
   }
-  const bool leads = tid < g.M && before % 8 == 0;
+  const bool leads = tid < g.M && before % g.item_rows == 0;
   const unsigned vote = __ballot_sync(0xffffffffu, leads);
   int* votes = ids + FEW_MAX;                       // [warps]
   if (lane == 0) votes[warp] = __popc(vote);
@@ -173,7 +173,7 @@ __device__ __forceinline__ Item few_item(const AdapterArgs& g, int index, int* r
   __syncthreads();
   Item item = {found[0] - 2, 0};
   const int base = found[1];
-  const bool mine = tid < g.M && found[0] && id == item.id && before >= base && before < base + 8;
+  const bool mine = tid < g.M && found[0] && id == item.id && before >= base && before < base + g.item_rows;
   if (mine) rows[before - base] = tid;
   item.count = __syncthreads_count(mine);
   return item;
@@ -181,8 +181,9 @@ __device__ __forceinline__ Item few_item(const AdapterArgs& g, int index, int* r
 
 __device__ __forceinline__ Item get_item(const AdapterArgs& g, int index, int* rows, int* ids, int* found) {
   if (!g.items) return few_item(g, index, rows, ids, found);
-  const int4 v = __ldcg(g.items + index / SUB_ITEMS);
-  const int first = index % SUB_ITEMS * FEW_ROWS, count = max(0, min(FEW_ROWS, v.z - first));
+  const int subs = MAX_ROWS / g.item_rows;
+  const int4 v = __ldcg(g.items + index / subs);
+  const int first = index % subs * g.item_rows, count = max(0, min(g.item_rows, v.z - first));
   if (threadIdx.x < (unsigned)count) rows[threadIdx.x] = __ldcg(g.order + v.y + first + threadIdx.x);
   __syncthreads();
   return Item{v.x, count};
@@ -275,8 +276,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) adapter_sums_kernel(const Ada
 // 4 g .. 4 g + 3 of tokens 2 t and 2 t + 1.  B and y of the next columns are loaded between the products and the stores of the last
 // ones.
 //
-// KG: groups of 32 k (0: as many as there are).  Sums and their rests take two passes, but for items of up to four rows, where the rests
-// stand in the place of four more tokens, and (FOLD) for up to 16 k, where they stand in the place of 16 more.
+// KG: groups of 32 k (0: as many as there are).  The rests of the sums ride along: with up to 16 k (FOLD) they stand in the place of 16
+// more, else items have up to four rows and the rests stand in the place of four more tokens.
 // BLOCKS: of an SM.  A grid that fits at two has the registers of two: 16 rows, ranks 4 to 32, 14336 x 4096 13.0 us become 9.9, one row
 // at 4096 x 6144 7.3 become 6.5; 128 rows at 4096 x 28672, which does not, would take 31.4 instead of 22.8.
 template <int KG, bool FOLD, int BLOCKS>
@@ -362,8 +363,7 @@ __global__ void __launch_bounds__(TILE_THREADS, BLOCKS) adapter_add_kernel(const
   }
   __syncthreads();
 
-  const bool half = !FOLD && item.count <= 4;                 // tokens 4 .. 7 are the rests of tokens 0 .. 3
-  const bf16* h0 = h + (half ? (gq & 3) + (gq >> 2) * FEW_ROWS : gq) * stride + t * 8;
+  const bf16* h0 = h + (FOLD ? gq : (gq & 3) + (gq >> 2) * FEW_ROWS) * stride + t * 8;
   const int second = g.pairs ? 2 * FEW_ROWS * stride : 0;     // the columns 2 i + 1 of pairs have sums of their own
   for (; c0 < c_end; c0 += TILE_WARPS * 32) {
     const int c = c0 + 4 * gq;
@@ -385,7 +385,6 @@ __global__ void __launch_bounds__(TILE_THREADS, BLOCKS) adapter_add_kernel(const
       for (int m = 0; m < 2; ++m) {
         const bf16* hp = h0 + k0 + (m ? second : 0);
         mma_k32(acc[m], v[m][0], v[m][1], load16(hp));
-        if (!FOLD && !half) mma_k32(acc[m], v[m][0], v[m][1], load16(hp + FEW_ROWS * stride));
       }
     };
     if (KG) {
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(TILE_THREADS, BLOCKS) adapter_add_kernel(const
       load_all_b(c + TILE_WARPS * 32);
       load_y(c + TILE_WARPS * 32);
     }
-    if (half) {
+    if (!FOLD) {
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -1098,7 +1097,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
 // ---- the plan: rows in the order of their adapters, and items of up to 64 of them
 
 #define PLAN_THREADS 1024
-#define PLAN_MAX_ADAPTERS 2048
+#define PLAN_MAX_ADAPTERS 1024
 
 __global__ void __launch_bounds__(PLAN_THREADS)
 adapter_plan_kernel(const int* ids, int M, int n, int* order, int4* items, int max_items) {
@@ -1235,9 +1234,9 @@ static cudaError_t launch_few(const AdapterArgs& g, int max_items, cudaStream_t 
 template <typename T, bool VEC>
 static cudaError_t launch_plain(const AdapterArgs& g, int max_items, cudaStream_t stream) {
   static size_t allowed[64];
-  const int groups = (g.P * g.R + TILE_WARPS * PLAIN_SUMS - 1) / (TILE_WARPS * PLAIN_SUMS);
-  cudaError_t e = cudaSuccess;
-  if (g.n > 0 && g.R > 0) e = MI_LAUNCH((adapter_sums_plain_kernel<T, VEC>), dim3(g.ks, max_items, groups), TILE_THREADS, 0, stream, g);
+  // (also where there is nothing to add: the second kernel looks for its rows ahead of its wait, and may because this one waits)
+  const int groups = g.R > 0 ? (g.P * g.R + TILE_WARPS * PLAIN_SUMS - 1) / (TILE_WARPS * PLAIN_SUMS) : 1;
+  cudaError_t e = MI_LAUNCH((adapter_sums_plain_kernel<T, VEC>), dim3(g.ks, max_items, groups), TILE_THREADS, 0, stream, g);
   if (e != cudaSuccess) return e;
   const size_t bytes = (size_t)(g.pairs ? 2 : 1) * ((g.R + 3) & ~3) * FEW_ROWS * 4;
   e = allow_smem(adapter_add_plain_kernel<T, VEC>, bytes, allowed);
@@ -1289,13 +1288,17 @@ static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t
 // How a call runs, and the scratch memory (h) that it takes.
 enum { BY_ELEMENTS, BY_FEW, BY_MANY };
 struct Route {
-  int way, items, ks;
+  int way, items, item_rows, ks;
   long long floats, held_floats;      // of h, and behind it of `held`
 };
 static Route route_of(const void* y, long long ldy, const void* x, long long ldx, const void* a, const void* b, const void* out,
                       long long ldo, int M, int N, int K, int n, int P, int R, const int* ends, int pairs, int dtype) {
-  Route r = {BY_ELEMENTS, 0, 1, (long long)M * P * R, 0};
-  r.items = M <= FEW_MAX ? (M < n + 1 + M / 8 ? M : n + 1 + M / 8) : plan_items(M, n) * SUB_ITEMS;
+  Route r = {BY_ELEMENTS, 0, 0, 1, (long long)M * P * R, 0};
+  const auto few_items = [&](int rows) {
+    r.item_rows = rows;
+    r.items = M <= FEW_MAX ? (M < n + 1 + M / rows ? M : n + 1 + M / rows) : plan_items(M, n) * (MAX_ROWS / rows);
+  };
+  few_items(FEW_ROWS);
   // The tensor-core kernels take rows of x, A and B in pieces of 16 bytes.
   if (dtype != MI_DTYPE_BF16 || n <= 0 || R <= 0 || R > 256 || K <= 0 || R % 8 || K % 8 || !mi_aligned(a, 16) ||
       !mi_aligned(b, 16) || !mi_aligned(x, 16) || (M > 1 && ldx % 8)) {
@@ -1320,8 +1323,9 @@ static Route route_of(const void* y, long long ldy, const void* x, long long ldx
     r.held_floats = (long long)M * P * held_sums(R) / 2;
   } else {
     r.way = BY_FEW;
+    few_items(R <= 16 ? FEW_ROWS : FEW_ROWS / 2);
     const int units = (K + 31) / 32, groups = (P * R + SUM_GROUP - 1) / SUM_GROUP;
-    r.ks = 2 * 148 / (r.items * groups);
+    r.ks = 3 * 148 / (r.items * groups);
     if (r.ks > units / TILE_WARPS) r.ks = units / TILE_WARPS;
     r.ks = r.ks < 1 ? 1 : r.ks > 16 ? 16 : r.ks;
   }
@@ -1382,6 +1386,7 @@ extern "C" int mi_adapter_add(const AdapterCall* call, float* h, cudaStream_t st
   if (M > FEW_MAX && !(g.order && g.items)) MI_REFUSE("adapter_add: a plan of %d rows without their order", M);
   if (M <= FEW_MAX) g.items = nullptr;
   g.ks = r.ks;
+  g.item_rows = r.item_rows;
   if (r.way != BY_ELEMENTS) {
     g.max_items = r.way == BY_MANY ? r.items : 0;
     g.tiles = count_chunks(g, ADD_COLS);

@@ -248,6 +248,31 @@ def test_a_rows_sum_does_not_depend_on_its_company(M):
     assert torch.equal(o.adapter_add(y, x, a, b, o.adapter_plan(ids, n)), one)
 
 
+def test_a_rows_sum_does_not_depend_on_how_many_share_its_adapter():
+    """Items of up to four rows and of more hold the sums' rests elsewhere, and add up in the same order."""
+    o, M, n, K, N = ops(), 16, 3, 264, 200
+    for R in (16, 24, 64, 104):
+        a, b = adapters(n, (N,), R, K, BF, seed=R)
+        y, x = rnd(M, N, dtype=BF, seed=5), rnd(M, K, dtype=BF, seed=6)
+        alone = ints([0, 1, 0, 1, 1, 0, 2, 2, 2, -1, -1, -1, -1, -1, -1, -1])
+        together = ints([0, 1, 0, 1, 1, 0, 2, 2, 2, 0, 1, 0, 1, 0, 1, 2])
+        few = o.adapter_add(y, x, a, b, o.adapter_plan(alone, n))
+        more = o.adapter_add(y, x, a, b, o.adapter_plan(together, n))
+        assert torch.equal(few[:9], more[:9])
+
+
+@pytest.mark.parametrize("dtype", [F, BF])
+def test_a_plan_read_by_a_kernel_that_starts_early(dtype):
+    """Calls that add nothing, behind a fresh plan: rows come out as they were, whatever the memory of the plan held before."""
+    o, M = ops(), 2000
+    y = rnd(M, 24, dtype=dtype, seed=1)
+    for n, R, K in ((0, 8, 16), (3, 0, 16), (3, 8, 0)):
+        x, a, b = rnd(M, K, dtype=dtype), rnd(n, 1, R, K, dtype=dtype), rnd(n, 24, R, dtype=dtype)
+        for i in range(20):
+            ids = spread_ids(M, max(n, 1), i)
+            assert torch.equal(o.adapter_add(y, x, a, b, o.adapter_plan(ids, n)), y)
+
+
 # ----------------------------------------------------------------------------- logits
 
 

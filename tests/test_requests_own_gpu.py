@@ -122,6 +122,8 @@ def test_captured_steps_with_and_without_adapters(model_dirs):
     assert runner.load_adapter("y", other[1], other[0]) == 0
     assert generate(["y", "y"]) == [P.greedy_generate(merged(state, *other), TINY["C"], p, 7) for p in prompts]
     assert generate([None, None]) == bare
+    assert runner.capture_decode_steps(3) == 4          # (1,) and (3,), each with and without
+    assert generate(["y", None]) == [P.greedy_generate(merged(state, *other), TINY["C"], prompts[0], 7), bare[1]]
 
 
 def test_adapters_are_refused_where_they_do_not_fit(model_dirs):
