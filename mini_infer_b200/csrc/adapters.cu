@@ -525,11 +525,12 @@ __device__ __forceinline__ float4 four_values(const T* row, int k, int n) {
 
 // Items of up to eight rows as above, so that what is read of A and B serves all of them; float32 products have no tensor cores that
 // keep their bits.  Bound by the loads' latency (one row of rank 16 at 4096 x 6144 8.5 us) and, for many rows, by the CUDA
-// cores: 1500 rows 109 us, of which the products at their rate are 3 and the rest is what feeds them.
+// cores: 1500 rows 117 us, of which the products at their rate are 3 and the rest is what feeds them.
 //
 // The first product: a warp makes four sums of an item's up to eight rows over a share of K, its lanes four values of k each; the 32
 // totals are shared out over the lanes while they are added up.
 #define PLAIN_SUMS 4
+#define PLAIN_UNITS 2         // of 128 k in a part of the sum, at least
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(TILE_THREADS, 3) adapter_sums_plain_kernel(const AdapterArgs g) {
   mi_pdl_wait();
@@ -1380,11 +1381,10 @@ static Route route_of(const void* y, long long ldy, const void* x, long long ldx
   // The tensor-core kernels take rows of x, A and B in pieces of 16 bytes.
   if (dtype != MI_DTYPE_BF16 || n <= 0 || R <= 0 || R > 256 || K <= 0 || R % 8 || K % 8 || !mi_aligned(a, 16) ||
       !mi_aligned(b, 16) || !mi_aligned(x, 16) || (M > 1 && ldx % 8)) {
-    const int groups = (P * R + TILE_WARPS * PLAIN_SUMS - 1) / (TILE_WARPS * PLAIN_SUMS), units = (K + 127) / 128;
-    const int likely = M <= FEW_MAX ? r.items : M / FEW_ROWS + n;      // (a plan has room for more items than there are)
-    // (1500 rows of rank 16 at 4096 x 6144: 109 us, with half as many blocks 114, with twice 110)
-    r.ks = 12 * 148 / (likely * groups + 1);
-    if (r.ks > units) r.ks = units;
+    // Parts of the sum over K follow from K alone, so that float32 rows have the same bits in whatever company.  Rank 16, 4096 x 6144, parts of
+    // 256 k and of 512: one row 8.3 and 9.5 us, 1500 rows 117 and 110 (with parts by the number of rows 8.4 and 108).
+    const int units = (K + 127) / 128;
+    r.ks = units / PLAIN_UNITS;
     r.ks = r.ks < 1 ? 1 : r.ks > 16 ? 16 : r.ks;
     r.floats *= r.ks;
     return r;
@@ -1478,7 +1478,7 @@ extern "C" int mi_adapter_add(const AdapterCall* call, float* h, cudaStream_t st
     if (e != cudaSuccess) return refused_by_cuda(e);
     MI_RETURN_LAUNCH_STATUS();
   }
-  // (1500 rows of rank 16 at 4096 x 6144: 109 us, with half as many blocks 116, with twice 111)
+  // (1500 rows of rank 16 at 4096 x 6144, with parts by the number of rows: 109 us, with half as many blocks 116, with twice 111)
   g.span = 2048;
   while (g.span > 256 && (long long)(M <= FEW_MAX ? r.items : M / FEW_ROWS + n) * count_chunks(g, g.span) < 6 * 148) g.span /= 2;
   if (R > 3000) MI_REFUSE("adapter_add: rank %d, at most 3000", R);

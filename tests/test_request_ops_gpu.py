@@ -261,6 +261,41 @@ def test_a_rows_sum_does_not_depend_on_how_many_share_its_adapter():
         assert torch.equal(few[:9], more[:9])
 
 
+@pytest.mark.parametrize("K", [200, 4096])
+def test_float32_rows_have_the_same_bits_in_any_company(K):
+    """As every sum of the 32-bit path: alone, among few rows, among many, beside more adapters, on strided rows."""
+    o, n, N, M = ops(), 6, 136, 700
+    a, b = adapters(n, (N,), 12, K, F)
+    y, x = rnd(M, N, seed=5), rnd(M, K, seed=6)
+    ids = spread_ids(M, n, 3)
+    whole = o.adapter_add(y, x, a, b, o.adapter_plan(ids, n))
+    for lo, hi in ((0, 1), (5, 6), (0, 9), (100, 300), (300, 699)):
+        part = ids[lo:hi].contiguous()
+        assert torch.equal(o.adapter_add(y[lo:hi], x[lo:hi], a, b, o.adapter_plan(part, n)), whole[lo:hi])
+    wide = torch.empty(M, K + 1, device=DEV)
+    wide[:, 1:] = x                              # rows off their 16-byte boundaries
+    assert torch.equal(o.adapter_add(y, wide[:, 1:], a, b, o.adapter_plan(ids, n)), whole)
+
+
+@pytest.mark.parametrize("M,n,R,widths,pairs", [
+    (200, 40, 16, (520, 8, 300, 772), False), (256, 3, 24, (2000, 24), False), (130, 130, 64, (1304,), False),
+    (256, 64, 16, (1368, 1368), True), (90, 30, 200, (264, 1000), False), (300, 9, 136, (1400, 8, 264), False),
+    (700, 3, 200, (900, 900), True)])
+def test_tiles_of_many_items_shared_out_over_blocks(M, n, R, widths, pairs):
+    """Stretches of tiles that cross parts and items, among them items of rank 0 and rows without an adapter."""
+    o, K = ops(), 1040
+    a, b = adapters(n, widths, R, K, BF)
+    y, x = rnd(M, sum(widths), dtype=BF, seed=5), rnd(M, K, dtype=BF, seed=6)
+    ids = spread_ids(M, n, 2)
+    ranks = ints([(0, R, 1, 8, R - 3)[i % 5] for i in range(n)])
+    plan = o.adapter_plan(ids, n)
+    got = o.adapter_add(y, x, a, b, plan, ranks=ranks, parts=widths, pairs=pairs)
+    check_adapter(got, y, x, a, b, ids, ranks=ranks, parts=widths, pairs=pairs)
+    y2 = y.clone()
+    o.adapter_add(y2, x, a, b, plan, ranks=ranks, parts=widths, pairs=pairs, out=y2)
+    assert torch.equal(y2, got)
+
+
 @pytest.mark.parametrize("dtype", [F, BF])
 def test_a_plan_read_by_a_kernel_that_starts_early(dtype):
     """Calls that add nothing, behind a fresh plan: rows come out as they were, whatever the memory of the plan held before."""
