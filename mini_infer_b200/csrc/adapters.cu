@@ -83,7 +83,7 @@ __device__ __forceinline__ uint4 first_of(uint4 v, int n) {
   return v;
 }
 
-// A sum of the first product as two bfloat16 numbers, h = hi + lo: what is left of it is up to 2^-17 of it, below what the result's
+// A sum of the first product as two bfloat16 numbers, h = hi + lo: what is left of it is up to 2^-16 of it, below what the result's
 // own rounding leaves.  The second product takes both.
 __device__ __forceinline__ void split_bf16(float v, bf16& hi, bf16& lo) {
   hi = __float2bfloat16_rn(v);

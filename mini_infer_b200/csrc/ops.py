@@ -3021,7 +3021,9 @@ ADAPTER_FEW_ROWS = 256       # rows whose adapters the kernels look through by t
 
 
 def adapter_plan(ids: torch.Tensor, adapters: int) -> AdapterPlan:
-    """``ids`` int32 ``[M]``: the adapter of each row, in any order; a number outside ``[0, adapters)`` is none."""
+    """``ids`` int32 ``[M]``: the adapter of each row, in any order; a number outside ``[0, adapters)`` is none.  The plan keeps
+    ``ids`` itself, which stay as they are while calls with the plan are in flight; a graph that captures the plan with the
+    calls may find other ids in their memory at each replay.  More than ``ADAPTER_FEW_ROWS`` rows take at most 1024 adapters."""
     if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous():
         raise KernelError("adapter_plan: ids must be a contiguous int32 vector")
     if adapters < 0:
@@ -3047,8 +3049,11 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     what the low-rank adapters of a step's requests add to the output ``y [M, N]`` of the projection of ``x [M, K]`` that
     they share.  ``out`` is a new tensor, ``y`` itself, or one that overlaps neither operand.
 
-    ``a [adapters, P, R, K]``, ``b [adapters, N, R]``, contiguous and in the dtype of ``x`` and ``y`` (float32 or bfloat16; sums
-    are fp32 and rounded once).  ``P`` projections may be merged along their columns: ``parts`` are their widths, side by
+    ``a [adapters, P, R, K]``, ``b [adapters, N, R]``, contiguous and in the dtype of ``x`` and ``y`` (float32 or bfloat16), ranks to 3000.
+    Sums are fp32 and the result is rounded once; in bfloat16 the sums over ``K`` enter the second product as two bfloat16 numbers
+    each (off by up to 2^-16 of them), and from rank 33 on with more than ``ADAPTER_FEW_ROWS`` rows as one (up to 2^-8).  Rows of
+    float32 have the same bits in whatever company; in bfloat16 the order of sums follows from the rows and adapters of the call.
+    ``P`` projections may be merged along their columns: ``parts`` are their widths, side by
     side, at most four (default: one), or with ``pairs`` two of equal width that alternate column by column (gate 0, up 0,
     gate 1, ...).  A column of part ``p`` takes ``a[:, p]``.  ``ranks`` (int32): adapters whose rank is below ``R``; what lies
     behind it is not read.  ``w_constant``: no kernel in flight writes ``a`` and ``b``."""
