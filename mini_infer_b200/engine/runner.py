@@ -9,6 +9,7 @@ reduced to what a single-GPU engine for local model folders needs.
 from __future__ import annotations
 
 import os
+import threading
 from typing import Any, Mapping, Sequence
 
 import torch
@@ -66,6 +67,7 @@ class ModelRunner:
         self.num_blocks = num_blocks
         self.block_size = block_size
         self._adapter_names: list[str | None] | None = None      # by index; None: adapters are off
+        self._adapter_lock = threading.RLock()                   # names and users: requests come from any thread
 
     @classmethod
     def from_pretrained(cls, model_dir: str | os.PathLike, *, device="cuda:0", dtype="bfloat16",
@@ -118,22 +120,25 @@ class ModelRunner:
     def enable_adapters(self, count: int = 8, rank: int = 16) -> None:
         """Make room for ``count`` low-rank adapters of rank up to ``rank`` beside every product of the model that takes them
         (``Part.adapted``).  Once, before the first is loaded."""
-        if self._adapter_names is not None:
-            raise ValueError("adapters are enabled already")
         if count <= 0 or rank <= 0:
             raise ValueError(f"room for {count} adapters of rank {rank}")
         if rank > 256:
             raise ValueError(f"adapters of rank {rank}: at most 256")
-        held = -(-rank // 8) * 8          # whole pieces of 16 bytes
-        parts = [p for p in self.model.all_parts() if p.adapted()]
-        if not parts:
-            raise ValueError("no part of this model takes adapters")
-        for p in parts:
-            p.banks = {q.name: AdapterBank(q, count, held, self.dtype, self.device) for q in p.adapted()}
-        self._adapter_names = [None] * count
-        self._adapter_users = [0] * count
-        self._adapter_rank = rank
-        self.stepper.adapter_count = count
+        if count > 1024:
+            raise ValueError(f"{count} adapters: at most 1024")
+        with self._adapter_lock:
+            if self._adapter_names is not None:
+                raise ValueError("adapters are enabled already")
+            held = -(-rank // 8) * 8          # whole pieces of 16 bytes
+            parts = [p for p in self.model.all_parts() if p.adapted()]
+            if not parts:
+                raise ValueError("no part of this model takes adapters")
+            for p in parts:
+                p.banks = {q.name: AdapterBank(q, count, held, self.dtype, self.device) for q in p.adapted()}
+            self._adapter_names = [None] * count
+            self._adapter_users = [0] * count
+            self._adapter_rank = rank
+            self.stepper.adapter_count = count
 
     def load_adapter(self, name: str, source, config: Mapping[str, Any] | None = None) -> int:
         """Load an adapter under ``name`` and return its index: ``source`` is a folder (``weights.read_adapter``), or the adapter's
@@ -160,34 +165,36 @@ class ModelRunner:
                                   + "; ".join(filter(None, [f"no product that takes adapters: {unknown}" if unknown else "",
                                                             f"sizes (expected, found): {wrong}" if wrong else ""])),
                                   unexpected=unknown, mismatched=wrong)
-        if self._adapter_names is None:
-            self.enable_adapters(rank=rank)
-        if rank > self._adapter_rank:
-            raise ValueError(f"adapter {name!r} has rank {rank}, room is for {self._adapter_rank}")
-        if name in self._adapter_names:
-            raise ValueError(f"an adapter {name!r} is loaded already")
-        if None not in self._adapter_names:
-            raise ValueError(f"all {len(self._adapter_names)} places for adapters are taken")
-        index = self._adapter_names.index(None)
-        with torch.inference_mode():
-            for p in self.model.all_parts():
-                for q in (p.adapted() if p.banks is not None else ()):
-                    mine = {local: matrices[p.spec.tensor_name(local)] for local in q.tensors
-                            if p.spec.tensor_name(local) in matrices}
-                    p.banks[q.name].put(index, mine, scale)
-        self._adapter_names[index] = name
-        return index
+        with self._adapter_lock:
+            if self._adapter_names is None:
+                self.enable_adapters(rank=rank)
+            if rank > self._adapter_rank:
+                raise ValueError(f"adapter {name!r} has rank {rank}, room is for {self._adapter_rank}")
+            if name in self._adapter_names:
+                raise ValueError(f"an adapter {name!r} is loaded already")
+            if None not in self._adapter_names:
+                raise ValueError(f"all {len(self._adapter_names)} places for adapters are taken")
+            index = self._adapter_names.index(None)
+            with torch.inference_mode():
+                for p in self.model.all_parts():
+                    for q in (p.adapted() if p.banks is not None else ()):
+                        mine = {local: matrices[p.spec.tensor_name(local)] for local in q.tensors
+                                if p.spec.tensor_name(local) in matrices}
+                        p.banks[q.name].put(index, mine, scale)
+            self._adapter_names[index] = name
+            return index
 
     def unload_adapter(self, name: str) -> None:
         """Give an adapter's place back; refused while requests use it."""
-        index = self.adapter_index(name)
-        if self._adapter_users[index]:
-            raise ValueError(f"adapter {name!r} is in use by {self._adapter_users[index]} requests")
-        with torch.inference_mode():
-            for p in self.model.all_parts():
-                for bank in (p.banks or {}).values():
-                    bank.clear(index)
-        self._adapter_names[index] = None
+        with self._adapter_lock:
+            index = self.adapter_index(name)
+            if self._adapter_users[index]:
+                raise ValueError(f"adapter {name!r} is in use by {self._adapter_users[index]} requests")
+            with torch.inference_mode():
+                for p in self.model.all_parts():
+                    for bank in (p.banks or {}).values():
+                        bank.clear(index)
+            self._adapter_names[index] = None
 
     def adapter_index(self, name: str) -> int:
         if self._adapter_names is None or name is None or name not in self._adapter_names:
@@ -196,12 +203,14 @@ class ModelRunner:
 
     def hold_adapter(self, name: str) -> int:
         """The adapter's index, for a request that uses it until ``release_adapter``."""
-        index = self.adapter_index(name)
-        self._adapter_users[index] += 1
-        return index
+        with self._adapter_lock:
+            index = self.adapter_index(name)
+            self._adapter_users[index] += 1
+            return index
 
     def release_adapter(self, index: int) -> None:
-        self._adapter_users[index] -= 1
+        with self._adapter_lock:
+            self._adapter_users[index] -= 1
 
     # -- requests -----------------------------------------------------------------------
 

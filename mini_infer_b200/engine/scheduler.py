@@ -38,6 +38,7 @@ import enum
 import json
 import threading
 import time
+import warnings
 from typing import Any, Callable, Hashable, Sequence
 
 import numpy as np
@@ -69,7 +70,8 @@ class Request:
     max_tokens: int = 16
     adapter: str | None = None      # name of a low-rank adapter that the runner has loaded
     # a grammar: given the tokens generated so far, the ids of the tokens that may come next, or their bits (a numpy int32
-    # array of ceil(V / 32) words); None: any token.  No token at all ends the request as "stop".
+    # array of ceil(V / 32) words); None: any token.  No token at all ends the request as "stop", an exception as "cancelled"
+    # (with a warning; other requests go on).
     token_mask: Callable[[list[int]], Any] | None = None
 
 
@@ -120,7 +122,7 @@ class RunningRequest:
         self.cancel_requested = False
         self.in_flight_after_done = False       # finished while a step launched ahead still writes its pages
         self.adapter = -1                       # the runner's index of the request's adapter
-        self.mask_ended = False                 # the grammar allows no further token
+        self.mask_ended: str | None = None      # "stop": the grammar allows no further token; "cancelled": it failed
 
     def result(self, detokenize=None) -> GenerationResult:
         text = detokenize(self.generated) if detokenize else ""
@@ -690,7 +692,7 @@ class ContinuousScheduler:
         pages stay until that step has been read.  The request's streaming callback is not
         called here (the lock is held) but noted in ``emitted`` for ``_emit``."""
         if token in self.eos_token_ids or rr.mask_ended:
-            self._retire(rr, "stop", still_in_flight)
+            self._retire(rr, rr.mask_ended or "stop", still_in_flight)
             return
         rr.generated.append(token)
         rr.next_token = token
@@ -723,16 +725,27 @@ class ContinuousScheduler:
         for rr in rrs:
             row = AdjustedRow(rr.rid, rr.request.sampling_params, rr.prompt_ids, rr.generated)
             if rr.request.token_mask is not None:
-                said = rr.request.token_mask(list(rr.generated))
-                if said is not None:
-                    row.words = said if getattr(said, "dtype", None) == np.int32 else mask_words(said, V)
-                    if row.words.shape != (-(-V // 32),):
-                        raise ValueError(f"a mask of {row.words.shape} words for {V} tokens")
+                try:
+                    row.words = self._grammar(rr, V)
+                except Exception as e:  # noqa: BLE001
+                    warnings.warn(f"request {rr.rid}: its token_mask failed: {e!r}")
+                    rr.mask_ended = "cancelled"
+                if row.words is not None:
                     row.words = self._adjuster.mask_of(row)
-                    rr.mask_ended = not mask_any(row.words, V)
+                    rr.mask_ended = None if mask_any(row.words, V) else "stop"
             rows.append(row)
         self._adjuster.apply(logits, rows)
         return rows
+
+    @staticmethod
+    def _grammar(rr: RunningRequest, V: int) -> "np.ndarray | None":
+        said = rr.request.token_mask(list(rr.generated))
+        if said is None:
+            return None
+        words = said if getattr(said, "dtype", None) == np.int32 else mask_words(said, V)
+        if words.shape != (-(-V // 32),):
+            raise ValueError(f"a mask of {words.shape} words for {V} tokens")
+        return words
 
     def _finish(self, rr: RunningRequest, reason: str) -> None:
         if self._adjuster is not None:

@@ -99,11 +99,14 @@ class LogitsAdjuster:
         ops.record_tokens(self.counts, self.seen, slots, starts, tokens, n_prompt=n_prompt, fresh=True)
 
     def mask_of(self, row: AdjustedRow) -> np.ndarray | None:
-        """The row's mask: what it is limited to for good and what its grammar allows now."""
-        if row.params.allowed_token_ids is None:
+        """The row's mask: what it is limited to for good and what its grammar allows now, without the tokens that a bias rules out (so
+        that a mask with a bit has a token that may come)."""
+        allowed, never = row.params.allowed_token_ids, row.params.never
+        if allowed is None and (row.words is None or not never):
             return row.words
         if row.rid not in self._limits:
-            self._limits[row.rid] = mask_words(row.params.allowed_token_ids, self.vocab_size)
+            whole = np.full(-(-self.vocab_size // 32), -1, dtype=np.int32) if allowed is None else mask_words(allowed, self.vocab_size)
+            self._limits[row.rid] = whole & ~mask_words(never, self.vocab_size)
         return self._limits[row.rid] if row.words is None else self._limits[row.rid] & row.words
 
     def apply(self, logits: torch.Tensor, rows: Sequence[AdjustedRow]) -> None:

@@ -22,6 +22,9 @@ import math
 from typing import Mapping, Sequence
 
 
+_FP32_LEAST, _FP32_MOST = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127
+
+
 @dataclasses.dataclass(frozen=True)
 class SamplingParams:
     temperature: float = 0.0
@@ -43,25 +46,33 @@ class SamplingParams:
             raise ValueError(f"top_p must be in [0, 1], got {self.top_p}")
         if self.seed is not None and not 0 <= self.seed < 2 ** 64:
             raise ValueError(f"seed must fit 64 bits, got {self.seed}")
-        if not (self.repetition_penalty > 0 and math.isfinite(self.repetition_penalty)):
+        # (what the device computes with are fp32 numbers)
+        if not _FP32_LEAST <= self.repetition_penalty <= _FP32_MOST:
             raise ValueError(f"repetition_penalty must be positive, got {self.repetition_penalty}")
         for name in ("frequency_penalty", "presence_penalty"):
-            if not math.isfinite(getattr(self, name)):
+            if not abs(getattr(self, name)) <= _FP32_MOST:
                 raise ValueError(f"{name} must be a number, got {getattr(self, name)}")
         if self.logit_bias is not None:
             items = tuple((int(t), float(b)) for t, b in dict(self.logit_bias).items())
-            if any(t < 0 or math.isnan(b) or b == math.inf for t, b in items):
+            if any(t < 0 or not (abs(b) <= _FP32_MOST or b == -math.inf) for t, b in items):
                 raise ValueError(f"logit_bias gives numbers (or minus infinity) to token ids, got {self.logit_bias}")
             object.__setattr__(self, "logit_bias", items)       # hashable, and nobody's to change
         if self.allowed_token_ids is not None:
             ids = tuple(sorted({int(t) for t in self.allowed_token_ids}))
             if not ids or ids[0] < 0:
                 raise ValueError("allowed_token_ids must name at least one token")
+            if not set(ids) - set(self.never):
+                raise ValueError("logit_bias rules out every token of allowed_token_ids")
             object.__setattr__(self, "allowed_token_ids", ids)
 
     @property
     def greedy(self) -> bool:
         return self.temperature == 0.0
+
+    @property
+    def never(self) -> tuple[int, ...]:
+        """The tokens whose bias is minus infinity."""
+        return tuple(t for t, b in self.logit_bias or () if b == -math.inf)
 
     @property
     def penalised(self) -> bool:
@@ -74,6 +85,8 @@ class SamplingParams:
         return self.penalised or bool(self.logit_bias) or self.allowed_token_ids is not None
 
     def check_vocabulary(self, vocab_size: int) -> None:
+        if len(self.never) == vocab_size:
+            raise ValueError("logit_bias rules out every token")
         for t, _ in self.logit_bias or ():
             if t >= vocab_size:
                 raise ValueError(f"logit_bias names token {t} of {vocab_size}")

@@ -12,7 +12,7 @@ from mini_infer_b200.engine import Request
 from mini_infer_b200.engine.step import StepEntry, StepError, StepRunner
 from mini_infer_b200.parts import AdaptedProduct, AdapterBank, PartSpec, build_part
 from mini_infer_b200.sampling import SamplingParams, mask_any, mask_words
-from mini_infer_b200.sampling.adjust import LogitsAdjuster
+from mini_infer_b200.sampling.adjust import AdjustedRow, LogitsAdjuster
 from mini_infer_b200.weights import SafetensorsError, WeightLoadError, adapter_scale, pair_matrices, read_adapter
 from test_scheduler import FakeRunner, FakeSampler, make, prompt
 
@@ -27,6 +27,59 @@ from test_scheduler import FakeRunner, FakeSampler, make, prompt
 def test_options_are_checked(bad):
     with pytest.raises(ValueError):
         SamplingParams(**bad)
+
+
+@pytest.mark.parametrize("bad", [dict(repetition_penalty=1e39), dict(repetition_penalty=1e-40), dict(frequency_penalty=-1e39),
+                                 dict(presence_penalty=3.41e38), dict(logit_bias={3: 1e39}), dict(logit_bias={3: -1e39}),
+                                 dict(allowed_token_ids=[4, 7], logit_bias={4: -math.inf, 7: -math.inf})])
+def test_options_that_fp32_does_not_hold_or_that_leave_no_token(bad):
+    with pytest.raises(ValueError):
+        SamplingParams(**bad)
+
+
+def test_biases_that_rule_out_every_token():
+    p = SamplingParams(logit_bias={t: -math.inf for t in range(10)})
+    p.check_vocabulary(11)
+    with pytest.raises(ValueError, match="every token"):
+        p.check_vocabulary(10)
+    # a mask holds no token that a bias rules out
+    adjuster = LogitsAdjuster("cpu", 40, 2)
+    never = SamplingParams(logit_bias={5: -math.inf, 6: 2.0})
+    row = AdjustedRow("a", never, [1], [], mask_words([5], 40))
+    assert not mask_any(adjuster.mask_of(row), 40)
+    assert (adjuster.mask_of(AdjustedRow("a", never, [1], [], mask_words([5, 6, 39], 40))) == mask_words([6, 39], 40)).all()
+    assert adjuster.mask_of(AdjustedRow("a", never, [1], [])) is None
+    both = SamplingParams(logit_bias={5: -math.inf}, allowed_token_ids=[5, 9])
+    assert (adjuster.mask_of(AdjustedRow("b", both, [1], [])) == mask_words([9], 40)).all()
+
+
+def test_a_grammar_that_fails_ends_its_request_alone(monkeypatch):
+    from mini_infer_b200.engine import scheduler
+
+    class Adjuster(LogitsAdjuster):
+        def apply(self, logits, rows):
+            pass
+
+        def record(self, tokens, rows):
+            pass
+
+    monkeypatch.setattr(scheduler, "LogitsAdjuster", Adjuster)
+    runner = RunnerWithAdapters(64)
+    runner.device = "cpu"
+    sched = scheduler.ContinuousScheduler(runner, sampler=FakeSampler(), max_tokens_per_step=8)
+
+    def broken(generated):
+        if len(generated) == 2:
+            raise KeyError("no such state")
+        return range(1000)
+
+    handles = [sched.submit(Request(prompt(4), SamplingParams(), 5, token_mask=g))
+               for g in (broken, None, lambda said: np.zeros(3, np.int32), lambda said: [1000], lambda said: [] if said else None)]
+    with pytest.warns(UserWarning, match="token_mask failed"):
+        sched.run_until_done()
+    results = [h.wait() for h in handles]
+    assert [(r.finish_reason, len(r.tokens)) for r in results] == [("cancelled", 2), ("length", 5), ("cancelled", 0), ("cancelled", 0), ("stop", 1)]
+    assert runner.cache.num_requests == 0
 
 
 def test_options_say_what_they_change():
