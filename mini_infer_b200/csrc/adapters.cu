@@ -45,7 +45,7 @@ struct AdapterArgs {
 // way from the ids to the rows.  Three ways, by rows and types:
 //
 //   few rows (up to FEW_MAX, bfloat16)   mma.sync, blocks find their rows themselves: 6.4 us for a row of rank 16 at 4096 x 6144
-//   many rows (bfloat16)                 a plan, tcgen05: 252 us for 8192 rows of ranks to 64 at 4096 x 28672 (155 at the rate of a copy)
+//   many rows (bfloat16)                 a plan, tcgen05: 213 us for 8192 rows of ranks to 64 at 4096 x 28672 (155 at the rate of a copy)
 //   float32, and what is not in pieces of 16 bytes   CUDA cores
 //
 // ---------------------------------------------------------------------------------------------- few rows, bfloat16
@@ -901,6 +901,12 @@ __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_A
 //   eight summing warps  add a buffer to y in shared memory (a thread has a row) and write the result (a lane has pieces of
 //                        rows).  y lies in rows of 256 bytes, 16-byte pieces permuted by the row, so that both ways touch all banks.
 //
+// Bound by memory in long calls: a tile takes 1.6 us of a block, 1.5 us are its bytes at a copy's rate (8192 rows of ranks to 64 at
+// 4096 x 28672: 213 us for all kernels, of which this one is 175), in short ones by the 6 us until the first tile is there.  What a
+// warp does for a tile is a chain of latencies, so that a thread's numbers and its y are all asked for at once and a stage is given back
+// before the stores (together 253 us become 213); the first items and their ranks are looked up while tensor memory is allocated
+// (2048 rows of rank 16 at 4096 x 4096 33 us become 31).
+//
 // Copies gather (rows of an item lie anywhere), which a tensor map does not; a copy warp says that a tile is there once its own
 // copies have landed and are visible to the tensor cores.
 #define ADD_SUM_WARPS 8
@@ -908,7 +914,11 @@ __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_A
 #define ADD_COPY_THREADS (32 * ADD_COPY_WARPS)
 #define ADD_THREADS (32 * (ADD_SUM_WARPS + ADD_COPY_WARPS + 1))
 
+#define ADD_ITEMS 64                 // items that a block looks up ahead
+
 struct AddBlock {
+  int4 items[ADD_ITEMS];                                     // the first items, their rank instead of the last number
+  int n_items;
   uint64_t full[ADD_MAX_STAGES], empty[ADD_MAX_STAGES];      // a stage is there; the summing warps are through with it
   uint64_t done[2], free_[2];                                // a buffer's products have ended; it has been read
   uint64_t h_free;                                           // the products that read an item's sums have ended
@@ -919,15 +929,15 @@ struct AddBlock {
 // f(tile number of the block, item, rank, whether the item begins, whether it ends, chunk of columns) for a block's tiles in
 // order, until f returns false; items of which nothing changes are passed over.
 template <typename F>
-__device__ __forceinline__ void for_tiles(const AdapterArgs& g, F f) {
+__device__ __forceinline__ void for_tiles(const AdapterArgs& g, const AddBlock& s, F f) {
   const int per_item = g.tiles;
-  const long long all = (long long)__ldcg(&g.items[g.max_items].x) * per_item;
+  const long long all = (long long)s.n_items * per_item;
   const int t0 = (int)(all * blockIdx.x / gridDim.x), t1 = (int)(all * (blockIdx.x + 1) / gridDim.x);
   int count = 0;
   for (int t = t0; t < t1;) {
     const int index = t / per_item, end = min(t1, (index + 1) * per_item);
-    const int4 item = __ldcg(g.items + index);
-    const int rank = rank_of(g, item.x);
+    const int4 item = index < ADD_ITEMS ? s.items[index] : __ldcg(g.items + index);
+    const int rank = index < ADD_ITEMS ? item.w : rank_of(g, item.x);
     if (rank > 0 || g.out != g.y) {
       for (int u = t; u < end; ++u)
         if (!f(count++, item, rank, u == t, u + 1 == end, u - index * per_item)) return;
@@ -936,7 +946,7 @@ __device__ __forceinline__ void for_tiles(const AdapterArgs& g, F f) {
   }
 }
 
-template <int STAGES>
+template <int STAGES, bool PAIRS>
 __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const AdapterArgs g) {
   extern __shared__ unsigned char tc_smem[];
   __shared__ AddBlock s;
@@ -944,7 +954,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
   // is there, tensor memory is nobody's any more, and the copy warps alone wait, before they take the sums.)
   const uint32_t base = (smem_u32(tc_smem) + 1023) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = g.R;
-  const int np = g.pairs ? 2 : 1, rp = padded_rank(R), ha = sums_atoms(R), ba = b_atoms(R);
+  const int np = PAIRS ? 2 : 1, rp = padded_rank(R), ha = sums_atoms(R), ba = b_atoms(R);
   const uint32_t h_at = base, stages_at = base + np * ha * TC_ATOM, stage_bytes = add_stage_bytes(R);
   if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) {
     if (lane == 0) {
@@ -962,6 +972,11 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
     }
     __syncwarp();
     tc_alloc(&s.tmem, 2 * ADD_COLS);
+  } else if (tid < ADD_ITEMS) {
+    int4 item = __ldcg(g.items + min(tid, g.max_items - 1));
+    if (tid == 0) s.n_items = __ldcg(&g.items[g.max_items].x);
+    item.w = rank_of(g, item.x);
+    s.items[tid] = item;
   }
   tc_fence_before();
   __syncthreads();
@@ -982,7 +997,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
     constexpr int YN = TC_ROWS * 16 / ADD_COPY_THREADS;
     const uint32_t y_row = ba * TC_ATOM + yr * 256, y_place[2] = {y_row + ((yq ^ yr) << 4), y_row + ((yq ^ (yr + 8)) << 4)};
     const uint32_t b_place = bq / 8 * TC_ATOM + b_col * 128 + (((bq & 7) ^ (b_col & 7)) << 4);
-    const int b_stride = (g.pairs ? 2 : 1) * b_step * R;      // elements between a thread's columns
+    const int b_stride = (PAIRS ? 2 : 1) * b_step * R;      // elements between a thread's columns
     const bf16* y_from[YN];
     uint32_t y_in = 0;
     int items = 0, asked = 0, told = 0, last_part = -1;                       // begun so far, of those with an adapter; tiles asked for, and said to be there
@@ -990,7 +1005,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
       if (told < upto) smem_for_tensor_cores();
       for (; told < upto; ++told) mbar_arrive(&s.full[told % STAGES]);
     };
-    for_tiles(g, [&](int j, const int4& item, int rank, bool begins, bool, int chunk) {
+    for_tiles(g, s, [&](int j, const int4& item, int rank, bool begins, bool, int chunk) {
       const int stage = j % STAGES;
       const uint32_t to = stages_at + stage * stage_bytes;
       if (begins) {
@@ -999,7 +1014,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         for (int i = 0; i < YN; ++i) {
           const int row = yr + i * (TC_ROWS / YN);
           if (row < item.z) {
-            y_from[i] = y + __ldcg(g.order + item.y + row) * g.ldy + yq * 8;
+            y_from[i] = y + g.order[item.y + row] * g.ldy + yq * 8;
             y_in |= 1u << i;
           }
         }
@@ -1013,14 +1028,14 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         const bf16* b = (const bf16*)g.b + (size_t)item.x * g.N * R + bq * 8;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int first = g.pairs ? c + 2 * b_col + half : c + half * 64 + b_col;
+          const int first = PAIRS ? c + 2 * b_col + half : c + half * 64 + b_col;
           const bf16* from = b + (size_t)first * R;
           uint32_t at = to + b_place + half * (TC_ATOM / 2);
           if (c + ADD_COLS <= c_end && there == 16) {
             for (int col = b_col; col < 64; col += b_step, from += b_stride, at += b_step * 128) copy_piece(at, from, 16);
           } else {
             int column = first;
-            for (int col = b_col; col < 64; col += b_step, from += b_stride, at += b_step * 128, column += (g.pairs ? 2 : 1) * b_step) {
+            for (int col = b_col; col < 64; col += b_step, from += b_stride, at += b_step * 128, column += (PAIRS ? 2 : 1) * b_step) {
               const bool in = there && column < c_end;
               copy_piece(at, in ? from : (const bf16*)g.b, in ? there : 0);
             }
@@ -1047,7 +1062,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
         if (items++ == 0) mi_pdl_wait();
         if (hq < h_pieces)
           for (int row = h_row; row < item.z; row += h_step) {
-            const bf16* from = g.held + (size_t)__ldcg(g.order + item.y + row) * g.P * hp + hq * 8;
+            const bf16* from = g.held + (size_t)g.order[item.y + row] * g.P * hp + hq * 8;
             for (int p = 0; p < np; ++p)
               copy_piece(h_at + (p * ha + hq / 8) * TC_ATOM + row * 128 + (((hq & 7) ^ (row & 7)) << 4), from + (size_t)(part + p) * hp, 16);
           }
@@ -1064,9 +1079,9 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
   } else if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) {
     // ---- products
     if (lane == 0) {
-      const uint32_t desc = product_desc(g.pairs ? ADD_COLS / 2 : ADD_COLS);
+      const uint32_t desc = product_desc(PAIRS ? ADD_COLS / 2 : ADD_COLS);
       const int rests = with_rests(R);
-      for_tiles(g, [&](int j, const int4&, int rank, bool, bool ends, int chunk) {
+      for_tiles(g, s, [&](int j, const int4&, int rank, bool, bool ends, int chunk) {
         const int stage = j % STAGES, buf = j & 1;
         if (!mbar_wait(&s.full[stage], (j / STAGES) & 1, &s.give_up)) return false;
         if (j >= 2 && !mbar_wait(&s.free_[buf], (j / 2 - 1) & 1, &s.give_up)) return false;
@@ -1093,63 +1108,75 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
   } else {
     // ---- sums: a warp has 32 rows and half of a tile's columns
     const int row = (warp & 3) * 32 + lane, half = warp >> 2;
-    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21) + (g.pairs ? half * 32 : half * 64);
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21) + (PAIRS ? half * 32 : half * 64);
     const int q0 = lane & 7, r0 = (warp & 3) * 32 + (lane >> 3);       // the result: a piece of every 4th row
-    long long out_off[8];
+    int out_row[8];
     uint32_t out_in = 0;
-    for_tiles(g, [&](int j, const int4& item, int rank, bool begins, bool, int chunk) {
+    for_tiles(g, s, [&](int j, const int4& item, int rank, bool begins, bool, int chunk) {
       const int stage = j % STAGES, buf = j & 1;
       if (begins) {
         out_in = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (r0 + 4 * i < item.z) {
-            out_off[i] = __ldcg(g.order + item.y + r0 + 4 * i) * g.ldo + half * 64 + q0 * 8;
+            out_row[i] = g.order[item.y + r0 + 4 * i];
             out_in |= 1u << i;
           }
       }
       int part, c, c_end;
       find_chunk(g, chunk, ADD_COLS, part, c, c_end);
       const uint32_t y_at = stages_at + stage * stage_bytes + ba * TC_ATOM;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.full[stage], (j / STAGES) & 1, &s.give_up))) return false;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.done[buf], (j / 2) & 1, &s.give_up))) return false;
+      const bool there = mbar_wait(&s.full[stage], (j / STAGES) & 1, &s.give_up) && mbar_wait(&s.done[buf], (j / 2) & 1, &s.give_up);
+      if (!__all_sync(0xffffffffu, there)) return false;
       if (rank > 0) {
+        // 32 columns at a time, the next ones on their way meanwhile (a row behind the item's last is added up too, and not written)
+        uint32_t v[2][32];
+        const uint32_t from = lanes + buf * ADD_COLS, y_row = y_at + row * 256, turn = row & 15;
+        const auto fetch = [&](int o) {
+          tc_load16(from + (PAIRS ? o * 16 : o * 32), v[o]);
+          tc_load16(from + (PAIRS ? 64 + o * 16 : o * 32 + 16), v[o] + 16);
+        };
         tc_fence_after();
+        fetch(0);
 #pragma unroll
-        for (int o = 0; o < 2; ++o) {                         // 32 columns at a time
-          uint32_t v[32];
-          tc_load16(lanes + buf * ADD_COLS + (g.pairs ? o * 16 : o * 32), v);
-          tc_load16(lanes + buf * ADD_COLS + (g.pairs ? 64 + o * 16 : o * 32 + 16), v + 16);
+        for (int o = 0; o < 2; ++o) {
+          uint32_t w[16];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[4 * q]), "=r"(w[4 * q + 1]), "=r"(w[4 * q + 2]), "=r"(w[4 * q + 3])
+                         : "r"(y_row + (((half * 8 + o * 4 + q) ^ turn) << 4))
+                         : "memory");
           tc_load_wait();
-          if (o == 1) {
+          if (o == 0) {
+            fetch(1);
+          } else {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.free_[buf]);
           }
-          if (row < item.z) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint32_t place = y_at + row * 256 + (((half * 8 + o * 4 + q) ^ (row & 15)) << 4);
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place) : "memory");
+          for (int q = 0; q < 4; ++q) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int k = q * 8 + 2 * e;                  // the pair's first column of the 32
-                const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[e]));
-                const float d0 = __uint_as_float(g.pairs ? v[k / 2] : v[k]), d1 = __uint_as_float(g.pairs ? v[16 + k / 2] : v[k + 1]);
-                __nv_bfloat162 sum = __floats2bfloat162_rn(f.x + d0, f.y + d1);
-                w[e] = *reinterpret_cast<uint32_t*>(&sum);
-              }
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+            for (int e = 0; e < 4; ++e) {
+              const int k = q * 8 + 2 * e;                    // the pair's first column of the 32
+              const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[4 * q + e]));
+              const float d0 = __uint_as_float(PAIRS ? v[o][k / 2] : v[o][k]), d1 = __uint_as_float(PAIRS ? v[o][16 + k / 2] : v[o][k + 1]);
+              __nv_bfloat162 sum = __floats2bfloat162_rn(f.x + d0, f.y + d1);
+              w[4 * q + e] = *reinterpret_cast<uint32_t*>(&sum);
             }
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(y_row + (((half * 8 + o * 4 + q) ^ turn) << 4)), "r"(w[4 * q]),
+                         "r"(w[4 * q + 1]), "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                         : "memory");
           }
         }
       } else if (lane == 0) {
         mbar_arrive(&s.free_[buf]);
       }
       __syncwarp();
-      if (c + half * 64 + q0 * 8 < c_end) {
-        uint4 w[8];
+      const bool mine = c + half * 64 + q0 * 8 < c_end;
+      uint4 w[8];
+      if (mine) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if ((out_in >> i) & 1u) {
@@ -1159,12 +1186,15 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
                          : "r"(y_at + r * 256 + (((half * 8 + q0) ^ (r & 15)) << 4))
                          : "memory");
           }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if ((out_in >> i) & 1u) *reinterpret_cast<uint4*>(out + out_off[i] + c) = w[i];
       }
+      // (the stage is free once it has been read; the stores follow)
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.empty[stage]);
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((out_in >> i) & 1u) *reinterpret_cast<uint4*>(out + out_row[i] * g.ldo + (c + half * 64 + q0 * 8)) = w[i];
+      }
       return true;
     });
   }
@@ -1331,21 +1361,21 @@ static cudaError_t launch_plain(const AdapterArgs& g, int max_items, cudaStream_
 }
 
 // Stages that fit beside the sums: four up to rank 64, three up to 128 (two of pairs).
-static int add_tc_stages(int R, int pairs) {
-  const int left = 225 * 1024 - (pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM;
+static int add_tc_stages(int R, int pairs) {      // (of 227 KB 1 is for the alignment and up to 2 are AddBlock's)
+  const int left = 224 * 1024 - (pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM;
   const int n = left / add_stage_bytes(R);
   return n > ADD_MAX_STAGES ? ADD_MAX_STAGES : n;
 }
 
 static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t stream) {
-  static bool allowed[5][64];
+  static bool allowed[6][64];
   const int PR = g.P * g.R;
   const dim3 sums_grid(g.ks, max_items, (PR + 127) / 128);
   // two blocks on an SM: four stages of up to 96 sums, three of more (8192 rows of rank 16 at 14336 x 4096: 105 us, with three 108)
   const int sums_stages = PR <= 96 ? 4 : 3;
   const size_t sums_bytes = (size_t)sums_stages * sums_stage_bytes(PR) + 1024;
   const auto sums = sums_stages == 4 ? adapter_sums_tc_kernel<4> : adapter_sums_tc_kernel<3>;
-  cudaError_t e = allow_smem(sums, sums_bytes, allowed[sums_stages == 4 ? 4 : 0]);
+  cudaError_t e = allow_smem(sums, sums_bytes, allowed[sums_stages == 4 ? 5 : 0]);
   if (e != cudaSuccess) return e;
   e = MI_LAUNCH((sums), sums_grid, TC_THREADS, sums_bytes, stream, g);
   if (e != cudaSuccess) return e;
@@ -1356,16 +1386,12 @@ static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t
   const size_t bytes = (size_t)(g.pairs ? 2 : 1) * sums_atoms(g.R) * TC_ATOM + (size_t)stages * add_stage_bytes(g.R) + 1024;
   const long long tiles = (long long)max_items * g.tiles;
   const int grid = tiles < 148 ? (int)tiles : 148;
-  if (stages == 4) {
-    e = allow_smem(adapter_add_tc_kernel<4>, bytes, allowed[1]);
-    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<4>), grid, ADD_THREADS, bytes, stream, g);
-  }
-  if (stages == 3) {
-    e = allow_smem(adapter_add_tc_kernel<3>, bytes, allowed[2]);
-    return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<3>), grid, ADD_THREADS, bytes, stream, g);
-  }
-  e = allow_smem(adapter_add_tc_kernel<2>, bytes, allowed[3]);
-  return e != cudaSuccess ? e : MI_LAUNCH((adapter_add_tc_kernel<2>), grid, ADD_THREADS, bytes, stream, g);
+  const auto run = [&](auto kernel, bool* room) {
+    const cudaError_t e = allow_smem(kernel, bytes, room);
+    return e != cudaSuccess ? e : MI_LAUNCH((kernel), grid, ADD_THREADS, bytes, stream, g);
+  };
+  if (g.pairs) return stages == 4 ? run(adapter_add_tc_kernel<4, true>, allowed[1]) : run(adapter_add_tc_kernel<2, true>, allowed[2]);
+  return stages == 4 ? run(adapter_add_tc_kernel<4, false>, allowed[3]) : run(adapter_add_tc_kernel<3, false>, allowed[4]);
 }
 
 // How a call runs, and the scratch memory (h) that it takes.
