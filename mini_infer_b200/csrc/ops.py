@@ -3058,25 +3058,25 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     gate 1, ...).  A column of part ``p`` takes ``a[:, p]``.  ``ranks`` (int32): adapters whose rank is below ``R``; what lies
     behind it is not read.  ``w_constant``: no kernel in flight writes ``a`` and ``b``."""
     what = "adapter_add"
-    if x.dim() != 2 or y.dim() != 2 or a.dim() != 4 or b.dim() != 3:
-        raise KernelError(f"{what}: y [M, N], x [M, K], a [adapters, parts, R, K] and b [adapters, N, R]")
-    M, K = x.shape
-    N = y.shape[1]
-    n, P, R = a.shape[0], a.shape[1], a.shape[2]
-    if y.shape[0] != M or a.shape[3] != K or tuple(b.shape) != (n, N, R):
+    try:
+        (M, K), (rows, N), (n, P, R, depth), (n_b, N_b, R_b) = x.shape, y.shape, a.shape, b.shape
+    except ValueError:
+        raise KernelError(f"{what}: y [M, N], x [M, K], a [adapters, parts, R, K] and b [adapters, N, R]") from None
+    if rows != M or depth != K or n_b != n or N_b != N or R_b != R:
         raise KernelError(f"{what}: shapes y {tuple(y.shape)}, x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)} do not match")
     dtype = x.dtype
     code = _code(dtype)
-    if y.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
+    if y.dtype is not dtype or a.dtype is not dtype or b.dtype is not dtype:
         raise KernelError(f"{what}: operands of {x.dtype}, {y.dtype}, {a.dtype} and {b.dtype}")
-    if not (a.is_contiguous() and b.is_contiguous()) or (K and x.stride(1) != 1) or (N and y.stride(1) != 1):
+    (ldx, unit_x), (ldy, unit_y) = x.stride(), y.stride()
+    if not (a.is_contiguous() and b.is_contiguous()) or (K and unit_x != 1) or (N and unit_y != 1):
         raise KernelError(f"{what}: the adapters must be contiguous, x and y have unit inner stride")
     if plan.rows != M or plan.adapters != n:
         raise KernelError(f"{what}: a plan of {plan.rows} rows and {plan.adapters} adapters for {M} rows and {n} adapters")
     if pairs:
         if P != 2 or N % 2 or (parts is not None and tuple(parts) != (N // 2, N // 2)):
             raise KernelError(f"{what}: pairs are two parts of equal width, got {P} parts {parts} of {N} columns")
-        ends = (N, N, N, N)
+        e0 = e1 = e2 = N
     else:
         widths = (N,) if parts is None else tuple(parts)
         if len(widths) != P or P > ADAPTER_MAX_PARTS or sum(widths) != N or min(widths) < 0:
@@ -3084,30 +3084,36 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
         e0 = widths[0]
         e1 = e0 + (widths[1] if P > 1 else 0)
         e2 = e1 + (widths[2] if P > 2 else 0)
-        ends = (e0, e1, e2, N)
     if scale is not None:
         _vector(what, "scale", scale, torch.float32, n)
     if ranks is not None:
         _vector(what, "ranks", ranks, torch.int32, n)
+    ids = plan.ids
     if out is None:
-        _same_device(what, x, y, a, b, plan.ids, scale, ranks)
+        _same_device(what, x, y, a, b, ids, scale, ranks)
         out = torch.empty_like(y) if y.is_contiguous() else torch.empty((M, N), dtype=dtype, device=x.device)
+        ldo = N
+    elif out is y and (M <= 1 or ldy >= N) and _apart(y, x):
+        _same_device(what, x, y, a, b, ids, scale, ranks)
+        ldo = ldy
     else:
         if out.shape != y.shape or out.dtype != dtype or (N and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise KernelError(f"{what}: out must be [M, N] in the operands' dtype, rows apart, with unit inner stride")
-        same = out.data_ptr() == y.data_ptr() and (M <= 1 or out.stride(0) == y.stride(0))
+        same = out.data_ptr() == y.data_ptr() and (M <= 1 or out.stride(0) == ldy)
         if not (same or _apart(out, y)) or not _apart(out, x):
             raise KernelError(f"{what}: out overlaps x, or y without being y")
-        _same_device(what, x, y, a, b, plan.ids, scale, ranks, out)
+        _same_device(what, x, y, a, b, ids, scale, ranks, out)
+        ldo = out.stride(0)
     if M == 0 or N == 0:
         return out
-    lib = _waiting_lib("adapters", x.device)
+    device = x.device
+    lib = _waiting_lib("adapters", device)
     order, items = plan.order, plan.items
-    block = _ADAPTER_BLOCK(y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), out.data_ptr(),
-                           out.stride(0), plan.ids.data_ptr(), 0 if order is None else order.data_ptr(),
-                           0 if items is None else items.data_ptr(), 0 if scale is None else scale.data_ptr(),
-                           0 if ranks is None else ranks.data_ptr(), M, N, K, n, P, R, *ends, pairs, w_constant, code, 0)
-    h = torch.empty(lib.mi_adapter_scratch(block), dtype=torch.float32, device=x.device)
+    block = _ADAPTER_BLOCK(y.data_ptr(), ldy, x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), out.data_ptr(), ldo, ids.data_ptr(),
+                           0 if order is None else order.data_ptr(), 0 if items is None else items.data_ptr(),
+                           0 if scale is None else scale.data_ptr(), 0 if ranks is None else ranks.data_ptr(), M, N, K, n, P, R,
+                           e0, e1, e2, N, pairs, w_constant, code, 0)
+    h = torch.empty(lib.mi_adapter_scratch(block), dtype=torch.float32, device=device)
     _finish(lib, lib.mi_adapter_add(block, h.data_ptr(), _stream()), what)
     return out
 
@@ -3141,9 +3147,9 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor | None = None, *, slot
     *Masks* ``[n, ceil(V / 32)]`` int32, one bit a token (bit ``v % 32`` of word ``v / 32``): row ``b`` keeps the tokens of
     mask ``mask_rows[b]`` (default ``b``; a number outside the masks: all tokens), the others become minus infinity whatever they were."""
     what = "adjust_logits"
-    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] and logits.stride(1) != 1):
+    if logits.dtype is not torch.float32 or logits.dim() != 2 or (logits.shape[1] and logits.stride(1) != 1):
         raise KernelError(f"{what}: logits must be fp32 [B, V] with unit inner stride")
-    B, V = logits.shape
+    (B, V), ld_in = logits.shape, logits.stride(0)
     n_slots = n_masks = n_bias = 0
     if seen is not None:
         n_slots = _history(what, counts, seen, V)
@@ -3155,9 +3161,9 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor | None = None, *, slot
         _vector(what, "slots", slots, torch.int32, B)
     elif seen is not None and n_slots < B:
         raise KernelError(f"{what}: {n_slots} histories for {B} rows without slots")
-    _vector(what, "repetition", repetition, torch.float32, B)
-    _vector(what, "presence", presence, torch.float32, B)
-    _vector(what, "frequency", frequency, torch.float32, B)
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if t is not None:
+            _vector(what, name, t, torch.float32, B)
     starts = ids = values = None
     if bias is not None:
         starts, ids, values = bias
@@ -3174,12 +3180,16 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor | None = None, *, slot
             raise KernelError(f"{what}: {n_masks} masks for {B} rows without mask_rows")
     elif mask_rows is not None:
         raise KernelError(f"{what}: mask_rows without masks")
-    if B > 1 and logits.stride(0) < V:
+    if B > 1 and ld_in < V:
         raise KernelError(f"{what}: the rows of the logits overlap")
     _same_device(what, logits, out, slots, seen, counts, repetition, presence, frequency, starts, ids, values, masks, mask_rows)
-    if out is None:
+    ld_out = V
+    if out is logits:
+        ld_out = ld_in
+    elif out is None:
         out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((B, V), dtype=torch.float32, device=logits.device)
     else:
+        ld_out = out.stride(0) if out.dim() == 2 else V
         if out.dtype != torch.float32 or out.shape != logits.shape or (V and out.stride(1) != 1) or (B > 1 and out.stride(0) < V):
             raise KernelError(f"{what}: out must be fp32 [B, V], rows apart, with unit inner stride")
         same = out.data_ptr() == logits.data_ptr() and (B <= 1 or out.stride(0) == logits.stride(0))
@@ -3187,13 +3197,9 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor | None = None, *, slot
             raise KernelError(f"{what}: out overlaps the logits without being them")
     if B == 0 or V == 0:
         return out
-    def at(t):
-        return 0 if t is None else t.data_ptr()
-
     lib = _lib("logits")
-    block = _ADJUST_BLOCK(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), B, V, at(slots), at(seen), at(counts),
-                          n_slots, at(repetition), at(presence), at(frequency), at(starts), at(ids), at(values), n_bias, at(masks),
-                          at(mask_rows), n_masks)
+    at = [0 if t is None else t.data_ptr() for t in (slots, seen, counts, repetition, presence, frequency, starts, ids, values, masks, mask_rows)]
+    block = _ADJUST_BLOCK(logits.data_ptr(), ld_in, out.data_ptr(), ld_out, B, V, *at[:3], n_slots, *at[3:9], n_bias, *at[9:], n_masks)
     _finish(lib, lib.mi_adjust_logits(block, _stream()), what)
     return out
 
