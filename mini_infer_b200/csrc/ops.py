@@ -3018,6 +3018,7 @@ class AdapterPlan:
 
 
 ADAPTER_FEW_ROWS = 256       # rows whose adapters the kernels look through by themselves
+ADAPTER_MAX_ROWS = 8_000_000
 
 
 def adapter_plan(ids: torch.Tensor, adapters: int) -> AdapterPlan:
@@ -3028,6 +3029,8 @@ def adapter_plan(ids: torch.Tensor, adapters: int) -> AdapterPlan:
         raise KernelError("adapter_plan: ids must be a contiguous int32 vector")
     if adapters < 0:
         raise KernelError(f"adapter_plan: {adapters} adapters")
+    if ids.shape[0] > ADAPTER_MAX_ROWS:
+        raise KernelError(f"adapter_plan: {ids.shape[0]} rows, at most {ADAPTER_MAX_ROWS}")
     _same_device("adapter_plan", ids)
     plan = AdapterPlan(ids, int(adapters))
     if plan.rows > ADAPTER_FEW_ROWS:

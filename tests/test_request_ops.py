@@ -69,6 +69,8 @@ def test_adapter_plan_refuses():
         ops.adapter_plan(torch.zeros(3, dtype=I), -1)
     with pytest.raises(ops.KernelError, match="CUDA tensors only"):
         ops.adapter_plan(torch.zeros(3, dtype=I), 2)
+    with pytest.raises(ops.KernelError, match="at most 8000000"):
+        ops.adapter_plan(torch.zeros(8_000_001, dtype=I), 2)
 
 
 B, V, W = 3, 100, 4
