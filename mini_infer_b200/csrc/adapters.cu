@@ -322,10 +322,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) adapter_sums_kernel(const Ada
 // KG: groups of 32 k whose operands are loaded ahead (0: none, ranks above 64).  The rests of the sums ride along: with up to 16 k (FOLD) they
 // stand in the place of 16 more, else a product takes four rows and their rests, and an item of more than four rows takes two.
 //
-// The tiles of all items are cut evenly among as many blocks as the chip holds, so that none has more than another, whatever the
-// items are: 128 rows, 24 adapters, 4096 x 28672: ranks to 64 31.7 us, with blocks of 2048 columns of an item 42.1; rank 16 22.1 and
+// The tiles of all items are shared out over as many blocks as the chip holds, so that hardly one has more than another, whatever the
+// items are: 128 rows, 24 adapters, 4096 x 28672: ranks to 64 31.3 us, with blocks of 2048 columns of an item 42.1; rank 16 21.3 and
 // 22.6.  BLOCKS of an SM: two, which leaves a thread 128 registers (one row at 4096 x 6144 6.4 us, with three 7.8); three for ranks
-// 17 to 32 (96 rows, 32 adapters, 4096 x 28672 30.6 and 32.6).
+// 17 to 32 (96 rows, 32 adapters, 4096 x 28672 30.6 and 32.6).  Columns for two tiles ahead instead of one made no difference.
 template <int KG, bool FOLD, int BLOCKS>
 __global__ void __launch_bounds__(TILE_THREADS, BLOCKS) adapter_add_kernel(const AdapterArgs g) {
   extern __shared__ __align__(16) unsigned char add_smem[];
@@ -344,9 +344,19 @@ __global__ void __launch_bounds__(TILE_THREADS, BLOCKS) adapter_add_kernel(const
     t0 = blockIdx.y * g.tiles + min(g.tiles, (int)blockIdx.x * PLAN_TILES);
     t1 = blockIdx.y * g.tiles + min(g.tiles, (int)(blockIdx.x + 1) * PLAN_TILES);
   } else {
+    // Whole items in equal pieces, where that makes no block longer by more than a tile, else the same number of tiles for all: another
+    // item costs a block a look-up, its sums and a barrier (64 rows, 24 adapters of rank 16 at 4096 x 6144: 11.6 us, 12.5 when blocks
+    // take equal numbers always; rank 64 at 4096 x 28672 30.4 and 31.5).
     const long long all = (long long)items * g.tiles;
-    t0 = (int)(all * blockIdx.x / gridDim.x);
-    t1 = (int)(all * (blockIdx.x + 1) / gridDim.x);
+    const int blocks = (int)gridDim.x, pieces = max(1, min(g.tiles, blocks / items)), longest = (g.tiles + pieces - 1) / pieces;
+    if (items <= blocks && longest <= (int)((all + blocks - 1) / blocks) + 1) {
+      const int index = (int)blockIdx.x / pieces, piece = (int)blockIdx.x - index * pieces, first = min(index, items) * g.tiles;
+      t0 = first + (index < items ? (int)((long long)g.tiles * piece / pieces) : 0);
+      t1 = first + (index < items ? (int)((long long)g.tiles * (piece + 1) / pieces) : 0);
+    } else {
+      t0 = (int)(all * blockIdx.x / blocks);
+      t1 = (int)(all * (blockIdx.x + 1) / blocks);
+    }
   }
 
   const int t8 = (FOLD ? t & 1 : t) * 8;
@@ -662,8 +672,8 @@ __global__ void __launch_bounds__(TILE_THREADS) adapter_add_plain_kernel(const A
 #define TC_ROWS 128
 #define TC_ATOM (TC_ROWS * 128)      // bytes of 128 rows of 64 k
 #define SUMS_MAX_STAGES 4
-#define ADD_COLS 128                 // columns of a tile of the result
-#define ADD_MAX_STAGES 4
+#define A1_COLS 128                 // columns of a tile of the result
+#define A1_MAX_STAGES 4
 
 __device__ __forceinline__ void copy_piece(uint32_t to, const void* from, int bytes) {      // the rest of 16 bytes: zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -891,7 +901,7 @@ __global__ void __launch_bounds__(256) adapter_held_kernel(const AdapterArgs g) 
 // Shared memory of the second product: the item's sums, then stages of B and of y
 __host__ __device__ inline int sums_atoms(int R) { return (held_sums(R) + 63) / 64; }      // a part's sums and rests
 __host__ __device__ inline int b_atoms(int R) { return (padded_rank(R) + 63) / 64; }
-__host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_ATOM + TC_ROWS * ADD_COLS * 2; }
+__host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_ATOM + TC_ROWS * A1_COLS * 2; }
 
 // The second product and the sum with y, in tiles of 128 columns.  One block per SM takes an equal stretch of all items' tiles; its warps
 // have parts of their own and meet at mbarriers alone, so that copies, products and sums of different tiles run side by side:
@@ -909,17 +919,17 @@ __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_A
 //
 // Copies gather (rows of an item lie anywhere), which a tensor map does not; a copy warp says that a tile is there once its own
 // copies have landed and are visible to the tensor cores.
-#define ADD_SUM_WARPS 8
-#define ADD_COPY_WARPS 4
-#define ADD_COPY_THREADS (32 * ADD_COPY_WARPS)
-#define ADD_THREADS (32 * (ADD_SUM_WARPS + ADD_COPY_WARPS + 1))
+#define A1_SUM_WARPS 8
+#define A1_COPY_WARPS 4
+#define A1_COPY_THREADS (32 * A1_COPY_WARPS)
+#define A1_THREADS (32 * (A1_SUM_WARPS + A1_COPY_WARPS + 1))
 
-#define ADD_ITEMS 64                 // items that a block looks up ahead
+#define A1_ITEMS 64                 // items that a block looks up ahead
 
 struct AddBlock {
-  int4 items[ADD_ITEMS];                                     // the first items, their rank instead of the last number
+  int4 items[A1_ITEMS];                                     // the first items, their rank instead of the last number
   int n_items;
-  uint64_t full[ADD_MAX_STAGES], empty[ADD_MAX_STAGES];      // a stage is there; the summing warps are through with it
+  uint64_t full[A1_MAX_STAGES], empty[A1_MAX_STAGES];      // a stage is there; the summing warps are through with it
   uint64_t done[2], free_[2];                                // a buffer's products have ended; it has been read
   uint64_t h_free;                                           // the products that read an item's sums have ended
   uint32_t tmem;
@@ -936,8 +946,8 @@ __device__ __forceinline__ void for_tiles(const AdapterArgs& g, const AddBlock& 
   int count = 0;
   for (int t = t0; t < t1;) {
     const int index = t / per_item, end = min(t1, (index + 1) * per_item);
-    const int4 item = index < ADD_ITEMS ? s.items[index] : __ldcg(g.items + index);
-    const int rank = index < ADD_ITEMS ? item.w : rank_of(g, item.x);
+    const int4 item = index < A1_ITEMS ? s.items[index] : __ldcg(g.items + index);
+    const int rank = index < A1_ITEMS ? item.w : rank_of(g, item.x);
     if (rank > 0 || g.out != g.y) {
       for (int u = t; u < end; ++u)
         if (!f(count++, item, rank, u == t, u + 1 == end, u - index * per_item)) return;
@@ -947,7 +957,7 @@ __device__ __forceinline__ void for_tiles(const AdapterArgs& g, const AddBlock& 
 }
 
 template <int STAGES, bool PAIRS>
-__global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const AdapterArgs g) {
+__global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const AdapterArgs g) {
   extern __shared__ unsigned char tc_smem[];
   __shared__ AddBlock s;
   // (The kernel in front, which holds the sums, started this one once the first product's had ended: everything that was before that
@@ -956,23 +966,23 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = g.R;
   const int np = PAIRS ? 2 : 1, rp = padded_rank(R), ha = sums_atoms(R), ba = b_atoms(R);
   const uint32_t h_at = base, stages_at = base + np * ha * TC_ATOM, stage_bytes = add_stage_bytes(R);
-  if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) {
+  if (warp == A1_SUM_WARPS + A1_COPY_WARPS) {
     if (lane == 0) {
       for (int i = 0; i < STAGES; ++i) {
-        mbar_init(&s.full[i], ADD_COPY_THREADS);
-        mbar_init(&s.empty[i], ADD_SUM_WARPS);
+        mbar_init(&s.full[i], A1_COPY_THREADS);
+        mbar_init(&s.empty[i], A1_SUM_WARPS);
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s.done[i], 1);
-        mbar_init(&s.free_[i], ADD_SUM_WARPS);
+        mbar_init(&s.free_[i], A1_SUM_WARPS);
       }
       mbar_init(&s.h_free, 1);
       s.give_up = 0;
       asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     __syncwarp();
-    tc_alloc(&s.tmem, 2 * ADD_COLS);
-  } else if (tid < ADD_ITEMS) {
+    tc_alloc(&s.tmem, 2 * A1_COLS);
+  } else if (tid < A1_ITEMS) {
     int4 item = __ldcg(g.items + min(tid, g.max_items - 1));
     if (tid == 0) s.n_items = __ldcg(&g.items[g.max_items].x);
     item.w = rank_of(g, item.x);
@@ -986,15 +996,15 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
   const bf16* y = (const bf16*)g.y;
   bf16* out = (bf16*)g.out;
 
-  if (warp >= ADD_SUM_WARPS && warp < ADD_SUM_WARPS + ADD_COPY_WARPS) {
+  if (warp >= A1_SUM_WARPS && warp < A1_SUM_WARPS + A1_COPY_WARPS) {
     // ---- copies.  Pieces of a row by as many threads, rounded up to a power of two
     constexpr int LAG = STAGES > 2 ? STAGES - 2 : 0;          // tiles under way behind the one just asked for
-    const int ct = tid - 32 * ADD_SUM_WARPS;
+    const int ct = tid - 32 * A1_SUM_WARPS;
     const int hp = held_sums(R), h_pieces = hp / 8, b_pieces = rp / 8, b_shift = b_pieces <= 2 ? 1 : b_pieces <= 4 ? 2 : b_pieces <= 8 ? 3 : 4;
-    const int bq = ct & ((1 << b_shift) - 1), b_col = ct >> b_shift, b_step = ADD_COPY_THREADS >> b_shift;
-    const int h_shift = b_shift + with_rests(R), hq = ct & ((1 << h_shift) - 1), h_row = ct >> h_shift, h_step = ADD_COPY_THREADS >> h_shift;
+    const int bq = ct & ((1 << b_shift) - 1), b_col = ct >> b_shift, b_step = A1_COPY_THREADS >> b_shift;
+    const int h_shift = b_shift + with_rests(R), hq = ct & ((1 << h_shift) - 1), h_row = ct >> h_shift, h_step = A1_COPY_THREADS >> h_shift;
     const int yq = ct & 15, yr = ct >> 4;                     // piece `yq` of every 8th row
-    constexpr int YN = TC_ROWS * 16 / ADD_COPY_THREADS;
+    constexpr int YN = TC_ROWS * 16 / A1_COPY_THREADS;
     const uint32_t y_row = ba * TC_ATOM + yr * 256, y_place[2] = {y_row + ((yq ^ yr) << 4), y_row + ((yq ^ (yr + 8)) << 4)};
     const uint32_t b_place = bq / 8 * TC_ATOM + b_col * 128 + (((bq & 7) ^ (b_col & 7)) << 4);
     const int b_stride = (PAIRS ? 2 : 1) * b_step * R;      // elements between a thread's columns
@@ -1021,7 +1031,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
       }
       if (j >= STAGES && !mbar_wait(&s.empty[stage], (j / STAGES - 1) & 1, &s.give_up)) return false;
       int part, c, c_end;
-      find_chunk(g, chunk, ADD_COLS, part, c, c_end);
+      find_chunk(g, chunk, A1_COLS, part, c, c_end);
       if (rank > 0 && bq < b_pieces) {
         // rows of B: the tile's columns, of pairs the first ones and then the second ones
         const int there = 2 * max(0, min(8, rank - bq * 8));
@@ -1031,7 +1041,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
           const int first = PAIRS ? c + 2 * b_col + half : c + half * 64 + b_col;
           const bf16* from = b + (size_t)first * R;
           uint32_t at = to + b_place + half * (TC_ATOM / 2);
-          if (c + ADD_COLS <= c_end && there == 16) {
+          if (c + A1_COLS <= c_end && there == 16) {
             for (int col = b_col; col < 64; col += b_step, from += b_stride, at += b_step * 128) copy_piece(at, from, 16);
           } else {
             int column = first;
@@ -1076,10 +1086,10 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
     copies_wait<0>();
     tell(asked);
     mi_pdl_wait();
-  } else if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) {
+  } else if (warp == A1_SUM_WARPS + A1_COPY_WARPS) {
     // ---- products
     if (lane == 0) {
-      const uint32_t desc = product_desc(PAIRS ? ADD_COLS / 2 : ADD_COLS);
+      const uint32_t desc = product_desc(PAIRS ? A1_COLS / 2 : A1_COLS);
       const int rests = with_rests(R);
       for_tiles(g, s, [&](int j, const int4&, int rank, bool, bool ends, int chunk) {
         const int stage = j % STAGES, buf = j & 1;
@@ -1092,14 +1102,14 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
             const uint64_t bd = operand_desc(at + p * 64 * 128 + k / 64 * TC_ATOM + k % 64 * 2);
             for (int lo = 0; lo <= rests; ++lo) {
               const int e = k + lo * rp;
-              tc_mma(tmem + buf * ADD_COLS + p * 64, operand_desc(h_at + (p * ha + e / 64) * TC_ATOM + e % 64 * 2), bd, desc, k > 0 || lo > 0);
+              tc_mma(tmem + buf * A1_COLS + p * 64, operand_desc(h_at + (p * ha + e / 64) * TC_ATOM + e % 64 * 2), bd, desc, k > 0 || lo > 0);
             }
           }
         tc_commit(&s.done[buf]);
         int part, next, c, c_end;
-        find_chunk(g, chunk, ADD_COLS, part, c, c_end);
+        find_chunk(g, chunk, A1_COLS, part, c, c_end);
         next = part;
-        if (!ends) find_chunk(g, chunk + 1, ADD_COLS, next, c, c_end);
+        if (!ends) find_chunk(g, chunk + 1, A1_COLS, next, c, c_end);
         if ((ends || next != part) && rank > 0) tc_commit(&s.h_free);
         return true;
       });
@@ -1124,14 +1134,14 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
           }
       }
       int part, c, c_end;
-      find_chunk(g, chunk, ADD_COLS, part, c, c_end);
+      find_chunk(g, chunk, A1_COLS, part, c, c_end);
       const uint32_t y_at = stages_at + stage * stage_bytes + ba * TC_ATOM;
       const bool there = mbar_wait(&s.full[stage], (j / STAGES) & 1, &s.give_up) && mbar_wait(&s.done[buf], (j / 2) & 1, &s.give_up);
       if (!__all_sync(0xffffffffu, there)) return false;
       if (rank > 0) {
         // 32 columns at a time, the next ones on their way meanwhile (a row behind the item's last is added up too, and not written)
         uint32_t v[2][32];
-        const uint32_t from = lanes + buf * ADD_COLS, y_row = y_at + row * 256, turn = row & 15;
+        const uint32_t from = lanes + buf * A1_COLS, y_row = y_at + row * 256, turn = row & 15;
         const auto fetch = [&](int o) {
           tc_load16(from + (PAIRS ? o * 16 : o * 32), v[o]);
           tc_load16(from + (PAIRS ? 64 + o * 16 : o * 32 + 16), v[o] + 16);
@@ -1200,7 +1210,7 @@ __global__ void __launch_bounds__(ADD_THREADS, 1) adapter_add_tc_kernel(const Ad
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == ADD_SUM_WARPS + ADD_COPY_WARPS) tc_free(tmem, 2 * ADD_COLS);
+  if (warp == A1_SUM_WARPS + A1_COPY_WARPS) tc_free(tmem, 2 * A1_COLS);
 }
 
 // ---- the plan: rows in the order of their adapters, and items of up to MAX_ROWS of them
@@ -1333,12 +1343,15 @@ static cudaError_t launch_few(const AdapterArgs& g, int max_items, cudaStream_t 
   cudaError_t e = MI_LAUNCH((adapter_sums_kernel), (unsigned)(g.items || jobs < SUM_BLOCKS ? jobs : SUM_BLOCKS), TILE_THREADS, 0, stream, g);
   if (e != cudaSuccess) return e;
   const size_t bytes = (size_t)(g.pairs ? 2 : 1) * 2 * FEW_ROWS * h_stride(g.R) * 2;
-  // as many blocks as the chip holds, and no more than there are tiles
+  // As many blocks as the chip holds, and no more than there are tiles; or as many as it holds beside the first kernel's, where that makes a
+  // block's way a tile longer at most: those are under way when the sums come, the others begin then (8 rows, 8 adapters of rank 16
+  // at 4096 x 28672: 9.2 us, with all 296 blocks 11.0).
   const auto run = [&](auto kernel, int blocks, bool* allowed) {
     const cudaError_t e = allow_smem(kernel, bytes, allowed);
     if (e != cudaSuccess) return e;
-    const long long most = (long long)max_items * g.tiles;
-    const dim3 grid = g.items ? dim3((g.tiles + PLAN_TILES - 1) / PLAN_TILES, max_items) : dim3((unsigned)(most < blocks * 148 ? most : blocks * 148));
+    const long long most = (long long)max_items * g.tiles, all = blocks * 148, beside = all - (jobs < SUM_BLOCKS ? jobs : SUM_BLOCKS);
+    const long long room = beside > 0 && (most + beside - 1) / beside <= (most + all - 1) / all + 1 ? beside : all;
+    const dim3 grid = g.items ? dim3((g.tiles + PLAN_TILES - 1) / PLAN_TILES, max_items) : dim3((unsigned)(most < room ? most : room));
     return MI_LAUNCH((kernel), grid, TILE_THREADS, bytes, stream, g);
   };
   if (g.R <= 16) return run(adapter_add_kernel<1, true, 2>, 2, allowed[0]);
@@ -1364,7 +1377,7 @@ static cudaError_t launch_plain(const AdapterArgs& g, int max_items, cudaStream_
 static int add_tc_stages(int R, int pairs) {      // (of 227 KB 1 is for the alignment and up to 2 are AddBlock's)
   const int left = 224 * 1024 - (pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM;
   const int n = left / add_stage_bytes(R);
-  return n > ADD_MAX_STAGES ? ADD_MAX_STAGES : n;
+  return n > A1_MAX_STAGES ? A1_MAX_STAGES : n;
 }
 
 static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t stream) {
@@ -1388,7 +1401,7 @@ static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t
   const int grid = tiles < 148 ? (int)tiles : 148;
   const auto run = [&](auto kernel, bool* room) {
     const cudaError_t e = allow_smem(kernel, bytes, room);
-    return e != cudaSuccess ? e : MI_LAUNCH((kernel), grid, ADD_THREADS, bytes, stream, g);
+    return e != cudaSuccess ? e : MI_LAUNCH((kernel), grid, A1_THREADS, bytes, stream, g);
   };
   if (g.pairs) return stages == 4 ? run(adapter_add_tc_kernel<4, true>, allowed[1]) : run(adapter_add_tc_kernel<2, true>, allowed[2]);
   return stages == 4 ? run(adapter_add_tc_kernel<4, false>, allowed[3]) : run(adapter_add_tc_kernel<3, false>, allowed[4]);
@@ -1494,7 +1507,7 @@ extern "C" int mi_adapter_add(const AdapterCall* call, float* h, cudaStream_t st
   g.ks = r.ks;
   if (r.way != BY_ELEMENTS) {
     g.max_items = r.items;
-    g.tiles = count_chunks(g, r.way == BY_MANY ? ADD_COLS : TILE_COLS);
+    g.tiles = count_chunks(g, r.way == BY_MANY ? A1_COLS : TILE_COLS);
     if ((long long)r.items * g.tiles > 0x7fffffffLL) MI_REFUSE("adapter_add: %d rows of %d columns", M, N);
     g.held = (bf16*)(h + r.floats);
     bool starts4 = true;
