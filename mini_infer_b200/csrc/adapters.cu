@@ -132,7 +132,7 @@ inline int count_chunks(const AdapterArgs& g, int size) {
 
 // Items are up to 8 rows that share an adapter (or have none).  For up to FEW_MAX rows, one to a thread, every block finds the items in the
 // ids; for more, adapter_plan has put the rows in order.  256 rows without a plan and with one, on tcgen05 (us): 32 adapters of rank
-// 16 at 4096 x 6144 17.4 and 39.7, 4 of them 16.9 and 22.4, 4 of rank 64 at 4096 x 28672 37.3 and 40.4.
+// 16 at 4096 x 6144 17.5 and 39.7, 4 of them 17.2 and 22.4, 4 of rank 64 at 4096 x 28672 37.8 and 40.4.
 
 #define TILE_THREADS 256
 #define TILE_WARPS (TILE_THREADS / 32)
