@@ -12,7 +12,7 @@
 
 MI_DEFINE_ERROR_API()
 
-#define ADJUST_THREADS 256
+#define ADJUST_THREADS 128
 #define ADJUST_GROUPS 8                         // groups of 4 columns of a lane: a word of bits per lane, in other order
 #define ADJUST_WARP_COLS (32 * ADJUST_GROUPS * 4)
 
@@ -42,9 +42,9 @@ struct AdjustArgs {
 // bits and a store.  A row that starts off a 16-byte boundary is taken from its first boundary on; the up to three columns in front
 // are the first warp's.  In place, columns that do not change are neither read nor written.
 //
-// 256 rows of 128256 with histories of up to 1000 tokens and 100 biases each, out of place: 52 us, 5.0 TB/s (a thread per column
-// with its bits and count 130 us); histories of 500 tokens alone 48 us, and in place 15; 16 rows with histories of up to 1500 6.4 us; one
-// row of 32000 with everything 3.7 us, which is launch and latency.
+// 256 rows of 128256 with histories of up to 1000 tokens and 100 biases each, out of place: 49 us, 5.4 TB/s (a thread per column
+// with its bits and count 130 us); 16 rows with histories of up to 1500 5.7 us; one row of 32000 with everything 3.5 us, which is
+// launch and latency.  Blocks of four warps: of eight, whose rows and tails share out worse, 53, 6.4 and 3.7 us.
 template <bool IN_PLACE>
 __global__ void __launch_bounds__(ADJUST_THREADS) adjust_logits_kernel(const AdjustArgs a) {
   mi_pdl_enter();   // the logits and the histories come from the kernels before this one
