@@ -45,7 +45,7 @@ struct AdapterArgs {
 // way from the ids to the rows.  Three ways, by rows and types:
 //
 //   few rows (up to FEW_MAX, bfloat16)   mma.sync, blocks find their rows themselves: 6.4 us for a row of rank 16 at 4096 x 6144
-//   many rows (bfloat16)                 a plan, tcgen05: 213 us for 8192 rows of ranks to 64 at 4096 x 28672 (155 at the rate of a copy)
+//   many rows (bfloat16)                 a plan, tcgen05: 219 us for 8192 rows of ranks to 64 at 4096 x 28672 (155 at the rate of a copy)
 //   float32, and what is not in pieces of 16 bytes   CUDA cores
 //
 // ---------------------------------------------------------------------------------------------- few rows, bfloat16
@@ -695,6 +695,12 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint3
                "l"(a), "l"(b), "r"(desc), "r"(accumulate)
                : "memory");
 }
+// the same with the first operand in tensor memory: row i in lane i, two of k a column
+__device__ __forceinline__ void tc_mma_held(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+               "r"(a), "l"(b), "r"(desc), "r"(accumulate)
+               : "memory");
+}
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -721,6 +727,14 @@ __device__ __forceinline__ void tc_load16(uint32_t from, uint32_t* r) {
       : "r"(from)
       : "memory");
 }
+__device__ __forceinline__ void tc_store16(uint32_t to, const uint4 (&v)[4]) {      // 16 columns of this thread's row
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(to),
+      "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w), "r"(v[2].x), "r"(v[2].y),
+      "r"(v[2].z), "r"(v[2].w), "r"(v[3].x), "r"(v[3].y), "r"(v[3].z), "r"(v[3].w)
+      : "memory");
+}
+__device__ __forceinline__ void tc_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 
 // Tensor memory for a block, by its first warp; the address is in `holder` behind a barrier of the block.  Only then may the next kernel's
@@ -856,16 +870,14 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_sums_tc_kernel(const Adapt
   if (tid < 32) tc_free(s.tmem, 128);
 }
 
-// A part's sums for the second product: whole groups of 16 k, and behind them their rests for ranks up to 32, where they cost
-// little (2048 rows of rank 16 at 4096 x 4096 35.3 us, without them 34.3).  Beyond, a sum is rounded to bfloat16 once (off by up
-// to 2^-8 of it, as much as the rounding of the result): with the rests the products double and a stage of the ring goes, and 8192 rows
-// of ranks to 64 at 4096 x 28672 take 289 us instead of 252, at 4096 x 6144 138 instead of 120.
+// A part's sums for the second product, two bfloat16 numbers each as with few rows: whole groups of 16 k, and behind them their rests.
+// In tensor memory they cost no stage of the ring, and the products, twice as many, hide behind the tiles' bytes: 8192 rows of ranks to
+// 64 at 4096 x 28672 219 us, with one number a sum 214, at 4096 x 6144 106 and 105.
 __host__ __device__ inline int padded_rank(int R) { return (R + 15) & ~15; }
-__host__ __device__ inline int with_rests(int R) { return R <= 32; }
-__host__ __device__ inline int held_sums(int R) { return (with_rests(R) ? 2 : 1) * padded_rank(R); }
+__host__ __device__ inline int held_sums(int R) { return 2 * padded_rank(R); }
 
-// The sums over all of K, scaled, in bfloat16: four sums a thread.  A kernel of its own, since the second product gathers them with
-// cp.async as often as an item's tiles are shared out; some 3 us, hidden in part by that kernel's start.
+// The sums over all of K, scaled and split: four sums a thread.  A kernel of its own, since the second product reads them as often as
+// an item's tiles are shared out; some 3 us, hidden in part by that kernel's start.
 __global__ void __launch_bounds__(256) adapter_held_kernel(const AdapterArgs g) {
   mi_pdl_wait();
   mi_pdl_launch_dependents();
@@ -895,18 +907,18 @@ __global__ void __launch_bounds__(256) adapter_held_kernel(const AdapterArgs g) 
   for (int q = 0; q < 4; ++q) split_bf16(r + q < rank ? f[q] * scale : 0.f, hi[q], lo[q]);
   bf16* to = g.held + ((size_t)row * g.P + p) * held_sums(g.R) + r;
   *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
-  if (with_rests(g.R)) *reinterpret_cast<uint2*>(to + rp) = *reinterpret_cast<uint2*>(lo);
+  *reinterpret_cast<uint2*>(to + rp) = *reinterpret_cast<uint2*>(lo);
 }
 
-// Shared memory of the second product: the item's sums, then stages of B and of y
-__host__ __device__ inline int sums_atoms(int R) { return (held_sums(R) + 63) / 64; }      // a part's sums and rests
+// Shared memory of the second product: stages of B and of y
 __host__ __device__ inline int b_atoms(int R) { return (padded_rank(R) + 63) / 64; }
 __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_ATOM + TC_ROWS * A1_COLS * 2; }
 
 // The second product and the sum with y, in tiles of 128 columns.  One block per SM takes an equal stretch of all items' tiles; its warps
 // have parts of their own and meet at mbarriers alone, so that copies, products and sums of different tiles run side by side:
 //
-//   four copy warps      bring B and y of a tile into a ring of stages, and an item's sums when it begins;
+//   four copy warps      bring B and y of a tile into a ring of stages, and an item's sums into tensor memory when it begins (a
+//                        thread has a row);
 //   one thread           issues a tile's products into one of two buffers in tensor memory;
 //   eight summing warps  add a buffer to y in shared memory (a thread has a row) and write the result (a lane has pieces of
 //                        rows).  y lies in rows of 256 bytes, 16-byte pieces permuted by the row, so that both ways touch all banks.
@@ -925,6 +937,10 @@ __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_A
 #define A1_THREADS (32 * (A1_SUM_WARPS + A1_COPY_WARPS + 1))
 
 #define A1_ITEMS 64                 // items that a block looks up ahead
+// Tensor memory: two buffers of a tile's sums, and behind them the first operand, a column for two of a row's sums and rests: at most two
+// parts of rank 128.
+#define A1_TMEM 512
+#define A1_HELD (2 * A1_COLS)
 
 struct AddBlock {
   int4 items[A1_ITEMS];                                     // the first items, their rank instead of the last number
@@ -964,8 +980,8 @@ __global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const Ada
   // is there, tensor memory is nobody's any more, and the copy warps alone wait, before they take the sums.)
   const uint32_t base = (smem_u32(tc_smem) + 1023) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = g.R;
-  const int np = PAIRS ? 2 : 1, rp = padded_rank(R), ha = sums_atoms(R), ba = b_atoms(R);
-  const uint32_t h_at = base, stages_at = base + np * ha * TC_ATOM, stage_bytes = add_stage_bytes(R);
+  const int np = PAIRS ? 2 : 1, rp = padded_rank(R), ba = b_atoms(R);
+  const uint32_t stages_at = base, stage_bytes = add_stage_bytes(R);
   if (warp == A1_SUM_WARPS + A1_COPY_WARPS) {
     if (lane == 0) {
       for (int i = 0; i < STAGES; ++i) {
@@ -981,7 +997,7 @@ __global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const Ada
       asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     __syncwarp();
-    tc_alloc(&s.tmem, 2 * A1_COLS);
+    tc_alloc(&s.tmem, A1_TMEM);
   } else if (tid < A1_ITEMS) {
     int4 item = __ldcg(g.items + min(tid, g.max_items - 1));
     if (tid == 0) s.n_items = __ldcg(&g.items[g.max_items].x);
@@ -998,11 +1014,10 @@ __global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const Ada
 
   if (warp >= A1_SUM_WARPS && warp < A1_SUM_WARPS + A1_COPY_WARPS) {
     // ---- copies.  Pieces of a row by as many threads, rounded up to a power of two
-    constexpr int LAG = STAGES > 2 ? STAGES - 2 : 0;          // tiles under way behind the one just asked for
+    constexpr int LAG = STAGES - 2;                           // tiles under way behind the one just asked for
     const int ct = tid - 32 * A1_SUM_WARPS;
-    const int hp = held_sums(R), h_pieces = hp / 8, b_pieces = rp / 8, b_shift = b_pieces <= 2 ? 1 : b_pieces <= 4 ? 2 : b_pieces <= 8 ? 3 : 4;
+    const int b_pieces = rp / 8, b_shift = b_pieces <= 2 ? 1 : b_pieces <= 4 ? 2 : b_pieces <= 8 ? 3 : 4;
     const int bq = ct & ((1 << b_shift) - 1), b_col = ct >> b_shift, b_step = A1_COPY_THREADS >> b_shift;
-    const int h_shift = b_shift + with_rests(R), hq = ct & ((1 << h_shift) - 1), h_row = ct >> h_shift, h_step = A1_COPY_THREADS >> h_shift;
     const int yq = ct & 15, yr = ct >> 4;                     // piece `yq` of every 8th row
     constexpr int YN = TC_ROWS * 16 / A1_COPY_THREADS;
     const uint32_t y_row = ba * TC_ATOM + yr * 256, y_place[2] = {y_row + ((yq ^ yr) << 4), y_row + ((yq ^ (yr + 8)) << 4)};
@@ -1029,7 +1044,7 @@ __global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const Ada
           }
         }
       }
-      if (j >= STAGES && !mbar_wait(&s.empty[stage], (j / STAGES - 1) & 1, &s.give_up)) return false;
+      if (j >= STAGES && !__all_sync(0xffffffffu, mbar_wait(&s.empty[stage], (j / STAGES - 1) & 1, &s.give_up))) return false;
       int part, c, c_end;
       find_chunk(g, chunk, A1_COLS, part, c, c_end);
       if (rank > 0 && bq < b_pieces) {
@@ -1068,15 +1083,25 @@ __global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const Ada
         // the last item's products have to end first, and for that to be told of all their tiles
         copies_wait<1>();
         tell(j);
-        if (items > 0 && !mbar_wait(&s.h_free, (items - 1) & 1, &s.give_up)) return false;
+        if (items > 0 && !__all_sync(0xffffffffu, mbar_wait(&s.h_free, (items - 1) & 1, &s.give_up))) return false;
         if (items++ == 0) mi_pdl_wait();
-        if (hq < h_pieces)
-          for (int row = h_row; row < item.z; row += h_step) {
-            const bf16* from = g.held + (size_t)g.order[item.y + row] * g.P * hp + hq * 8;
-            for (int p = 0; p < np; ++p)
-              copy_piece(h_at + (p * ha + hq / 8) * TC_ATOM + row * 128 + (((hq & 7) ^ (row & 7)) << 4), from + (size_t)(part + p) * hp, 16);
-          }
-        copies_commit();                                      // (one group more than tiles: waits for tiles wait for no less)
+        tc_fence_after();
+        const int row = (warp & 3) * 32 + lane, columns = np * rp;      // (the parts of pairs lie side by side, here and there)
+        const uint32_t to_held = tmem + A1_HELD + ((uint32_t)(warp & 3) << 21);
+        const uint4* from = reinterpret_cast<const uint4*>(g.held + ((size_t)(row < item.z ? g.order[item.y + row] : 0) * g.P + part) * (2 * rp));
+        // A lane's pieces of a row follow one another, so that a sector of L2 serves two of its loads through L1 (past L1, 8192 rows
+        // of rank 64 at 4096 x 6144 take 118 us instead of 106).  8 loads under way at once: 16 would not leave registers.
+        for (int h0 = 0; h0 < columns; h0 += 32) {
+          uint4 v[2][4];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            v[i / 4][i % 4] = row < item.z && h0 + i / 4 * 16 < columns ? from[h0 / 4 + i] : zero4();
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (h0 + i * 16 < columns) tc_store16(to_held + h0 + i * 16, v[i]);
+        }
+        tc_store_wait();
+        tc_fence_before();
       }
       asked = j + 1;
       copies_wait<LAG>();
@@ -1090,7 +1115,6 @@ __global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const Ada
     // ---- products
     if (lane == 0) {
       const uint32_t desc = product_desc(PAIRS ? A1_COLS / 2 : A1_COLS);
-      const int rests = with_rests(R);
       for_tiles(g, s, [&](int j, const int4&, int rank, bool, bool ends, int chunk) {
         const int stage = j % STAGES, buf = j & 1;
         if (!mbar_wait(&s.full[stage], (j / STAGES) & 1, &s.give_up)) return false;
@@ -1100,10 +1124,8 @@ __global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const Ada
         for (int p = 0; p < np && rank > 0; ++p)
           for (int k = 0; k < rp; k += 16) {
             const uint64_t bd = operand_desc(at + p * 64 * 128 + k / 64 * TC_ATOM + k % 64 * 2);
-            for (int lo = 0; lo <= rests; ++lo) {
-              const int e = k + lo * rp;
-              tc_mma(tmem + buf * A1_COLS + p * 64, operand_desc(h_at + (p * ha + e / 64) * TC_ATOM + e % 64 * 2), bd, desc, k > 0 || lo > 0);
-            }
+            for (int lo = 0; lo < 2; ++lo)
+              tc_mma_held(tmem + buf * A1_COLS + p * 64, tmem + A1_HELD + p * rp + (k + lo * rp) / 2, bd, desc, k > 0 || lo > 0);
           }
         tc_commit(&s.done[buf]);
         int part, next, c, c_end;
@@ -1210,7 +1232,7 @@ __global__ void __launch_bounds__(A1_THREADS, 1) adapter_add_tc_kernel(const Ada
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == A1_SUM_WARPS + A1_COPY_WARPS) tc_free(tmem, 2 * A1_COLS);
+  if (warp == A1_SUM_WARPS + A1_COPY_WARPS) tc_free(tmem, A1_TMEM);
 }
 
 // ---- the plan: rows in the order of their adapters, and items of up to MAX_ROWS of them
@@ -1373,10 +1395,9 @@ static cudaError_t launch_plain(const AdapterArgs& g, int max_items, cudaStream_
   return MI_LAUNCH((adapter_add_plain_kernel<T, VEC>), dim3(count_chunks(g, g.span), max_items), TILE_THREADS, bytes, stream, g);
 }
 
-// Stages that fit beside the sums: four up to rank 64, three up to 128 (two of pairs).
-static int add_tc_stages(int R, int pairs) {      // (of 227 KB 1 is for the alignment and up to 2 are AddBlock's)
-  const int left = 224 * 1024 - (pairs ? 2 : 1) * sums_atoms(R) * TC_ATOM;
-  const int n = left / add_stage_bytes(R);
+// Stages that fit: four up to rank 64, three up to 128.
+static int add_tc_stages(int R) {      // (of 227 KB 1 is for the alignment and up to 2 are AddBlock's)
+  const int n = 224 * 1024 / add_stage_bytes(R);
   return n > A1_MAX_STAGES ? A1_MAX_STAGES : n;
 }
 
@@ -1395,15 +1416,15 @@ static cudaError_t launch_many(const AdapterArgs& g, int max_items, cudaStream_t
   const long long quarters = (long long)g.M * g.P * (padded_rank(g.R) / 4);
   e = MI_LAUNCH((adapter_held_kernel), (unsigned)((quarters + 255) / 256), 256, 0, stream, g);
   if (e != cudaSuccess) return e;
-  const int stages = add_tc_stages(g.R, g.pairs);
-  const size_t bytes = (size_t)(g.pairs ? 2 : 1) * sums_atoms(g.R) * TC_ATOM + (size_t)stages * add_stage_bytes(g.R) + 1024;
+  const int stages = add_tc_stages(g.R);
+  const size_t bytes = (size_t)stages * add_stage_bytes(g.R) + 1024;
   const long long tiles = (long long)max_items * g.tiles;
   const int grid = tiles < 148 ? (int)tiles : 148;
   const auto run = [&](auto kernel, bool* room) {
     const cudaError_t e = allow_smem(kernel, bytes, room);
     return e != cudaSuccess ? e : MI_LAUNCH((kernel), grid, A1_THREADS, bytes, stream, g);
   };
-  if (g.pairs) return stages == 4 ? run(adapter_add_tc_kernel<4, true>, allowed[1]) : run(adapter_add_tc_kernel<2, true>, allowed[2]);
+  if (g.pairs) return stages == 4 ? run(adapter_add_tc_kernel<4, true>, allowed[1]) : run(adapter_add_tc_kernel<3, true>, allowed[2]);
   return stages == 4 ? run(adapter_add_tc_kernel<4, false>, allowed[3]) : run(adapter_add_tc_kernel<3, false>, allowed[4]);
 }
 

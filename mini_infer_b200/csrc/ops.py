@@ -3054,8 +3054,8 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
 
     ``a [adapters, P, R, K]``, ``b [adapters, N, R]``, contiguous and in the dtype of ``x`` and ``y`` (float32 or bfloat16), ranks to 3000.
     Sums are fp32 and the result is rounded once; in bfloat16 the sums over ``K`` enter the second product as two bfloat16 numbers
-    each (off by up to 2^-16 of them), and from rank 33 on with more than ``ADAPTER_FEW_ROWS`` rows as one (up to 2^-8).  Rows of
-    float32 have the same bits in whatever company; in bfloat16 the order of sums follows from the rows and adapters of the call.
+    each (off by up to 2^-16 of them).  Rows of float32 have the same bits in whatever company; in bfloat16 the order of sums
+    follows from the rows and adapters of the call.
     ``P`` projections may be merged along their columns: ``parts`` are their widths, side by
     side, at most four (default: one), or with ``pairs`` two of equal width that alternate column by column (gate 0, up 0,
     gate 1, ...).  A column of part ``p`` takes ``a[:, p]``.  ``ranks`` (int32): adapters whose rank is below ``R``; what lies
