@@ -10,7 +10,8 @@ from __future__ import annotations
 
 import os
 import threading
-from typing import Any, Mapping, Sequence
+from contextlib import contextmanager
+from typing import Any, Iterator, Mapping, Sequence
 
 import torch
 
@@ -68,6 +69,11 @@ class ModelRunner:
         self.block_size = block_size
         self._adapter_names: list[str | None] | None = None      # by index; None: adapters are off
         self._adapter_lock = threading.RLock()                   # names and users: requests come from any thread
+        # A step, which may be recorded as a graph, or work on the adapters' banks by another thread: one after the other on the
+        # host, and in that order on the device whatever streams the two are on.
+        self._device_lock = threading.RLock()
+        self._step_stream: torch.cuda.Stream | None = None       # of the last step since adapters are on
+        self._banks_written: torch.cuda.Event | None = None      # behind work on the banks that no step has waited for yet
 
     @classmethod
     def from_pretrained(cls, model_dir: str | os.PathLike, *, device="cuda:0", dtype="bfloat16",
@@ -117,6 +123,23 @@ class ModelRunner:
 
     # -- adapters -----------------------------------------------------------------------
 
+    @contextmanager
+    def _between_steps(self) -> Iterator[None]:
+        """Work on the adapters' banks: behind every step before it, and in front of every step behind it."""
+        with self._device_lock:
+            if self.device.type != "cuda":
+                yield
+                return
+            stream = torch.cuda.current_stream(self.device)
+            if self._step_stream is not None:
+                stream.wait_stream(self._step_stream)
+            if self._banks_written is not None:
+                stream.wait_event(self._banks_written)
+            try:
+                yield
+            finally:
+                self._banks_written = stream.record_event()
+
     def enable_adapters(self, count: int = 8, rank: int = 16) -> None:
         """Make room for ``count`` low-rank adapters of rank up to ``rank`` beside every product of the model that takes them
         (``Part.adapted``).  Once, before the first is loaded."""
@@ -133,12 +156,13 @@ class ModelRunner:
             parts = [p for p in self.model.all_parts() if p.adapted()]
             if not parts:
                 raise ValueError("no part of this model takes adapters")
-            for p in parts:
-                p.banks = {q.name: AdapterBank(q, count, held, self.dtype, self.device) for q in p.adapted()}
+            with self._between_steps():
+                for p in parts:
+                    p.banks = {q.name: AdapterBank(q, count, held, self.dtype, self.device) for q in p.adapted()}
+                self.stepper.adapter_count = count
             self._adapter_names = [None] * count
             self._adapter_users = [0] * count
             self._adapter_rank = rank
-            self.stepper.adapter_count = count
 
     def load_adapter(self, name: str, source, config: Mapping[str, Any] | None = None) -> int:
         """Load an adapter under ``name`` and return its index: ``source`` is a folder (``weights.read_adapter``), or the adapter's
@@ -175,7 +199,7 @@ class ModelRunner:
             if None not in self._adapter_names:
                 raise ValueError(f"all {len(self._adapter_names)} places for adapters are taken")
             index = self._adapter_names.index(None)
-            with torch.inference_mode():
+            with self._between_steps(), torch.inference_mode():
                 for p in self.model.all_parts():
                     for q in (p.adapted() if p.banks is not None else ()):
                         mine = {local: matrices[p.spec.tensor_name(local)] for local in q.tensors
@@ -190,7 +214,7 @@ class ModelRunner:
             index = self.adapter_index(name)
             if self._adapter_users[index]:
                 raise ValueError(f"adapter {name!r} is in use by {self._adapter_users[index]} requests")
-            with torch.inference_mode():
+            with self._between_steps(), torch.inference_mode():
                 for p in self.model.all_parts():
                     for bank in (p.banks or {}).values():
                         bank.clear(index)
@@ -224,7 +248,13 @@ class ModelRunner:
     device_token_feedback = True
 
     def step(self, entries: Sequence[StepEntry], device_tokens: torch.Tensor | None = None) -> StepResult:
-        return self.stepper.step(entries, device_tokens)
+        with self._device_lock:
+            if self.stepper.adapter_count and self.device.type == "cuda":
+                self._step_stream = torch.cuda.current_stream(self.device)
+                if self._banks_written is not None:
+                    self._step_stream.wait_event(self._banks_written)
+                    self._banks_written = None
+            return self.stepper.step(entries, device_tokens)
 
     def capture_decode_steps(self, max_batch: int) -> int:
         """Capture the decode step of every batch size up to ``max_batch`` that has no graph yet
@@ -250,7 +280,7 @@ class ModelRunner:
                     if not self.cache.can_append([(r, 1) for r in rids]):
                         return made
                     # runs kernel by kernel once, then records
-                    self.stepper.step([StepEntry(r, [0], [0], adapter) for r in rids])
+                    self.step([StepEntry(r, [0], [0], adapter) for r in rids])
                     made += 1
                 finally:
                     for r in rids:

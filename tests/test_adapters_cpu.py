@@ -1,0 +1,70 @@
+"""Adapters' places, names and files in a runner whose steps are a stand-in, without a GPU."""
+
+import threading
+
+import pytest
+import torch
+
+from adapter_util import random_adapter
+from mini_infer_b200.config.registry import load_config
+from mini_infer_b200.engine.runner import ModelRunner
+from mini_infer_b200.parts.adapters import AdapterBank
+from mini_infer_b200.parts.model import DecoderModel
+from mini_infer_b200.weights import bind_random, random_state_dict
+from tiny_configs import TINY
+
+
+def cpu_runner(raw):
+    arch, cfg = load_config(raw)
+    model = DecoderModel(arch.assemble(cfg))
+    bind_random(model, 1, torch.float32, torch.device("cpu"))
+    return ModelRunner(model, cfg, num_blocks=8, max_requests=2)
+
+
+class Stepper:
+    """A step that lasts until it is let go."""
+
+    def __init__(self):
+        self.begun, self.let_go, self.inside = threading.Event(), threading.Event(), False
+
+    def step(self, entries, device_tokens=None):
+        self.inside = True
+        self.begun.set()
+        assert self.let_go.wait(20)
+        self.inside = False
+
+
+def in_thread(f, *args):
+    t = threading.Thread(target=f, args=args, daemon=True)
+    t.start()
+    return t
+
+
+@pytest.mark.parametrize("what", ["load", "enable", "unload"])
+def test_banks_are_not_written_during_a_step(what, monkeypatch):
+    """A step may be recorded as a graph, which allocations of another thread spoil, and reads the banks."""
+    runner = cpu_runner(TINY["A"])
+    config, tensors = random_adapter("A", random_state_dict(TINY["A"], 1), 4, 1)
+    if what != "enable":
+        runner.enable_adapters(count=2, rank=8)
+        runner.load_adapter("first", tensors, config)
+    stepper = runner.stepper = Stepper()
+    stepper.adapter_count = 2
+    seen = []
+
+    def noted(name):
+        real = getattr(AdapterBank, name)
+        monkeypatch.setattr(AdapterBank, name, lambda self, *a, **kw: (seen.append(stepper.inside), real(self, *a, **kw))[1])
+
+    for name in ("__init__", "put", "clear"):
+        noted(name)
+    step = in_thread(runner.step, [])
+    assert stepper.begun.wait(20)
+    work = in_thread(*{"load": (runner.load_adapter, "second", tensors, config), "enable": (runner.enable_adapters, 2, 8),
+                       "unload": (runner.unload_adapter, "first")}[what])
+    work.join(0.5)
+    assert not any(seen)
+    stepper.let_go.set()
+    step.join(20)
+    work.join(20)
+    assert not work.is_alive() and seen and not any(seen)
