@@ -68,7 +68,10 @@ class ModelRunner:
         self.num_blocks = num_blocks
         self.block_size = block_size
         self._adapter_names: list[str | None] | None = None      # by index; None: adapters are off
-        self._adapter_lock = threading.RLock()                   # names and users: requests come from any thread
+        # Requests come from any thread and never wait for a load: names and users have a lock of their own, held for moments (the
+        # innermost one); whoever changes which adapters there are holds the outer one meanwhile.
+        self._adapter_lock = threading.RLock()
+        self._adapter_changes = threading.RLock()
         # A step, which may be recorded as a graph, or work on the adapters' banks by another thread: one after the other on the
         # host, and in that order on the device whatever streams the two are on.
         self._device_lock = threading.RLock()
@@ -149,7 +152,7 @@ class ModelRunner:
             raise ValueError(f"adapters of rank {rank}: at most 256")
         if count > 1024:
             raise ValueError(f"{count} adapters: at most 1024")
-        with self._adapter_lock:
+        with self._adapter_changes:
             if self._adapter_names is not None:
                 raise ValueError("adapters are enabled already")
             held = -(-rank // 8) * 8          # whole pieces of 16 bytes
@@ -160,9 +163,10 @@ class ModelRunner:
                 for p in parts:
                     p.banks = {q.name: AdapterBank(q, count, held, self.dtype, self.device) for q in p.adapted()}
                 self.stepper.adapter_count = count
-            self._adapter_names = [None] * count
-            self._adapter_users = [0] * count
-            self._adapter_rank = rank
+            with self._adapter_lock:
+                self._adapter_names = [None] * count
+                self._adapter_users = [0] * count
+                self._adapter_rank = rank
 
     def load_adapter(self, name: str, source, config: Mapping[str, Any] | None = None) -> int:
         """Load an adapter under ``name`` and return its index: ``source`` is a folder (``weights.read_adapter``), or the adapter's
@@ -189,7 +193,7 @@ class ModelRunner:
                                   + "; ".join(filter(None, [f"no product that takes adapters: {unknown}" if unknown else "",
                                                             f"sizes (expected, found): {wrong}" if wrong else ""])),
                                   unexpected=unknown, mismatched=wrong)
-        with self._adapter_lock:
+        with self._adapter_changes:
             if self._adapter_names is None:
                 self.enable_adapters(rank=rank)
             if rank > self._adapter_rank:
@@ -205,25 +209,28 @@ class ModelRunner:
                         mine = {local: matrices[p.spec.tensor_name(local)] for local in q.tensors
                                 if p.spec.tensor_name(local) in matrices}
                         p.banks[q.name].put(index, mine, scale)
-            self._adapter_names[index] = name
+            with self._adapter_lock:
+                self._adapter_names[index] = name
             return index
 
     def unload_adapter(self, name: str) -> None:
         """Give an adapter's place back; refused while requests use it."""
-        with self._adapter_lock:
-            index = self.adapter_index(name)
-            if self._adapter_users[index]:
-                raise ValueError(f"adapter {name!r} is in use by {self._adapter_users[index]} requests")
+        with self._adapter_changes:
+            with self._adapter_lock:
+                index = self.adapter_index(name)
+                if self._adapter_users[index]:
+                    raise ValueError(f"adapter {name!r} is in use by {self._adapter_users[index]} requests")
+                self._adapter_names[index] = None         # (nobody may take it up any more; the place is given out behind this)
             with self._between_steps(), torch.inference_mode():
                 for p in self.model.all_parts():
                     for bank in (p.banks or {}).values():
                         bank.clear(index)
-            self._adapter_names[index] = None
 
     def adapter_index(self, name: str) -> int:
-        if self._adapter_names is None or name is None or name not in self._adapter_names:
-            raise ValueError(f"no adapter {name!r} is loaded")
-        return self._adapter_names.index(name)
+        with self._adapter_lock:
+            if self._adapter_names is None or name is None or name not in self._adapter_names:
+                raise ValueError(f"no adapter {name!r} is loaded")
+            return self._adapter_names.index(name)
 
     def hold_adapter(self, name: str) -> int:
         """The adapter's index, for a request that uses it until ``release_adapter``."""

@@ -68,3 +68,50 @@ def test_banks_are_not_written_during_a_step(what, monkeypatch):
     step.join(20)
     work.join(20)
     assert not work.is_alive() and seen and not any(seen)
+
+
+def test_requests_come_and_go_while_an_adapter_is_loaded(monkeypatch):
+    runner = cpu_runner(TINY["A"])
+    config, tensors = random_adapter("A", random_state_dict(TINY["A"], 1), 4, 1)
+    runner.enable_adapters(count=3, rank=8)
+    runner.load_adapter("first", tensors, config)
+    begun, let_go, real = threading.Event(), threading.Event(), AdapterBank.put
+
+    def slow(self, *a, **kw):
+        begun.set()
+        assert let_go.wait(20)
+        real(self, *a, **kw)
+
+    monkeypatch.setattr(AdapterBank, "put", slow)
+    load = in_thread(runner.load_adapter, "second", tensors, config)
+    assert begun.wait(20)
+    held = []
+    user = in_thread(lambda: held.append(runner.hold_adapter("first")))
+    user.join(5)
+    assert held == [0]
+    runner.release_adapter(0)
+    with pytest.raises(ValueError, match="no adapter 'second'"):      # not before all of it is there
+        runner.hold_adapter("second")
+    let_go.set()
+    load.join(20)
+    assert runner.hold_adapter("second") == 1
+
+
+def test_a_failed_load_leaves_its_place_free(monkeypatch):
+    runner = cpu_runner(TINY["A"])
+    config, tensors = random_adapter("A", random_state_dict(TINY["A"], 1), 4, 1)
+    runner.enable_adapters(count=1, rank=8)
+    real, calls = AdapterBank.put, []
+
+    def fails(self, *a, **kw):
+        calls.append(self)
+        if len(calls) == 2:
+            raise RuntimeError("out of memory")
+        real(self, *a, **kw)
+
+    monkeypatch.setattr(AdapterBank, "put", fails)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        runner.load_adapter("x", tensors, config)
+    with pytest.raises(ValueError, match="no adapter"):
+        runner.adapter_index("x")
+    assert runner.load_adapter("x", tensors, config) == 0
