@@ -160,8 +160,10 @@ class ModelRunner:
             if not parts:
                 raise ValueError("no part of this model takes adapters")
             with self._between_steps():
-                for p in parts:
-                    p.banks = {q.name: AdapterBank(q, count, held, self.dtype, self.device) for q in p.adapted()}
+                # (all of them or, where memory runs out, none)
+                banks = [{q.name: AdapterBank(q, count, held, self.dtype, self.device) for q in p.adapted()} for p in parts]
+                for p, mine in zip(parts, banks):
+                    p.banks = mine
                 self.stepper.adapter_count = count
             with self._adapter_lock:
                 self._adapter_names = [None] * count

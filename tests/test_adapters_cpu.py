@@ -115,3 +115,21 @@ def test_a_failed_load_leaves_its_place_free(monkeypatch):
     with pytest.raises(ValueError, match="no adapter"):
         runner.adapter_index("x")
     assert runner.load_adapter("x", tensors, config) == 0
+
+
+def test_room_that_cannot_be_made_leaves_adapters_off(monkeypatch):
+    runner = cpu_runner(TINY["A"])
+    real, calls = AdapterBank.__init__, []
+
+    def fails(self, *a, **kw):
+        calls.append(self)
+        if len(calls) == 3:
+            raise RuntimeError("out of memory")
+        real(self, *a, **kw)
+
+    monkeypatch.setattr(AdapterBank, "__init__", fails)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        runner.enable_adapters(count=2, rank=8)
+    assert all(p.banks is None for p in runner.model.all_parts()) and runner.stepper.adapter_count == 0
+    runner.enable_adapters(count=2, rank=8)
+    assert runner.stepper.adapter_count == 2
