@@ -187,6 +187,8 @@ class ModelRunner:
             for q in p.adapted():
                 for local, width in zip(q.tensors, q.widths):
                     takes[p.spec.tensor_name(local)] = (width, q.inputs)
+        # (an adapter's files never say whether the tensor's own name ends in ".weight")
+        matrices = {n if n in takes else n.removesuffix(".weight") if n.removesuffix(".weight") in takes else n: m for n, m in matrices.items()}
         unknown = sorted(n for n in matrices if n not in takes)
         wrong = sorted((n, takes[n], (b.shape[0], a.shape[1])) for n, (a, b) in matrices.items()
                        if n in takes and takes[n] != (b.shape[0], a.shape[1]))

@@ -133,3 +133,37 @@ def test_room_that_cannot_be_made_leaves_adapters_off(monkeypatch):
     assert all(p.banks is None for p in runner.model.all_parts()) and runner.stepper.adapter_count == 0
     runner.enable_adapters(count=2, rank=8)
     assert runner.stepper.adapter_count == 2
+
+
+def gated_mlp_adapter(cfg, rank, salt, prefix=""):
+    """``(config, tensors)`` for the dense feed-forwards of a model whose tensors have no ``.weight`` in their names."""
+    g = torch.Generator().manual_seed(salt)
+    H, tensors = cfg["width"], {}
+    for i, layer in enumerate(cfg["layers"]):
+        if layer.get("mlp") and layer["mlp"]["kind"] == "dense":
+            ff = layer["mlp"]["ff"]
+            for name, out, inp in (("gate", ff, H), ("up", ff, H), ("down", H, ff)):
+                tensors[f"{prefix}l{i}.mlp.{name}.lora_A.weight"] = torch.randn(rank, inp, generator=g) * inp ** -0.5
+                tensors[f"{prefix}l{i}.mlp.{name}.lora_B.weight"] = torch.randn(out, rank, generator=g) * rank ** -0.5
+    return {"r": rank, "lora_alpha": 2 * rank}, tensors
+
+
+@pytest.mark.parametrize("family", ["lilulix", "ruburax"])
+def test_an_adapter_finds_tensors_with_plain_names(family):
+    import importlib
+
+    for which, raw in importlib.import_module(family + "_configs").CONFIGS.items():
+        runner = cpu_runner(raw)
+        for name, prefix in (("x", ""), ("y", "base_model.model.")):
+            config, tensors = gated_mlp_adapter(raw, 4, 7, prefix)
+            index = runner.load_adapter(name, tensors, config)
+            found = 0
+            for i, block in enumerate(runner.model.blocks):
+                ff = block.feed_forward
+                if not ff.adapted():
+                    continue
+                a = tensors[f"{prefix}l{i}.mlp.up.lora_A.weight"]
+                assert torch.equal(ff.banks["gate_up"].a[index, 1, :4], a)
+                assert torch.equal(ff.banks["down"].b[index, :, :4], tensors[f"{prefix}l{i}.mlp.down.lora_B.weight"])
+                found += 3
+            assert found and 2 * found == len(tensors)
