@@ -43,20 +43,24 @@ def pair_matrices(state: Mapping[str, torch.Tensor]) -> dict[str, tuple[torch.Te
     """``{model tensor name: (A, B)}`` from an adapter's tensors; everything that does not fit is named in one error."""
     sides: dict[str, dict[str, torch.Tensor]] = {}
     strange: list[str] = []
+    twice: list[str] = []
     for name, t in state.items():
         m = _NAME.match(name)
         if m is None or t.dim() != 2:
             strange.append(name)
+        elif m["side"] in sides.get(m["tensor"] + ".weight", ()):
+            twice.append(name)
         else:
             sides.setdefault(m["tensor"] + ".weight", {})[m["side"]] = t
     single = sorted(n for n, s in sides.items() if len(s) != 2)
     ranks = sorted(n for n, s in sides.items() if len(s) == 2 and s["A"].shape[0] != s["B"].shape[1])
-    if strange or single or ranks or not sides:
+    if strange or twice or single or ranks or not sides:
         raise WeightLoadError("; ".join(filter(None, [
             "an adapter without matrices" if not sides and not strange else "",
             f"not an adapter's matrices: {sorted(strange)}" if strange else "",
+            f"given twice, under other names: {sorted(twice)}" if twice else "",
             f"one matrix of two: {single}" if single else "",
-            f"matrices of different ranks: {ranks}" if ranks else ""])), unexpected=strange, missing=single, mismatched=ranks)
+            f"matrices of different ranks: {ranks}" if ranks else ""])), unexpected=strange + twice, missing=single, mismatched=ranks)
     return {n: (s["A"], s["B"]) for n, s in sides.items()}
 
 

@@ -10,7 +10,7 @@ from mini_infer_b200.config.registry import load_config
 from mini_infer_b200.engine.runner import ModelRunner
 from mini_infer_b200.parts.adapters import AdapterBank
 from mini_infer_b200.parts.model import DecoderModel
-from mini_infer_b200.weights import bind_random, random_state_dict
+from mini_infer_b200.weights import WeightLoadError, bind_random, pair_matrices, random_state_dict
 from tiny_configs import TINY
 
 
@@ -167,3 +167,12 @@ def test_an_adapter_finds_tensors_with_plain_names(family):
                 assert torch.equal(ff.banks["down"].b[index, :, :4], tensors[f"{prefix}l{i}.mlp.down.lora_B.weight"])
                 found += 3
             assert found and 2 * found == len(tensors)
+
+
+def test_a_matrix_given_twice_is_refused():
+    a, b = torch.zeros(4, 6), torch.zeros(5, 4)
+    once = {"x.lora_A.weight": a, "x.lora_B.weight": b}
+    assert set(pair_matrices(once)) == {"x.weight"}
+    for again in ("x.lora_A.default.weight", "base_model.model.x.lora_A.weight", "base_model.model.x.lora_B.default.weight"):
+        with pytest.raises(WeightLoadError, match="given twice"):
+            pair_matrices({**once, again: torch.ones(4, 6)})
