@@ -172,8 +172,8 @@ class ModelRunner:
 
     def load_adapter(self, name: str, source, config: Mapping[str, Any] | None = None) -> int:
         """Load an adapter under ``name`` and return its index: ``source`` is a folder (``weights.read_adapter``), or the adapter's
-        tensors by name with ``config`` (``r``, ``lora_alpha``).  Adapters need not be enabled before: room for eight of this
-        one's rank is then made."""
+        tensors by name with ``config`` (``r``, the rank of all its matrices, and ``lora_alpha``).  Adapters need not be enabled
+        before: room for eight of this one's rank is then made."""
         if isinstance(source, (str, os.PathLike)):
             if config is not None:
                 raise ValueError("a folder brings its own configuration")
@@ -181,7 +181,10 @@ class ModelRunner:
         if config is None:
             raise ValueError("an adapter's tensors need its configuration")
         matrices, scale = pair_matrices(source), adapter_scale(config)
-        rank = max(a.shape[0] for a, _ in matrices.values())
+        rank = int(config["r"])
+        others = sorted(n for n, (a, _) in matrices.items() if a.shape[0] != rank)
+        if others:
+            raise WeightLoadError(f"adapter {name!r}: r is {rank}, matrices of other ranks: {others}", mismatched=others)
         takes: dict[str, tuple[int, int]] = {}
         for p in self.model.all_parts():
             for q in p.adapted():

@@ -169,6 +169,17 @@ def test_an_adapter_finds_tensors_with_plain_names(family):
             assert found and 2 * found == len(tensors)
 
 
+def test_a_configuration_of_another_rank_is_refused():
+    """The scale is lora_alpha / r: with another r than the matrices' it would be another number."""
+    runner = cpu_runner(TINY["A"])
+    config, tensors = random_adapter("A", random_state_dict(TINY["A"], 1), 8, 1)
+    for r in (4, 16):
+        with pytest.raises(WeightLoadError, match="r is"):
+            runner.load_adapter("x", tensors, {**config, "r": r})
+    assert runner.stepper.adapter_count == 0                      # (and no room was made for it)
+    assert runner.load_adapter("x", tensors, config) == 0
+
+
 def test_a_matrix_given_twice_is_refused():
     a, b = torch.zeros(4, 6), torch.zeros(5, 4)
     once = {"x.lora_A.weight": a, "x.lora_B.weight": b}
