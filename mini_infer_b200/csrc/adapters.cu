@@ -83,13 +83,14 @@ __device__ __forceinline__ uint4 first_of(uint4 v, int n) {
   return v;
 }
 
-// A sum of the first product as two bfloat16 numbers, h = hi + lo: what is left of it is up to 2^-16 of it, below what the result's
-// own rounding leaves.  The second product takes both.
+// A sum of the first product as two bfloat16 numbers, h = hi + lo, both of its sign: hi is h cut off behind 8 bits, lo the rest, rounded.
+// What is left is up to 2^-16 of h (a rest below 2^-7 of h's power of two, by half a step of its 8 bits), below what the result's
+// own rounding leaves.  The second product takes both; where an element of B is infinite they have to say the same, so that lo is never of
+// the other sign, nor zero beside a hi that is not: 2^-18 of it is in its place (a sum below 2^-115 aside, which has none).
 __device__ __forceinline__ void split_bf16(float v, bf16& hi, bf16& lo) {
-  hi = __float2bfloat16_rn(v);
-  // (an infinite value has no rest: inf - inf would make it NaN)
-  const float rest = v - __bfloat162float(hi);
-  lo = __float2bfloat16_rn(isinf(v) || isinf(__bfloat162float(hi)) ? 0.f : rest);
+  hi = __float2bfloat16_rz(v);
+  const float whole = __bfloat162float(hi), rest = v - whole;
+  lo = __float2bfloat16_rn(rest == 0.f || isinf(v) ? whole * 0x1p-18f : rest);
 }
 
 // The stride, in elements, of a token's row of h in shared memory: whole groups of 32 k, and 64 bytes off a multiple of 128,
