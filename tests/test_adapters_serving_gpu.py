@@ -103,3 +103,44 @@ def test_a_step_waits_for_banks_written_on_another_stream(model_dirs):
         got = got[0].double().cpu()
         near, far = ((got - want[a]).norm() / want[a].norm() for a in (adapted, not adapted))
         assert near < 1e-4 and far > 1e-2
+
+
+@pytest.mark.parametrize("cuda_graph", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_request_without_an_adapter_beside_one_with(dtype, cuda_graph, model_dirs):
+    """Its logits have the same bits in float32 whether or not its neighbour has an adapter.  In bfloat16 they may round otherwise: few
+    rows finish a branch, and the gate, in a product's epilogue in fp32, and behind an adapter from its bfloat16 result.  Both are as
+    near to the formula as any step, and no further from one another."""
+    import numpy as np
+
+    import trace_util as T
+    from mini_infer_b200.engine import StepEntry
+
+    state = load_state(model_dirs["C"])
+    config, tensors = random_adapter("C", state, 16, 7)
+    mine, other = prompt_ids("C", 12, salt=71), prompt_ids("C", 10, salt=72)
+    runner = runner_of(model_dirs, "C", dtype=dtype, cuda_graph=cuda_graph)
+    runner.enable_adapters(count=2, rank=16)
+    runner.load_adapter("x", tensors, config)
+    cuts = [slice(0, 3), slice(3, 6), *(slice(i, i + 1) for i in range(6, 12))]
+    got = {}
+    for adapter in (-1, 0):
+        rows = []
+        for rid in "ab":
+            runner.add_request(rid)
+        for c in cuts:
+            theirs = (other + other)[c]
+            entries = [StepEntry("a", mine[c], list(range(len(mine[c])))), StepEntry("b", theirs, list(range(len(theirs))), adapter)]
+            result = runner.step(entries)
+            rows += [row.clone() for (rid, _), row in zip(result.rows, result.logits.double()) if rid == "a"]
+        for rid in "ab":
+            runner.free_request(rid)
+        got[adapter] = torch.stack(rows).cpu()
+    if dtype == "float32":
+        assert torch.equal(got[-1], got[0])
+        return
+    want = P.llama_logits(state, TINY["C"], mine).numpy()
+    tol = T.tolerance(dtype, float(np.abs(want).max()))
+    for z in got.values():
+        assert T.first_bad(z.numpy(), want, tol) is None
+    assert T.first_bad(got[0].numpy(), got[-1].numpy(), tol) is None
