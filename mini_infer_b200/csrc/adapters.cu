@@ -132,8 +132,9 @@ inline int count_chunks(const AdapterArgs& g, int size) {
 }
 
 // Items are up to 8 rows that share an adapter (or have none).  For up to FEW_MAX rows, one to a thread, every block finds the items in the
-// ids; for more, adapter_plan has put the rows in order.  256 rows without a plan and with one, on tcgen05 (us): 32 adapters of rank
-// 16 at 4096 x 6144 17.5 and 39.7, 4 of them 17.2 and 22.4, 4 of rank 64 at 4096 x 28672 37.8 and 40.4.
+// ids; for more, adapter_plan has put the rows in order.  FEW_MAX is what the threads of a block look through at once; more would take them
+// several turns, and where it would no longer pay has not been measured.  256 rows without a plan and 257 with one, on tcgen05 (us): 32
+// adapters of rank 16 at 4096 x 6144 17 and 36, 4 of them 17 and 21, 32 of rank 64 at 4096 x 28672 43 and 98, 4 of them 33 and 32.
 
 #define TILE_THREADS 256
 #define TILE_WARPS (TILE_THREADS / 32)
@@ -925,13 +926,14 @@ __host__ __device__ inline int add_stage_bytes(int R) { return b_atoms(R) * TC_A
 //                        rows).  y lies in rows of 256 bytes, 16-byte pieces permuted by the row, so that both ways touch all banks.
 //
 // Bound by memory in long calls: a tile takes 1.6 us of a block, 1.5 us are its bytes at a copy's rate (8192 rows of ranks to 64 at
-// 4096 x 28672: 213 us for all kernels, of which this one is 175), in short ones by the 6 us until the first tile is there.  What a
+// 4096 x 28672: 219 us for all kernels, of which this one is some 180), in short ones by the 6 us until the first tile is there.  What a
 // warp does for a tile is a chain of latencies, so that a thread's numbers and its y are all asked for at once and a stage is given back
-// before the stores (together 253 us become 213); the first items and their ranks are looked up while tensor memory is allocated
+// before the stores (with a sum as one number, 253 us became 213); the first items and their ranks are looked up while tensor memory is allocated
 // (2048 rows of rank 16 at 4096 x 4096 33 us become 31).
 //
-// Copies gather (rows of an item lie anywhere), which a tensor map does not; a copy warp says that a tile is there once its own
-// copies have landed and are visible to the tensor cores.
+// Copies are cp.async of 16 bytes, a thread's addresses once an item: rows of an item lie anywhere.  (Tensor copies that gather four rows
+// at a time have not been tried.)  A copy warp says that a tile is there once its own copies have landed and are visible to the tensor
+// cores.
 #define A1_SUM_WARPS 8
 #define A1_COPY_WARPS 4
 #define A1_COPY_THREADS (32 * A1_COPY_WARPS)
@@ -1439,7 +1441,8 @@ static Route route_of(const void* y, long long ldy, const void* x, long long ldx
                       long long ldo, int M, int N, int K, int n, int P, int R, const int* ends, int pairs, int dtype) {
   Route r = {BY_ELEMENTS, 0, 1, (long long)M * P * R, 0};
   r.items = M <= FEW_MAX ? (M < n + 1 + M / FEW_ROWS ? M : n + 1 + M / FEW_ROWS) : plan_items(M, n) * (MAX_ROWS / FEW_ROWS);
-  // The tensor-core kernels take rows of x, A and B in pieces of 16 bytes.
+  // The tensor-core kernels take rows of x, A and B in pieces of 16 bytes.  mma.sync and CUDA cores, 4 adapters at 4096 x 6144 (us): rank 16,
+  // 256 rows 17 and 51; rank 200, 256 rows 48 and 397, 257 over a plan 49 and 375, 2048 272 and 2580.
   if (dtype != MI_DTYPE_BF16 || n <= 0 || R <= 0 || R > 256 || K <= 0 || R % 8 || K % 8 || !mi_aligned(a, 16) ||
       !mi_aligned(b, 16) || !mi_aligned(x, 16) || (M > 1 && ldx % 8)) {
     // Parts of the sum over K follow from K alone, so that float32 rows have the same bits in whatever company.  Rank 16, 4096 x 6144, parts of
@@ -1452,6 +1455,9 @@ static Route route_of(const void* y, long long ldy, const void* x, long long ldx
   }
   bool whole = N % 8 == 0 && mi_aligned(y, 16) && mi_aligned(out, 16) && (M == 1 || (ldy % 8 == 0 && ldo % 8 == 0));
   for (int p = 0; p + 1 < P && !pairs; ++p) whole = whole && ends[p] % 8 == 0;
+  // Over a plan, tcgen05 and mma.sync (us): 4 adapters of rank 16 at 4096 x 6144, 257 rows 20.8 and 19.0, 512 22 and 22, 2048 32 and 51;
+  // 32 of them 36.4 and 34.6, 37 and 39, 45 and 69; 4 of rank 64 at 4096 x 28672 32 and 46, 36 and 77, 83 and 251; 32 of them 98 and 100,
+  // 101 and 126, 117 and 298.
   if (M > FEW_MAX && whole && R <= 128) {
     r.way = BY_MANY;
     r.items = plan_items(M, n);

@@ -69,9 +69,9 @@ class Request:
     sampling_params: SamplingParams = dataclasses.field(default_factory=SamplingParams)
     max_tokens: int = 16
     adapter: str | None = None      # name of a low-rank adapter that the runner has loaded
-    # a grammar: given the tokens generated so far, the ids of the tokens that may come next, or their bits (a numpy int32
-    # array of ceil(V / 32) words); None: any token.  No token at all ends the request as "stop", an exception as "cancelled"
-    # (with a warning; other requests go on).
+    # a grammar: given the tokens generated so far, the ids of the tokens that may come next, or their bits (a numpy array of
+    # int32, which is always ceil(V / 32) words of bits); None: any token.  No token at all ends the request as "stop", an
+    # exception as "cancelled" (with a warning; other requests go on).  While the request lives no step is launched ahead.
     token_mask: Callable[[list[int]], Any] | None = None
 
 

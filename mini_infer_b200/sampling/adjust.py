@@ -1,7 +1,8 @@
 """What requests ask of their logits before a token is chosen, on the device (the kernels are ``csrc/logits.cu``).
 
-``LogitsAdjuster`` keeps the token histories that penalties read, one slot per request that asks for one, and the masks of requests whose
-tokens are limited for good.  ``apply`` changes a step's logits in place; ``record`` puts the tokens that were chosen into the
+``LogitsAdjuster`` keeps the token histories that penalties read, on the device, one slot per request that asks for one, and on the host the
+masks of requests whose tokens are limited for good.  ``apply`` changes a step's logits in place (options, biases and masks go to the device
+with every step, in one copy); ``record`` puts the tokens that were chosen into the
 histories, on the device and in stream order, so that the next step may be launched before the host has seen them.
 """
 
