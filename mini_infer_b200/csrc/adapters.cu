@@ -873,8 +873,9 @@ __global__ void __launch_bounds__(TC_THREADS) adapter_sums_tc_kernel(const Adapt
 }
 
 // A part's sums for the second product, two bfloat16 numbers each as with few rows: whole groups of 16 k, and behind them their rests.
-// In tensor memory they cost no stage of the ring, and the products, twice as many, hide behind the tiles' bytes: 8192 rows of ranks to
-// 64 at 4096 x 28672 219 us, with one number a sum 214, at 4096 x 6144 106 and 105.
+// In tensor memory they cost no stage of the ring, and the products, twice as many, mostly hide behind the tiles' bytes: 8192 rows of
+// rank 64 at 4096 x 28672 219 us, with one number a sum 213, at 4096 x 6144 106 and 104; in a long loop of calls with other inputs each 239
+// and 228 (230 with the rests' products left out).
 __host__ __device__ inline int padded_rank(int R) { return (R + 15) & ~15; }
 __host__ __device__ inline int held_sums(int R) { return 2 * padded_rank(R); }
 
