@@ -65,7 +65,7 @@ def test_adapters_are_loaded_and_unloaded_while_steps_are_captured(model_dirs):
             loader.join(60)
         sched.stop()
     assert not failures and rounds > 0
-    assert {k for k in runner.stepper._graphs if len(k) == 2} >= {(1, "adapters"), (4, "adapters")}
+    assert any(len(k) == 2 and slot.replays for k, slot in runner.stepper._graphs.items())
 
 
 def test_a_step_waits_for_banks_written_on_another_stream(model_dirs):
