@@ -2,8 +2,8 @@
 
 A folder holds ``adapter_config.json`` (``r``, ``lora_alpha``, optional ``use_rslora``) and ``adapter_model.safetensors`` with two
 matrices per adapted tensor of the model, ``<tensor>.lora_A.weight [r, inputs]`` and ``<tensor>.lora_B.weight [outputs, r]``, where
-``<tensor>`` is the model's name, without ``.weight`` if it ends so, maybe behind ``base_model.model.``.  What is added to a product is ``s B (A x)``
-with ``s = lora_alpha / r`` (``lora_alpha / sqrt(r)`` with ``use_rslora``).
+``<tensor>`` is the model's name, without ``.weight`` if it ends so, maybe behind ``base_model.model.``.  What is added to a product is
+``s B (A x)`` with ``s = lora_alpha / r`` (``lora_alpha / sqrt(r)`` with ``use_rslora``); all matrices have rank ``r``.
 """
 
 from __future__ import annotations
